@@ -184,3 +184,12 @@ def qsgd_dequantize(levels: torch.Tensor, norms: torch.Tensor, quantum_num: int,
 
 pack_bitarray = _ref.pack_bitarray
 unpack_bitarray = _ref.unpack_bitarray
+
+from .language import (  # noqa: E402,F401
+    attention,
+    clip_grad_norm,
+    clip_grad_norm_,
+    grad_norm,
+    rotary,
+    rotary_frequencies,
+)

@@ -143,3 +143,101 @@ def qsgd_dequantize(levels: torch.Tensor, norms: torch.Tensor, quantum_num: int,
     l = torch.nn.functional.pad(levels.float(), (0, pad)).view(nb, bucket_size)
     v = norms.unsqueeze(1) / quantum_num * l
     return v.reshape(-1)[:n].contiguous()
+
+
+# --------------------------------------------------------------------------
+# language-model operators
+# --------------------------------------------------------------------------
+
+def _attention_parts(q, k, documents, slopes, causal, scale):
+    """(scores [B, Hq, Sq, Sk] in 32 bits, where they are visible)."""
+    sq, sk, group = q.shape[1], k.shape[1], q.shape[2] // k.shape[2]
+    qf = q.float().transpose(1, 2)
+    kf = k.float().transpose(1, 2).repeat_interleave(group, 1)
+    s = torch.matmul(qf, kf.transpose(2, 3)) * scale
+    p = torch.arange(sk - sq, sk, device=q.device).unsqueeze(1)
+    j = torch.arange(sk, device=q.device).unsqueeze(0)
+    if slopes is not None:
+        s = s - slopes.view(1, -1, 1, 1) * (p - j).abs()
+    seen = torch.ones(q.shape[0], 1, sq, sk, dtype=torch.bool, device=q.device)
+    if causal:
+        seen = seen & (j <= p)
+    if documents is not None:
+        key = documents[:, None, None, :]
+        seen = seen & (documents[:, None, sk - sq:, None] == key) & (key >= 0)
+    return s, seen.expand(s.shape)
+
+
+def _masked_product(w, x, seen):
+    """w @ x where w is 0 outside `seen`: what x holds there stays out."""
+    if bool(torch.isfinite(x).all()):
+        return torch.matmul(w, x)
+    y = torch.zeros(*w.shape[:-1], x.shape[-1], device=x.device)
+    for j in range(x.shape[-2]):
+        term = w[..., j:j + 1] * x[..., j:j + 1, :]
+        y += torch.where(seen[..., j:j + 1], term, torch.zeros_like(term))
+    return y
+
+
+def attention_forward(q, k, v, documents, slopes, causal, scale, want_lse):
+    s, seen = _attention_parts(q, k, documents, slopes, causal, scale)
+    s = s.masked_fill(~seen, float("-inf"))
+    lse = torch.logsumexp(s, -1) if s.shape[-1] else s.sum(-1) - float("inf")
+    base = torch.where(lse == float("-inf"), torch.zeros_like(lse), lse)
+    p = torch.where(seen, torch.exp(s - base.unsqueeze(-1)), torch.zeros_like(s))
+    vf = v.float().transpose(1, 2).repeat_interleave(q.shape[2] // v.shape[2], 1)
+    out = _masked_product(p, vf, seen).transpose(1, 2).contiguous().to(q.dtype)
+    return out, lse if want_lse else None
+
+
+def attention_backward(dout, q, k, v, out, lse, documents, slopes, causal, scale):
+    s, seen = _attention_parts(q, k, documents, slopes, causal, scale)
+    group = q.shape[2] // k.shape[2]
+    seen = seen & (lse != float("-inf")).unsqueeze(-1)
+    zero = torch.zeros_like(s)
+    p = torch.where(seen, torch.exp(s - lse.unsqueeze(-1)), zero)
+    qf, do = q.float().transpose(1, 2), dout.float().transpose(1, 2)
+    kf, vf = (t.float().transpose(1, 2).repeat_interleave(group, 1) for t in (k, v))
+    delta = (do * out.float().transpose(1, 2)).sum(-1, keepdim=True)
+    ds = torch.where(seen, p * (torch.matmul(do, vf.transpose(2, 3)) - delta), zero)
+    dq = _masked_product(ds, kf, seen) * scale
+    back = seen.transpose(2, 3)
+    dk = _masked_product(ds.transpose(2, 3), qf, back) * scale
+    dv = _masked_product(p.transpose(2, 3), do, back)
+    dk, dv = (t.unflatten(1, (k.shape[2], group)).sum(2) for t in (dk, dv))
+    return [t.transpose(1, 2).to(q.dtype) for t in (dq, dk, dv)]
+
+
+def rotary(xs, positions, frequencies, interleaved, inverse):
+    angle = positions.double().unsqueeze(-1) * frequencies
+    cos, sin = angle.cos().float().unsqueeze(2), angle.sin().float().unsqueeze(2)
+    if inverse:
+        sin = -sin
+    n = frequencies.numel()
+    outs = []
+    for x in xs:
+        y = x.float()
+        if interleaved:
+            a, b = y[..., 0:2 * n:2], y[..., 1:2 * n:2]
+            turned = torch.stack((a * cos - b * sin, a * sin + b * cos), -1).flatten(-2)
+        else:
+            a, b = y[..., :n], y[..., n:2 * n]
+            turned = torch.cat((a * cos - b * sin, a * sin + b * cos), -1)
+        outs.append(torch.cat((turned.to(x.dtype), x[..., 2 * n:]), -1))
+    return outs
+
+
+def _square_sum(grads) -> torch.Tensor:
+    return torch.stack([t.double().square().sum() for t in grads]).sum()
+
+
+def grad_norm(grads) -> torch.Tensor:
+    return _square_sum(grads).sqrt().float()
+
+
+def clip_grad_norm(grads, outs, max_norm: float) -> torch.Tensor:
+    norm = _square_sum(grads).sqrt()
+    factor = torch.where(norm <= max_norm, torch.ones_like(norm), max_norm / norm)
+    for t, o in zip(grads, outs):
+        o.copy_(t.double() * factor)
+    return norm.float()

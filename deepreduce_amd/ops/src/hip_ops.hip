@@ -21,6 +21,8 @@
 #include <algorithm>
 #include <vector>
 
+#include "lm_ops.h"
+
 #define WAVE 64
 #define CHECK_CUDA(x) TORCH_CHECK(x.is_cuda(), #x " must be a GPU tensor")
 
@@ -3244,4 +3246,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("pack_ints_cpu", &pack_ints_cpu, "n-bit pack (C++ CPU)");
     m.def("unpack_ints_cpu", &unpack_ints_cpu, "n-bit unpack (C++ CPU)");
     m.def("huffman_decode_cpu", &huffman_decode_cpu, "canonical Huffman decode (C++ CPU)");
+    m.def("grad_norm", &grad_norm, "global 2-norm of many tensors (HIP)");
+    m.def("clip_grad_norm", &clip_grad_norm,
+          "global 2-norm of many tensors, and the tensors scaled to at most max_norm (HIP)");
+    m.def("rotary", &rotary, "rotary positions of one or two tensors (HIP)");
+    m.def("attention_forward", &attention_forward,
+          "attention with documents, distance bias and causality -> (out, lse) (HIP)");
+    m.def("attention_backward", &attention_backward, "its gradient -> (dq, dk, dv) (HIP)");
 }

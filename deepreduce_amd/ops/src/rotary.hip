@@ -1,0 +1,234 @@
+// Rotary positions (gfx950): each pair (a, b) of a head's first `dim` values is
+// turned by the angle position * frequency,
+//
+//   (a, b) -> (a cos t - b sin t, a sin t + b cos t),
+//
+// pairs being (i, i + dim / 2) or, interleaved, (2 i, 2 i + 1); the values
+// behind `dim` are copied.  The gradient is the turn by -t.
+//
+// An angle depends on the token and the pair only, so a block computes the
+// sines of its tokens once, into shared memory, and uses them for all heads
+// of all tensors.  Angles are formed and reduced in 64 bits: position 1e6 has
+// an angle that 32 bits hold to 0.06.  The kernel is bound by the one read and
+// write of the heads.
+
+#include "lm_ops.h"
+
+#include <ATen/hip/HIPContext.h>
+#include <c10/core/DeviceGuard.h>
+#include <hip/hip_runtime.h>
+#include <algorithm>
+
+namespace {
+
+constexpr int THREADS = 256;
+constexpr int MOST_PAIRS = 2048;  // (cos, sin) of a block: 16 KB
+
+struct Heads {
+    const void* in;
+    void* out;              // [batch, length, heads, d], contiguous
+    int64_t sb, ss, sh;     // the input's strides, in values
+    int heads;
+};
+
+template <typename T, int V> struct Vec {
+    T v[V];
+};
+template <typename T, int V> struct alignas(sizeof(T) * V) Aligned : Vec<T, V> {};
+
+struct Args {
+    Heads x[2];
+    int tensors;
+    const void* positions;
+    int64_t pb, ps;         // the positions' strides
+    bool wide;              // positions are 64-bit
+    const double* frequencies;
+    int length, d, half;    // tokens of a row, head size, pairs
+    int64_t tokens;
+    int per_block;          // tokens of a block
+    float sign;             // -1: the turn back
+};
+
+template <typename T, int V, bool INTERLEAVED>
+__global__ __launch_bounds__(THREADS) void rotary_kernel(const Args a) {
+    __shared__ float2 turn[MOST_PAIRS];
+    int64_t first = (int64_t)blockIdx.x * a.per_block;
+    int tokens = (int)min((int64_t)a.per_block, a.tokens - first);
+    for (int i = threadIdx.x; i < tokens * a.half; i += THREADS) {
+        int64_t token = first + i / a.half;
+        int64_t b = token / a.length, s = token % a.length;
+        int64_t at = b * a.pb + s * a.ps;
+        double position = a.wide ? (double)((const int64_t*)a.positions)[at]
+                                 : (double)((const int*)a.positions)[at];
+        // quarters of a turn: what is left lies within an eighth of one
+        double quarters = position * a.frequencies[i % a.half] * 0.63661977236758134308;
+        double n = rint(quarters);
+        float sn, cs;
+        sincospif((float)(quarters - n) * 0.5f, &sn, &cs);
+        int q = (int)(n - 4.0 * floor(n * 0.25));
+        if (q & 1) {
+            float t = cs;
+            cs = -sn;
+            sn = t;
+        }
+        if (q & 2) cs = -cs, sn = -sn;
+        turn[i] = make_float2(cs, sn * a.sign);
+    }
+    __syncthreads();
+
+    using A = Aligned<T, V>;
+    // a work item turns V pairs (two vectors, or one with V / 2 pairs) or
+    // copies one vector behind them
+    const int turned = INTERLEAVED ? 2 * a.half / V : a.half / V;
+    const int per_head = turned + (a.d - 2 * a.half) / V;
+    for (int t = 0; t < a.tensors; ++t) {
+        const Heads& x = a.x[t];
+        const unsigned per_token = (unsigned)x.heads * per_head;
+        for (unsigned i = threadIdx.x; i < tokens * per_token; i += THREADS) {
+            unsigned tok = i / per_token, rest = i % per_token;
+            unsigned head = rest / per_head, slot = rest % per_head;
+            int64_t token = first + tok;
+            int64_t b = token / a.length, s = token % a.length;
+            const T* in = (const T*)x.in + b * x.sb + s * x.ss + head * x.sh;
+            T* out = (T*)x.out + (token * x.heads + head) * a.d;
+            if (slot >= (unsigned)turned) {
+                int at = 2 * a.half + (slot - turned) * V;
+                *(A*)(out + at) = *(const A*)(in + at);
+                continue;
+            }
+            const float2* w = turn + tok * a.half;
+            if constexpr (INTERLEAVED) {
+                A v = *(const A*)(in + slot * V), o;
+#pragma unroll
+                for (int e = 0; e < V / 2; ++e) {
+                    float2 c = w[slot * (V / 2) + e];
+                    float p = (float)v.v[2 * e], q = (float)v.v[2 * e + 1];
+                    o.v[2 * e] = (T)(p * c.x - q * c.y);
+                    o.v[2 * e + 1] = (T)(p * c.y + q * c.x);
+                }
+                *(A*)(out + slot * V) = o;
+            } else {
+                A v = *(const A*)(in + slot * V), u = *(const A*)(in + a.half + slot * V), o, r;
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                    float2 c = w[slot * V + e];
+                    float p = (float)v.v[e], q = (float)u.v[e];
+                    o.v[e] = (T)(p * c.x - q * c.y);
+                    r.v[e] = (T)(p * c.y + q * c.x);
+                }
+                *(A*)(out + slot * V) = o;
+                *(A*)(out + a.half + slot * V) = r;
+            }
+        }
+    }
+}
+
+template <typename T, int V>
+void launch(const Args& a, bool interleaved, int blocks, hipStream_t stream) {
+    if (interleaved) {
+        if constexpr (V > 1)
+            hipLaunchKernelGGL((rotary_kernel<T, V, true>), dim3(blocks), dim3(THREADS), 0,
+                               stream, a);
+    } else {
+        hipLaunchKernelGGL((rotary_kernel<T, V, false>), dim3(blocks), dim3(THREADS), 0, stream,
+                           a);
+    }
+}
+
+template <typename T>
+void launch_vec(const Args& a, int v, bool interleaved, int blocks, hipStream_t stream) {
+    switch (v) {
+        case 8:
+            if constexpr (sizeof(T) == 2) launch<T, 8>(a, interleaved, blocks, stream);
+            break;
+        case 4: launch<T, 4>(a, interleaved, blocks, stream); break;
+        case 2: launch<T, 2>(a, interleaved, blocks, stream); break;
+        default: launch<T, 1>(a, interleaved, blocks, stream); break;
+    }
+}
+
+}  // namespace
+
+std::vector<torch::Tensor> rotary(std::vector<torch::Tensor> xs, torch::Tensor positions,
+                                  torch::Tensor frequencies, bool interleaved, bool inverse) {
+    TORCH_CHECK(xs.size() >= 1 && xs.size() <= 2, "rotary takes one or two tensors");
+    const auto& x0 = xs[0];
+    c10::DeviceGuard guard(x0.device());
+    Args a{};
+    a.d = (int)x0.size(-1);
+    a.half = (int)frequencies.numel();
+    a.length = (int)x0.size(1);
+    a.tokens = x0.size(0) * x0.size(1);
+    TORCH_CHECK(frequencies.is_cuda() && frequencies.scalar_type() == torch::kFloat64 &&
+                    frequencies.dim() == 1 && frequencies.is_contiguous() &&
+                    frequencies.device() == x0.device(),
+                "frequencies must be a contiguous float64 vector on the tensors' device");
+    TORCH_CHECK(a.half >= 1 && 2 * a.half <= a.d && a.half <= MOST_PAIRS,
+                "frequencies turn more values than a head has");
+    TORCH_CHECK(positions.is_cuda() && positions.device() == x0.device() &&
+                    (positions.scalar_type() == torch::kInt64 ||
+                     positions.scalar_type() == torch::kInt32) &&
+                    positions.dim() == 2 && positions.size(0) == x0.size(0) &&
+                    positions.size(1) == x0.size(1),
+                "positions must be int32 or int64 [batch, length] on the tensors' device");
+    a.positions = positions.data_ptr();
+    a.pb = positions.stride(0);
+    a.ps = positions.stride(1);
+    a.wide = positions.scalar_type() == torch::kInt64;
+    a.frequencies = frequencies.data_ptr<double>();
+    a.sign = inverse ? -1.f : 1.f;
+    a.tensors = (int)xs.size();
+
+    // the widest vector that every address and extent is a multiple of
+    int size = (int)x0.element_size();
+    int v = 16 / size;
+    std::vector<torch::Tensor> outs;
+    int heads = 0;
+    for (size_t t = 0; t < xs.size(); ++t) {
+        auto& x = xs[t];
+        TORCH_CHECK(x.is_cuda() && x.dim() == 4 && x.device() == x0.device() &&
+                        x.scalar_type() == x0.scalar_type() && x.size(0) == x0.size(0) &&
+                        x.size(1) == x0.size(1) && x.size(3) == a.d,
+                    "rotary takes [batch, length, heads, d] tensors of one type");
+        if (x.stride(3) != 1 && a.d > 1) x = x.contiguous();
+        outs.push_back(torch::empty(x.sizes(), x.options()));
+        a.x[t] = {x.data_ptr(), outs[t].data_ptr(), x.stride(0), x.stride(1), x.stride(2),
+                  (int)x.size(2)};
+        heads += a.x[t].heads;
+        while (v > 1 && ((uintptr_t)x.data_ptr() % (v * size) || x.stride(0) % v ||
+                         x.stride(1) % v || x.stride(2) % v))
+            v /= 2;
+    }
+    while (v > 1 && (a.d % v || (interleaved ? 2 * a.half : a.half) % v)) v /= 2;
+    if (interleaved && v == 1) {
+        // pairs at odd addresses: a copy is aligned, and 2 divides its extents
+        // but for an odd head size
+        for (size_t t = 0; t < xs.size(); ++t) {
+            xs[t] = xs[t].contiguous();
+            a.x[t].in = xs[t].data_ptr();
+            a.x[t].sb = xs[t].stride(0);
+            a.x[t].ss = xs[t].stride(1);
+            a.x[t].sh = xs[t].stride(2);
+        }
+        TORCH_CHECK(a.d % 2 == 0, "interleaved pairs need an even head size");
+        v = 2;
+    }
+    if (a.tokens == 0 || heads == 0) return outs;
+
+    // A block's sines serve all its tokens' heads; tokens are shared out so
+    // that 8 blocks a CU have work first, and the sines fit.
+    int64_t per = std::max<int64_t>(1, a.tokens / 2048);
+    a.per_block = (int)std::min<int64_t>({per, (int64_t)8, (int64_t)(MOST_PAIRS / a.half)});
+    int64_t blocks = (a.tokens + a.per_block - 1) / a.per_block;
+    TORCH_CHECK(blocks <= INT_MAX, "too many tokens for one launch");
+    hipStream_t stream = at::hip::getCurrentHIPStream();
+    switch (x0.scalar_type()) {
+        case torch::kFloat32: launch_vec<float>(a, v, interleaved, (int)blocks, stream); break;
+        case torch::kBFloat16: launch_vec<__bf16>(a, v, interleaved, (int)blocks, stream); break;
+        case torch::kFloat16:
+            launch_vec<_Float16>(a, v, interleaved, (int)blocks, stream);
+            break;
+        default: TORCH_CHECK(false, "rotary takes float32, bfloat16 or float16");
+    }
+    return outs;
+}

@@ -20,8 +20,18 @@ setup(
     ext_modules=[
         CUDAExtension(
             name="deepreduce_amd._hip_ops",
-            sources=["deepreduce_amd/ops/src/hip_ops.hip"],
-            extra_compile_args={"cxx": ["-O3"], "nvcc": ["-O3"]},
+            sources=[
+                "deepreduce_amd/ops/src/hip_ops.hip",
+                "deepreduce_amd/ops/src/attention.hip",
+                "deepreduce_amd/ops/src/grad_norm.hip",
+                "deepreduce_amd/ops/src/rotary.hip",
+            ],
+            extra_compile_args={
+                "cxx": ["-O3"],
+                # packed float adds and products have given wrong results
+                # now and then: the compiler makes none
+                "nvcc": ["-O3", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"],
+            },
         )
     ],
     cmdclass={"build_ext": BuildExtension},
