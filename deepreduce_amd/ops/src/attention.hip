@@ -94,24 +94,30 @@ __device__ void forward_row(const Args& a, int b, int h, int i) {
     const int lane = threadIdx.x & 63, g = h / (a.hq / a.hkv), pos = i + a.sk - a.sq;
     const float slope = slope_of(a, h);
     const T* q = row<T>(a.q, b, i, h);
-    float top = -INFINITY, total = 0, o[2] = {0, 0};
     const int end = a.causal ? pos + 1 : a.sk;
+    auto score = [&](int j) {
+        return dot(q, row<T>(a.k, b, j, g), a.d) * (a.scale * LOG2E) - slope * abs(pos - j);
+    };
+    // the sum first: with whole probabilities no partial result passes the
+    // largest value
+    float top = -INFINITY, total = 0;
+    for (int j = lane; j < end; j += 64)
+        if (visible(a, b, pos, j)) {
+            float s = score(j), next = fmaxf(top, s);
+            float base = next == -INFINITY ? 0.f : next;
+            total = total * exp2_fast(top - base) + exp2_fast(s - base);
+            top = next;
+        }
+    float base = wave_max(top);
+    base = base == -INFINITY ? 0.f : base;
+    total = wave_sum(total * exp2_fast(top - base));
+    const float inv = total == 0.f ? 0.f : 1.f / total;
+    float o[2] = {0, 0};
     for (int j0 = 0; j0 < end; j0 += 64) {
         int j = j0 + lane;
         bool seen = j < end && visible(a, b, pos, j);
-        uint64_t any = __ballot(seen);
-        if (!any) continue;
-        float s = -INFINITY;
-        if (seen)
-            s = dot(q, row<T>(a.k, b, j, g), a.d) * (a.scale * LOG2E) - slope * abs(pos - j);
-        float next = fmaxf(top, wave_max(s));
-        float base = next == -INFINITY ? 0.f : next;
-        float keep = exp2_fast(top - base), p = seen ? exp2_fast(s - base) : 0.f;
-        top = next;
-        total = total * keep + wave_sum(p);
-        o[0] *= keep;
-        o[1] *= keep;
-        for (; any; any &= any - 1) {
+        float p = seen ? exp2_fast(score(j) - base) * inv : 0.f;
+        for (uint64_t any = __ballot(seen); any; any &= any - 1) {
             int n = __builtin_ctzll(any);
             float w = __shfl(p, n);
             const T* v = row<T>(a.v, b, j0 + n, g);
@@ -119,12 +125,11 @@ __device__ void forward_row(const Args& a, int b, int h, int i) {
             if (lane + 64 < a.d) o[1] = fmaf(w, (float)v[lane + 64], o[1]);
         }
     }
-    float inv = total == 0.f ? 0.f : 1.f / total;
     T* out = row<T>(a.out, b, i, h);
-    if (lane < a.d) out[lane] = (T)(total == 0.f ? 0.f : o[0] * inv);
-    if (lane + 64 < a.d) out[lane + 64] = (T)(total == 0.f ? 0.f : o[1] * inv);
+    if (lane < a.d) out[lane] = (T)o[0];
+    if (lane + 64 < a.d) out[lane + 64] = (T)o[1];
     if (lane == 0 && a.lse)
-        a.lse[((int64_t)b * a.hq + h) * a.sq + i] = total == 0.f ? -INFINITY : top + log2f(total);
+        a.lse[((int64_t)b * a.hq + h) * a.sq + i] = total == 0.f ? -INFINITY : base + log2f(total);
 }
 
 template <typename T>
@@ -237,6 +242,470 @@ void launch_rows(const Args& a, hipStream_t stream) {
 }
 
 // ---------------------------------------------------------------------------
+// Tiles on the matrix cores.  A fragment of a 32x32x16 product is 8 values a
+// lane: lane l holds row (or column) l % 32, k = (l / 32) * 8 + 0..7; of the
+// result it holds column l % 32 and rows 8 (i / 4) + 4 (l / 32) + i % 4.
+//
+// Scores are formed transposed, keys as rows and queries as columns.  A query
+// then lies in one lane and its other half, so its maximum and sum need one
+// exchange between lanes for a whole tile, and the lane's probabilities are,
+// in the order they come, the right operand of the product with V: k index
+// (l / 32) * 8 + j stands for key 8 (j / 4) + 4 (l / 32) + j % 4 on both
+// sides.  The left operand is V transposed, which the transposing read of
+// shared memory gives from rows as they lie in memory.
+// ---------------------------------------------------------------------------
+
+typedef float acc16 __attribute__((ext_vector_type(16)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+typedef short short4v __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+template <typename T> struct FragOf;
+template <> struct FragOf<__bf16> { typedef bf16x8 type; };
+template <> struct FragOf<_Float16> { typedef f16x8 type; };
+template <> struct FragOf<float> { typedef f32x8 type; };
+template <typename T> using Frag = typename FragOf<T>::type;
+
+__device__ __forceinline__ acc16 mma(bf16x8 a, bf16x8 b, acc16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ acc16 mma(f16x8 a, f16x8 b, acc16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+// 32-bit products have a k of 2, one value of each half of the wave: the 8
+// values of a fragment take 8 of them
+__device__ __forceinline__ acc16 mma(f32x8 a, f32x8 b, acc16 c) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], b[j], c, 0, 0, 0);
+    return c;
+}
+
+constexpr int RANGE = 64;            // positions whose documents share a range
+constexpr int NONE = 0x7fffffff;
+
+template <typename T, int DP> struct Tile {
+    static constexpr int PER = 16 / sizeof(T);
+    static constexpr int LD = DP + PER;  // rows 16 bytes apart of a multiple of the banks
+    static constexpr int VECS = DP / PER;
+    static constexpr int KEYS = sizeof(T) == 2 ? 64 : 32;
+};
+
+// Rows of one tile on their way from memory to shared memory, through
+// registers so that they travel while the tile before is worked on.
+template <typename T, int DP, int ROWS, int THREADS> struct Stage {
+    using G = Tile<T, DP>;
+    static constexpr int N = ROWS * G::VECS / THREADS;
+    static_assert(N * THREADS == ROWS * G::VECS, "threads share a tile's vectors evenly");
+    uint4 r[N];
+
+    __device__ __forceinline__ void load(const T* base, int64_t stride, int rows, int d) {
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            int v = threadIdx.x + n * THREADS, y = v / G::VECS, x = (v % G::VECS) * G::PER;
+            r[n] = make_uint4(0, 0, 0, 0);
+            if (y < rows && x < d) r[n] = *(const uint4*)(base + y * stride + x);
+        }
+    }
+    __device__ __forceinline__ void store(T* tile) const {
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            int v = threadIdx.x + n * THREADS, y = v / G::VECS, x = (v % G::VECS) * G::PER;
+            *(uint4*)(tile + y * G::LD + x) = r[n];
+        }
+    }
+};
+
+// rows y0 + l % 32 of a tile, values x0 + (l / 32) * 8 + 0..7
+template <typename T, int LD>
+__device__ __forceinline__ Frag<T> rows_of(const T* tile, int y0, int x0) {
+    const int lane = threadIdx.x & 63;
+    return *(const Frag<T>*)(tile + (y0 + (lane & 31)) * LD + x0 + (lane >> 5) * 8);
+}
+
+// columns x0 + l % 32, rows y0 + 8 (j / 4) + 4 (l / 32) + j % 4
+template <typename T, int LD>
+__device__ __forceinline__ Frag<T> columns_of(const T* tile, int y0, int x0) {
+    const int lane = threadIdx.x & 63;
+    Frag<T> f;
+    if constexpr (sizeof(T) == 2) {
+        // 16 lanes read 4 rows of 16 values and get a column of 4 each
+        const T* at = tile + (y0 + (lane >> 5) * 4 + ((lane & 15) >> 2)) * LD + x0 +
+                      ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
+        typedef __attribute__((address_space(3))) short4v* Shared;
+        short4v lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Shared)at);
+        short4v hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Shared)(at + 8 * LD));
+        __builtin_memcpy(&f, &lo, 8);
+        __builtin_memcpy((char*)&f + 8, &hi, 8);
+    } else {
+        const T* at = tile + (y0 + (lane >> 5) * 4) * LD + x0 + (lane & 31);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] = at[(8 * (j >> 2) + (j & 3)) * LD];
+    }
+    return f;
+}
+
+// 8 values of a row in memory, zero behind d or where there is no row
+template <typename T>
+__device__ __forceinline__ Frag<T> row_frag(const T* base, int x, int d, bool there) {
+    Frag<T> f = {};
+    if (there && x < d) f = *(const Frag<T>*)(base + x);
+    return f;
+}
+
+template <typename T>
+__device__ __forceinline__ Frag<T> to_frag(const acc16& c, int first) {
+    Frag<T> f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = (T)c[first + j];
+    return f;
+}
+
+// the other half of the wave's value for the same column
+__device__ __forceinline__ float max_halves(float x) {
+    auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
+}
+__device__ __forceinline__ float add_halves(float x) {
+    auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(s[0]) + __uint_as_float(s[1]);
+}
+
+// row of register i of a 32x32 result
+__device__ __forceinline__ int row_of(int i) {
+    return 8 * (i >> 2) + 4 * ((threadIdx.x & 63) >> 5) + (i & 3);
+}
+
+// The documents of RANGE positions: x is the least of those that are not
+// negative (NONE without one), with the top bit set if there are negative
+// ones too, y the largest.
+__device__ __forceinline__ int2 range_of_wave(int doc) {
+    int lo = doc < 0 ? NONE : doc, hi = doc;
+    for (int m = 32; m; m >>= 1) {
+        lo = min(lo, __shfl_xor(lo, m));
+        hi = max(hi, __shfl_xor(hi, m));
+    }
+    if (__any(doc < 0)) lo |= 0x80000000;
+    return make_int2(__builtin_amdgcn_readfirstlane(lo), __builtin_amdgcn_readfirstlane(hi));
+}
+__device__ __forceinline__ bool meet(int2 a, int2 b) {
+    return max(a.x & NONE, b.x & NONE) <= min(a.y, b.y);
+}
+// all positions of both hold one document, and it is the same
+__device__ __forceinline__ bool one_document(int2 a, int2 b) {
+    return a.x == a.y && b.x == b.y && a.x == b.x;
+}
+
+// ranges [batch, count] of the positions from `first` on
+__global__ __launch_bounds__(64) void ranges_kernel(const int* documents, int64_t sb, int first,
+                                                    int end, int count, int2* ranges) {
+    int t = blockIdx.x % count, b = blockIdx.x / count;
+    int at = first + t * RANGE + threadIdx.x;
+    int2 r = range_of_wave(at < end ? documents[b * sb + at] : -1);
+    if (threadIdx.x == 0) ranges[blockIdx.x] = r;
+}
+
+// Workgroups go round the 8 XCDs: neighbours in the order returned run on one
+// XCD and share its L2.
+__device__ __forceinline__ unsigned xcd_order(unsigned block, unsigned blocks) {
+    unsigned each = blocks / 8, more = blocks % 8, x = block % 8;
+    return x * each + min(x, more) + block / 8;
+}
+
+constexpr float HEADROOM = 3.f;  // how far (log2) a score may pass the reference maximum
+constexpr float SHIFT = 12.f;    // probabilities carry a factor 2^12, at most 2^15 in all:
+                                 // in fp16 the small ones keep their bits
+
+// One wave's 32 queries against tiles of keys: the running softmax.
+template <typename T, int DP> struct Forward {
+    using G = Tile<T, DP>;
+    static constexpr int KT = G::KEYS / 32;
+    Frag<T> q[DP / 16];
+    acc16 o[DP / 32];
+    float top, off, total;  // reference maximum, what exponents lose, this half's sum
+    float c;                // score factor, in units of log2
+    float slope;
+    bool scaled;            // scores are scaled before the maximum is taken
+    int doc;                // the lane's query's document, INT_MIN for none
+    int pos;                // its position
+
+    __device__ __forceinline__ void begin(const Args& a, const T* row, bool there, float slope_) {
+        const int hf = (threadIdx.x & 63) >> 5;
+        slope = slope_;
+        c = fabsf(a.scale) * LOG2E;
+        scaled = slope != 0.f || c == 0.f;
+#pragma unroll
+        for (int n = 0; n < DP / 16; ++n) {
+            q[n] = row_frag<T>(row, n * 16 + hf * 8, a.d, there);
+            if (a.scale < 0) q[n] = -q[n];
+        }
+#pragma unroll
+        for (int n = 0; n < DP / 32; ++n) o[n] = acc16{};
+        top = -INFINITY;
+        off = -SHIFT;
+        total = 0;
+    }
+
+    // keys key0 .. key0 + KEYS; `mixed`: some pairs may be hidden
+    __device__ __forceinline__ void step(const T* k, const T* v, const int* docs, int key0,
+                                         bool mixed, bool causal) {
+        const int hf = (threadIdx.x & 63) >> 5;
+        acc16 s[KT];
+#pragma unroll
+        for (int t = 0; t < KT; ++t) {
+            s[t] = acc16{};
+#pragma unroll
+            for (int n = 0; n < DP / 16; ++n)
+                s[t] = mma(rows_of<T, G::LD>(k, t * 32, n * 16), q[n], s[t]);
+        }
+        if (scaled) {
+            float far = (float)(pos - key0 - 4 * hf);
+#pragma unroll
+            for (int t = 0; t < KT; ++t)
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    s[t][i] = s[t][i] * c -
+                              slope * fabsf(far - (float)(t * 32 + 8 * (i >> 2) + (i & 3)));
+        }
+        const float cm = scaled ? 1.f : c;
+        if (mixed) {
+#pragma unroll
+            for (int t = 0; t < KT; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    int at = t * 32 + r * 8 + 4 * hf;
+                    int4 d = *(const int4*)(docs + at);
+                    const int kd[4] = {d.x, d.y, d.z, d.w};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        bool hidden = kd[e] != doc || (causal && key0 + at + e > pos);
+                        s[t][r * 4 + e] = hidden ? -INFINITY : s[t][r * 4 + e];
+                    }
+                }
+        }
+        float most = -INFINITY;
+#pragma unroll
+        for (int t = 0; t < KT; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; i += 2) most = fmaxf(most, fmaxf(s[t][i], s[t][i + 1]));
+        most = max_halves(most) * cm;
+        if (__any(most > top + HEADROOM)) {
+            float next = fmaxf(top, most);
+            float keep = next == top ? 1.f : exp2_fast(top - next);
+            top = next;
+            off = (top == -INFINITY ? 0.f : top) - SHIFT;
+            total *= keep;
+#pragma unroll
+            for (int n = 0; n < DP / 32; ++n)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[n][i] *= keep;
+        }
+#pragma unroll
+        for (int t = 0; t < KT; ++t) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                s[t][i] = exp2_fast(fmaf(s[t][i], cm, -off));
+                total += s[t][i];
+            }
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                Frag<T> p = to_frag<T>(s[t], u * 8);
+#pragma unroll
+                for (int n = 0; n < DP / 32; ++n)
+                    o[n] = mma(columns_of<T, G::LD>(v, t * 32 + u * 16, n * 32), p, o[n]);
+            }
+        }
+    }
+
+    __device__ __forceinline__ bool finite() const {
+        bool fine = true;
+#pragma unroll
+        for (int n = 0; n < DP / 32; ++n)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) fine &= fabsf(o[n][i]) <= 3.4028235e38f;
+        return fine;
+    }
+};
+
+// four values of a row, as they lie in a result's registers
+template <typename T>
+__device__ __forceinline__ void put4(T* at, float a, float b, float c, float d) {
+    typedef T Four __attribute__((ext_vector_type(4)));
+    *(Four*)at = Four{(T)a, (T)b, (T)c, (T)d};
+}
+
+// The tiles that a block visits: those whose documents meet its own, in
+// order, THREADS candidates at a time.
+template <int THREADS> struct Visits {
+    int list[THREADS];
+    int counts[THREADS / 64];
+
+    __device__ __forceinline__ int fill(int first, int end, int size, const int2* ranges,
+                                        int2 own) {
+        int t = first + threadIdx.x;
+        bool there = t < end && meet(ranges[t * size / RANGE], own);
+        uint64_t all = __ballot(there);
+        int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+        __syncthreads();
+        if (lane == 0) counts[wave] = __popcll(all);
+        __syncthreads();
+        int before = 0, n = 0;
+        for (int w = 0; w < THREADS / 64; ++w) {
+            if (w < wave) before += counts[w];
+            n += counts[w];
+        }
+        if (there) list[before + __popcll(all & ((1ull << lane) - 1))] = t;
+        __syncthreads();
+        return n;
+    }
+};
+
+// 32 queries for each wave, all heads and keys.  The block's waves share the
+// tiles of K and V; block tiles of one head are neighbours on one XCD, whose
+// L2 then serves the head's keys once.
+template <typename T, int DP, int WAVES>
+__global__ __launch_bounds__(WAVES * 64, DP == 128 && (WAVES == 2 || sizeof(T) == 4) ? 1 : 2)
+void forward_kernel(const Args a, const int2* ranges,
+                                                                int ranges_n, int tiles_q) {
+    using G = Tile<T, DP>;
+    constexpr int THREADS = WAVES * 64, N = G::KEYS;
+    __shared__ alignas(16) T tile_k[N * G::LD], tile_v[N * G::LD];
+    __shared__ alignas(16) int docs[N];
+    __shared__ int2 own[WAVES];
+    __shared__ Visits<THREADS> visits;
+
+    unsigned id = xcd_order(blockIdx.x, gridDim.x);
+    int qt = id % tiles_q, h = id / tiles_q % a.hq, b = id / tiles_q / a.hq;
+    if (a.causal) qt = tiles_q - 1 - qt;  // the longest first
+    const int g = h / (a.hq / a.hkv), lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int first = a.sk - a.sq, row0 = qt * WAVES * 32 + wave * 32;
+    const int i = row0 + (lane & 31);
+    const bool there = i < a.sq;
+    const int* doc_row = a.documents ? a.documents + b * a.documents_sb : nullptr;
+
+    Forward<T, DP> f;
+    f.begin(a, row<T>(a.q, b, there ? i : 0, h), there, slope_of(a, h));
+    f.pos = i + first;
+    int doc = there ? doc_row ? doc_row[f.pos] : 0 : -1;
+    f.doc = doc < 0 ? INT_MIN : doc;
+    const int2 wave_docs = range_of_wave(doc);
+    int2 block_docs = wave_docs;
+    if (doc_row) {
+        if (lane == 0) own[wave] = wave_docs;
+        __syncthreads();
+        for (int w = 0; w < WAVES; ++w) {
+            block_docs.x = min(block_docs.x & NONE, own[w].x & NONE);
+            block_docs.y = max(block_docs.y, own[w].y);
+        }
+    }
+    const int wave_first = row0 + first, wave_last = min(row0 + 31, a.sq - 1) + first;
+    int end = a.sk;
+    if (a.causal) end = min(end, (qt + 1) * WAVES * 32 + first);
+    const int tiles = (end + N - 1) / N;
+    const T *k = row<T>(a.k, b, 0, g), *v = row<T>(a.v, b, 0, g);
+
+    Stage<T, DP, N, THREADS> sk, sv;
+    for (int chunk = 0; chunk < tiles; chunk += THREADS) {
+        int n = min(THREADS, tiles - chunk);
+        if (doc_row) n = visits.fill(chunk, tiles, N, ranges + (int64_t)b * ranges_n, block_docs);
+        auto tile_at = [&](int m) { return (doc_row ? visits.list[m] : chunk + m) * N; };
+        int key0 = n ? tile_at(0) : 0, key_doc = -1;
+        auto fetch = [&](int at) {
+            sk.load(k + (int64_t)at * a.k.ss, a.k.ss, a.sk - at, a.d);
+            sv.load(v + (int64_t)at * a.v.ss, a.v.ss, a.sk - at, a.d);
+            int j = at + threadIdx.x;
+            if ((int)threadIdx.x < N) key_doc = j < a.sk ? doc_row ? max(doc_row[j], -1) : 0 : -1;
+        };
+        if (n) fetch(key0);
+        for (int m = 0; m < n; ++m) {
+            __syncthreads();
+            sk.store(tile_k);
+            sv.store(tile_v);
+            if ((int)threadIdx.x < N) docs[threadIdx.x] = key_doc;
+            __syncthreads();
+            const int at = key0;
+            if (m + 1 < n) {
+                key0 = tile_at(m + 1);
+                fetch(key0);
+            }
+            bool mixed = at + N > a.sk || (a.causal && at + N - 1 > wave_first);
+            if (a.causal && at > wave_last) continue;
+            if (doc_row) {
+                int2 r = ranges[(int64_t)b * ranges_n + at / RANGE];
+                if (!meet(r, wave_docs)) continue;
+                mixed |= !one_document(r, wave_docs);
+            }
+            f.step(tile_k, tile_v, docs, at, mixed, a.causal);
+        }
+    }
+
+    const float total = add_halves(f.total);
+    const float inv = total == 0.f ? 0.f : 1.f / total;
+    if (there) {
+        T* out = row<T>(a.out, b, i, h);
+#pragma unroll
+        for (int n = 0; n < DP / 32; ++n)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                int d = n * 32 + r * 8 + (lane >> 5) * 4;
+                if (d < a.d)
+                    put4(out + d, f.o[n][r * 4] * inv, f.o[n][r * 4 + 1] * inv,
+                         f.o[n][r * 4 + 2] * inv, f.o[n][r * 4 + 3] * inv);
+            }
+        if (a.lse && lane < 32)
+            a.lse[((int64_t)b * a.hq + h) * a.sq + i] =
+                total == 0.f ? -INFINITY : f.off + log2f(total);
+    }
+    // A hidden infinity or NaN times a probability of zero is NaN, and values
+    // near the largest pass it with the factor 2^12: such rows are done again
+    // pair by pair.
+    uint64_t bad = __ballot(there && !f.finite());
+    for (uint64_t rows = (bad | bad >> 32) & 0xffffffffull; rows; rows &= rows - 1)
+        forward_row<T>(a, b, h, row0 + __builtin_ctzll(rows));
+}
+
+int padded(int d) { return (d + 31) / 32 * 32; }
+
+template <typename T, int DP>
+void launch_forward(const Args& a, const int2* ranges, int ranges_n, hipStream_t stream) {
+    // 128 queries a block share a tile; with few blocks 64 spread wider
+    int64_t heads = (int64_t)a.b * a.hq;
+    bool wide = heads * ((a.sq + 127) / 128) >= 512;
+    int rows = wide ? 128 : 64, tiles_q = (a.sq + rows - 1) / rows;
+    int64_t blocks = heads * tiles_q;
+    TORCH_CHECK(blocks <= INT_MAX, "too many rows for one launch");
+    if (wide)
+        hipLaunchKernelGGL((forward_kernel<T, DP, 4>), dim3((unsigned)blocks), dim3(256), 0,
+                           stream, a, ranges, ranges_n, tiles_q);
+    else
+        hipLaunchKernelGGL((forward_kernel<T, DP, 2>), dim3((unsigned)blocks), dim3(128), 0,
+                           stream, a, ranges, ranges_n, tiles_q);
+}
+
+// f of the head size, as the constant of its padded width
+template <typename F>
+void for_width(int d, F f) {
+    switch (padded(d)) {
+        case 32: f(std::integral_constant<int, 32>{}); break;
+        case 64: f(std::integral_constant<int, 64>{}); break;
+        case 96: f(std::integral_constant<int, 96>{}); break;
+        default: f(std::integral_constant<int, 128>{}); break;
+    }
+}
+
+// [batch, count] ranges of the positions from `first` on, for a launch
+torch::Tensor ranges_for(const Args& a, int first, const torch::Tensor& like, hipStream_t stream) {
+    int count = (a.sk - first + RANGE - 1) / RANGE;
+    auto r = torch::empty({a.b, count, 2}, like.options().dtype(torch::kInt32));
+    if (a.b * (int64_t)count)
+        hipLaunchKernelGGL(ranges_kernel, dim3((unsigned)(a.b * count)), dim3(64), 0, stream,
+                           a.documents, a.documents_sb, first, a.sk, count,
+                           (int2*)r.data_ptr<int>());
+    return r;
+}
+
+// ---------------------------------------------------------------------------
 
 View view(const torch::Tensor& t) {
     return {t.data_ptr(), t.stride(0), t.stride(1), t.stride(2)};
@@ -317,9 +786,16 @@ std::vector<torch::Tensor> attention_forward(torch::Tensor q, torch::Tensor k, t
     a.q = view(q), a.k = view(k), a.v = view(v), a.out = view(out);
     a.lse = want_lse ? lse.data_ptr<float>() : nullptr;
     hipStream_t stream = at::hip::getCurrentHIPStream();
+    if (out.numel() == 0) return {out, lse};
+    torch::Tensor ranges;
+    if (documents) ranges = ranges_for(a, 0, q, stream);
     for_type(q.scalar_type(), [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
-        launch_rows<T, FORWARD>(a, stream);
+        for_width(a.d, [&](auto width) {
+            launch_forward<T, decltype(width)::value>(
+                a, documents ? (const int2*)ranges.data_ptr<int>() : nullptr,
+                documents ? (int)ranges.size(1) : 0, stream);
+        });
     });
     return {out, lse};
 }
