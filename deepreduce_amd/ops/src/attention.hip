@@ -205,42 +205,6 @@ __device__ void dkv_row(const Args& a, int b, int g, int j) {
     if (lane + 64 < a.d) to_k[lane + 64] = (T)(dk[1] * a.scale), to_v[lane + 64] = (T)dv[1];
 }
 
-enum Pass { FORWARD, DELTA, DQ, DKV };
-
-template <typename T>
-__device__ void delta_row(const Args& a, int b, int h, int i) {
-    const int lane = threadIdx.x & 63;
-    const T *x = row<T>(a.dout, b, i, h), *y = row<T>(a.out, b, i, h);
-    float s = 0;
-    for (int d = lane; d < a.d; d += 64) s = fmaf((float)x[d], (float)y[d], s);
-    s = wave_sum(s);
-    if (lane == 0) a.delta[((int64_t)b * a.hq + h) * a.sq + i] = s;
-}
-
-template <typename T, Pass PASS>
-__global__ __launch_bounds__(256) void rows_kernel(const Args a, int64_t rows, int length,
-                                                   int heads) {
-    int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (r >= rows) return;
-    int i = (int)(r % length);
-    int h = (int)(r / length % heads), b = (int)(r / length / heads);
-    if constexpr (PASS == FORWARD) forward_row<T>(a, b, h, i);
-    if constexpr (PASS == DELTA) delta_row<T>(a, b, h, i);
-    if constexpr (PASS == DQ) dq_row<T>(a, b, h, i);
-    if constexpr (PASS == DKV) dkv_row<T>(a, b, h, i);
-}
-
-template <typename T, Pass PASS>
-void launch_rows(const Args& a, hipStream_t stream) {
-    int length = PASS == DKV ? a.sk : a.sq, heads = PASS == DKV ? a.hkv : a.hq;
-    int64_t rows = (int64_t)a.b * length * heads;
-    if (rows == 0) return;
-    int64_t blocks = (rows + 3) / 4;
-    TORCH_CHECK(blocks <= INT_MAX, "too many rows for one launch");
-    hipLaunchKernelGGL((rows_kernel<T, PASS>), dim3((unsigned)blocks), dim3(256), 0, stream, a,
-                       rows, length, heads);
-}
-
 // ---------------------------------------------------------------------------
 // Tiles on the matrix cores.  A fragment of a 32x32x16 product is 8 values a
 // lane: lane l holds row (or column) l % 32, k = (l / 32) * 8 + 0..7; of the
@@ -683,6 +647,415 @@ void launch_forward(const Args& a, const int2* ranges, int ranges_n, hipStream_t
                            stream, a, ranges, ranges_n, tiles_q);
 }
 
+// ---------------------------------------------------------------------------
+// Backward.  delta and the queries' gradient, whose waves hold 32 queries as
+// the forward's do; then the keys' and values', whose waves hold 32 keys and
+// go over the queries of all heads that share them.  Scores are formed again
+// in both (7 products where 5 would do), so that nothing is added across
+// blocks: results repeat bit by bit and no buffer of gradients is needed.
+//
+// dS is rounded to the inputs' type for its products.  In fp16 it first gets
+// a factor, a power of two that puts its queries' largest dout near 2^-4 and
+// P's 2^12 with it, so that gradients of any size keep their bits.
+// ---------------------------------------------------------------------------
+
+constexpr int FACTOR_ROWS = 64;
+
+template <typename T> constexpr bool FACTORED = std::is_same<T, _Float16>::value;
+
+// rows that saw nothing have probabilities of zero
+__device__ __forceinline__ float usable(float lse) { return lse == -INFINITY ? INFINITY : lse; }
+
+// 64 rows a block, 4 threads a row; one read of dout and out bounds it
+template <typename T>
+__global__ __launch_bounds__(256) void delta_kernel(const Args a, int tiles, float* factors) {
+    int t = blockIdx.x % tiles, h = blockIdx.x / tiles % a.hq, b = blockIdx.x / tiles / a.hq;
+    int i = t * FACTOR_ROWS + (threadIdx.x >> 2);
+    float sum = 0, most = 0;
+    if (i < a.sq) {
+        const T *x = row<T>(a.dout, b, i, h), *y = row<T>(a.out, b, i, h);
+        for (int d = (threadIdx.x & 3) * 8; d < a.d; d += 32) {
+            Frag<T> u = *(const Frag<T>*)(x + d), w = *(const Frag<T>*)(y + d);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                sum = fmaf((float)u[e], (float)w[e], sum);
+                float size = fabsf((float)u[e]);
+                if (FACTORED<T> && size < INFINITY) most = fmaxf(most, size);
+            }
+        }
+    }
+    sum += __shfl_xor(sum, 1);
+    sum += __shfl_xor(sum, 2);
+    if (i < a.sq && (threadIdx.x & 3) == 0) a.delta[((int64_t)b * a.hq + h) * a.sq + i] = sum;
+    if constexpr (FACTORED<T>) {
+        __shared__ float shared[4];
+        most = wave_max(most);
+        if ((threadIdx.x & 63) == 0) shared[threadIdx.x >> 6] = most;
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            for (int w = 1; w < 4; ++w) most = fmaxf(most, shared[w]);
+            factors[blockIdx.x] = most == 0.f ? 1.f : exp2f(-4.f - ceilf(log2f(most)));
+        }
+    }
+}
+
+template <typename T, int DP, int WAVES>
+__global__ __launch_bounds__(WAVES * 64, DP == 128 ? 1 : 2)
+void dq_kernel(const Args a, const int2* ranges, int ranges_n, int tiles_q, const float* factors,
+               int factors_n) {
+    using G = Tile<T, DP>;
+    constexpr int THREADS = WAVES * 64, N = G::KEYS;
+    __shared__ alignas(16) T tile_k[N * G::LD], tile_v[N * G::LD];
+    __shared__ alignas(16) int docs[N];
+    __shared__ int2 own[WAVES];
+    __shared__ Visits<THREADS> visits;
+
+    unsigned id = xcd_order(blockIdx.x, gridDim.x);
+    int qt = id % tiles_q, h = id / tiles_q % a.hq, b = id / tiles_q / a.hq;
+    if (a.causal) qt = tiles_q - 1 - qt;
+    const int g = h / (a.hq / a.hkv), lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int hf = lane >> 5, first = a.sk - a.sq, row0 = qt * WAVES * 32 + wave * 32;
+    const int i = row0 + (lane & 31), pos = i + first;
+    const bool there = i < a.sq;
+    const int* doc_row = a.documents ? a.documents + b * a.documents_sb : nullptr;
+    const int64_t at_row = ((int64_t)b * a.hq + h) * a.sq + i;
+
+    const float c = fabsf(a.scale) * LOG2E, slope = slope_of(a, h);
+    Frag<T> q[DP / 16], dout[DP / 16];
+#pragma unroll
+    for (int n = 0; n < DP / 16; ++n) {
+        q[n] = row_frag<T>(row<T>(a.q, b, there ? i : 0, h), n * 16 + hf * 8, a.d, there);
+        dout[n] = row_frag<T>(row<T>(a.dout, b, there ? i : 0, h), n * 16 + hf * 8, a.d, there);
+        if (a.scale < 0) q[n] = -q[n];
+    }
+    acc16 acc[DP / 32];
+#pragma unroll
+    for (int n = 0; n < DP / 32; ++n) acc[n] = acc16{};
+    const float delta = there ? a.delta[at_row] : 0.f;
+    float off = there ? usable(a.lse[at_row]) : INFINITY, back = a.scale;
+    if constexpr (FACTORED<T>) {
+        float f = factors[((int64_t)b * a.hq + h) * factors_n + min(i, a.sq - 1) / FACTOR_ROWS];
+        off -= SHIFT + log2f(f);
+        back *= exp2f(-SHIFT) / f;
+    }
+
+    const int seen = there ? doc_row ? doc_row[pos] : 0 : -1;
+    const int doc = seen < 0 ? INT_MIN : seen;
+    const int2 wave_docs = range_of_wave(seen);
+    int2 block_docs = wave_docs;
+    if (doc_row) {
+        if (lane == 0) own[wave] = wave_docs;
+        __syncthreads();
+        for (int w = 0; w < WAVES; ++w) {
+            block_docs.x = min(block_docs.x & NONE, own[w].x & NONE);
+            block_docs.y = max(block_docs.y, own[w].y);
+        }
+    }
+    const int wave_first = row0 + first, wave_last = min(row0 + 31, a.sq - 1) + first;
+    int end = a.sk;
+    if (a.causal) end = min(end, (qt + 1) * WAVES * 32 + first);
+    const int tiles = (end + N - 1) / N;
+    const T *k = row<T>(a.k, b, 0, g), *v = row<T>(a.v, b, 0, g);
+
+    Stage<T, DP, N, THREADS> sk, sv;
+    for (int chunk = 0; chunk < tiles; chunk += THREADS) {
+        int n = min(THREADS, tiles - chunk);
+        if (doc_row) n = visits.fill(chunk, tiles, N, ranges + (int64_t)b * ranges_n, block_docs);
+        auto tile_at = [&](int m) { return (doc_row ? visits.list[m] : chunk + m) * N; };
+        int key0 = n ? tile_at(0) : 0, key_doc = -1;
+        auto fetch = [&](int at) {
+            sk.load(k + (int64_t)at * a.k.ss, a.k.ss, a.sk - at, a.d);
+            sv.load(v + (int64_t)at * a.v.ss, a.v.ss, a.sk - at, a.d);
+            int j = at + threadIdx.x;
+            if ((int)threadIdx.x < N) key_doc = j < a.sk ? doc_row ? max(doc_row[j], -1) : 0 : -1;
+        };
+        if (n) fetch(key0);
+        for (int m = 0; m < n; ++m) {
+            __syncthreads();
+            sk.store(tile_k);
+            sv.store(tile_v);
+            if ((int)threadIdx.x < N) docs[threadIdx.x] = key_doc;
+            __syncthreads();
+            const int at = key0;
+            if (m + 1 < n) {
+                key0 = tile_at(m + 1);
+                fetch(key0);
+            }
+            bool mixed = at + N > a.sk || (a.causal && at + N - 1 > wave_first);
+            if (a.causal && at > wave_last) continue;
+            if (doc_row) {
+                int2 r = ranges[(int64_t)b * ranges_n + at / RANGE];
+                if (!meet(r, wave_docs)) continue;
+                mixed |= !one_document(r, wave_docs);
+            }
+#pragma unroll
+            for (int t = 0; t < N / 32; ++t) {
+                acc16 s = {}, dp = {};
+#pragma unroll
+                for (int n = 0; n < DP / 16; ++n)
+                    s = mma(rows_of<T, G::LD>(tile_k, t * 32, n * 16), q[n], s);
+#pragma unroll
+                for (int n = 0; n < DP / 16; ++n)
+                    dp = mma(rows_of<T, G::LD>(tile_v, t * 32, n * 16), dout[n], dp);
+                if (slope != 0.f) {
+                    float far = (float)(pos - at - t * 32 - 4 * hf);
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        s[e] = fmaf(s[e], c, -off - slope * fabsf(far - (float)(8 * (e >> 2) + (e & 3))));
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) s[e] = fmaf(s[e], c, -off);
+                }
+                if (mixed) {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        int j = t * 32 + r * 8 + 4 * hf;
+                        int4 d = *(const int4*)(docs + j);
+                        const int kd[4] = {d.x, d.y, d.z, d.w};
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            bool hidden = kd[e] != doc || (a.causal && at + j + e > pos);
+                            s[r * 4 + e] = hidden ? -INFINITY : s[r * 4 + e];
+                        }
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < 16; ++e) s[e] = exp2_fast(s[e]) * (dp[e] - delta);
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    Frag<T> ds = to_frag<T>(s, u * 8);
+#pragma unroll
+                    for (int n = 0; n < DP / 32; ++n)
+                        acc[n] = mma(columns_of<T, G::LD>(tile_k, t * 32 + u * 16, n * 32), ds,
+                                     acc[n]);
+                }
+            }
+        }
+    }
+
+    bool fine = true;
+    if (there) {
+        T* dq = row<T>(a.dq, b, i, h);
+#pragma unroll
+        for (int n = 0; n < DP / 32; ++n)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                int d = n * 32 + r * 8 + hf * 4;
+                if (d < a.d)
+                    put4(dq + d, acc[n][r * 4] * back, acc[n][r * 4 + 1] * back,
+                         acc[n][r * 4 + 2] * back, acc[n][r * 4 + 3] * back);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) fine &= fabsf(acc[n][r * 4 + e]) <= 3.4028235e38f;
+            }
+    }
+    uint64_t bad = __ballot(!fine);
+    for (uint64_t rows = (bad | bad >> 32) & 0xffffffffull; rows; rows &= rows - 1)
+        dq_row<T>(a, b, h, row0 + __builtin_ctzll(rows));
+}
+
+template <typename T, int DP, int WAVES>
+__global__ __launch_bounds__(WAVES * 64, DP >= 96 ? 1 : 2)
+void dkv_kernel(const Args a, const int2* ranges, int ranges_n, int tiles_k, const float* factors,
+                int factors_n) {
+    using G = Tile<T, DP>;
+    constexpr int THREADS = WAVES * 64, N = G::KEYS;  // N queries a tile
+    __shared__ alignas(16) T tile_q[N * G::LD], tile_o[N * G::LD];
+    __shared__ alignas(16) int docs[N];
+    __shared__ alignas(16) float lses[N], deltas[N];
+    __shared__ int2 own[WAVES];
+    __shared__ Visits<THREADS> visits;
+
+    unsigned id = xcd_order(blockIdx.x, gridDim.x);
+    const int kt = id % tiles_k, g = id / tiles_k % a.hkv, b = id / tiles_k / a.hkv;
+    const int group = a.hq / a.hkv, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int hf = lane >> 5, first = a.sk - a.sq, block0 = kt * WAVES * 32;
+    const int key0 = block0 + wave * 32, j = key0 + (lane & 31);
+    const bool there = j < a.sk;
+    const int* doc_row = a.documents ? a.documents + b * a.documents_sb : nullptr;
+
+    const float c = fabsf(a.scale) * LOG2E;
+    Frag<T> k[DP / 16], v[DP / 16];
+#pragma unroll
+    for (int n = 0; n < DP / 16; ++n) {
+        k[n] = row_frag<T>(row<T>(a.k, b, there ? j : 0, g), n * 16 + hf * 8, a.d, there);
+        v[n] = row_frag<T>(row<T>(a.v, b, there ? j : 0, g), n * 16 + hf * 8, a.d, there);
+        if (a.scale < 0) k[n] = -k[n];
+    }
+    acc16 dk[DP / 32], dv[DP / 32];
+#pragma unroll
+    for (int n = 0; n < DP / 32; ++n) dk[n] = acc16{}, dv[n] = acc16{};
+    float factor = 1.f;  // what dk's sums have
+    bool begun = false;
+
+    const int seen = there ? doc_row ? doc_row[j] : 0 : -1;
+    const int doc = seen < 0 ? INT_MIN : seen;
+    const int2 wave_docs = range_of_wave(seen);
+    int2 block_docs = wave_docs;
+    if (doc_row) {
+        if (lane == 0) own[wave] = wave_docs;
+        __syncthreads();
+        for (int w = 0; w < WAVES; ++w) {
+            block_docs.x = min(block_docs.x & NONE, own[w].x & NONE);
+            block_docs.y = max(block_docs.y, own[w].y);
+        }
+    }
+    const int wave_last = min(key0 + 31, a.sk - 1);
+    const int tiles = (a.sq + N - 1) / N;
+    const int begin = a.causal ? max(0, block0 - first) / N : 0;
+
+    Stage<T, DP, N, THREADS> sq, so;
+    for (int chunk = begin; chunk < tiles; chunk += THREADS) {
+        int n = min(THREADS, tiles - chunk);
+        if (doc_row) n = visits.fill(chunk, tiles, N, ranges + (int64_t)b * ranges_n, block_docs);
+        auto tile_at = [&](int m) { return (doc_row ? visits.list[m] : chunk + m) * N; };
+        int next = 0, next_h = g * group, query_doc = -1;
+        float lse = 0, delta = 0, next_factor = 1.f;
+        auto fetch = [&](int m) {
+            next_h = g * group + m / n;
+            next = tile_at(m % n);
+            sq.load(row<T>(a.q, b, next, next_h), a.q.ss, a.sq - next, a.d);
+            so.load(row<T>(a.dout, b, next, next_h), a.dout.ss, a.sq - next, a.d);
+            if ((int)threadIdx.x < N) {
+                int i = next + threadIdx.x;
+                int64_t at = ((int64_t)b * a.hq + next_h) * a.sq + i;
+                lse = i < a.sq ? usable(a.lse[at]) : INFINITY;
+                delta = i < a.sq ? a.delta[at] : 0.f;
+                query_doc = i < a.sq ? doc_row ? max(doc_row[i + first], -1) : 0 : -1;
+            }
+            if constexpr (FACTORED<T>)
+                next_factor = factors[((int64_t)b * a.hq + next_h) * factors_n + next / FACTOR_ROWS];
+        };
+        if (n) fetch(0);
+        for (int m = 0; m < n * group; ++m) {
+            __syncthreads();
+            sq.store(tile_q);
+            so.store(tile_o);
+            if ((int)threadIdx.x < N) {
+                docs[threadIdx.x] = query_doc;
+                lses[threadIdx.x] = lse;
+                deltas[threadIdx.x] = delta;
+            }
+            __syncthreads();
+            const int at = next, h = next_h;
+            const float tile_factor = next_factor;
+            if (m + 1 < n * group) fetch(m + 1);
+            bool mixed = a.causal && at + first < wave_last;
+            if (a.causal && at + first + N - 1 < key0) continue;
+            if (doc_row) {
+                int2 r = ranges[(int64_t)b * ranges_n + at / RANGE];
+                if (!meet(r, wave_docs)) continue;
+                mixed |= !one_document(r, wave_docs);
+            }
+            if constexpr (FACTORED<T>) {
+                // larger gradients than before: dk's sums go to their factor
+                if (!begun || tile_factor < factor) {
+                    float by = begun ? tile_factor / factor : 1.f;
+#pragma unroll
+                    for (int n = 0; n < DP / 32; ++n)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) dk[n][e] *= by;
+                    factor = tile_factor;
+                    begun = true;
+                }
+            }
+            const float slope = slope_of(a, h);
+#pragma unroll
+            for (int t = 0; t < N / 32; ++t) {
+                acc16 s = {}, dp = {};
+#pragma unroll
+                for (int n = 0; n < DP / 16; ++n)
+                    s = mma(rows_of<T, G::LD>(tile_q, t * 32, n * 16), k[n], s);
+#pragma unroll
+                for (int n = 0; n < DP / 16; ++n)
+                    dp = mma(rows_of<T, G::LD>(tile_o, t * 32, n * 16), v[n], dp);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int i = t * 32 + r * 8 + 4 * hf;
+                    const f32x4 l = *(const f32x4*)(lses + i), dl = *(const f32x4*)(deltas + i);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        float off = l[e];
+                        if constexpr (FACTORED<T>) off -= SHIFT;
+                        if (slope != 0.f)
+                            off = fmaf(slope, fabsf((float)(at + first + i + e - j)), off);
+                        s[r * 4 + e] = fmaf(s[r * 4 + e], c, -off);
+                        if constexpr (FACTORED<T>)
+                            dp[r * 4 + e] = fmaf(dp[r * 4 + e], factor, -dl[e] * factor);
+                        else
+                            dp[r * 4 + e] -= dl[e];
+                    }
+                    if (mixed) {
+                        int4 d = *(const int4*)(docs + i);
+                        const int qd[4] = {d.x, d.y, d.z, d.w};
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            bool hidden = qd[e] != doc || (a.causal && j > at + first + i + e);
+                            s[r * 4 + e] = hidden ? -INFINITY : s[r * 4 + e];
+                        }
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    s[e] = exp2_fast(s[e]);
+                    dp[e] *= s[e];
+                }
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    Frag<T> p = to_frag<T>(s, u * 8), ds = to_frag<T>(dp, u * 8);
+#pragma unroll
+                    for (int n = 0; n < DP / 32; ++n) {
+                        dv[n] = mma(columns_of<T, G::LD>(tile_o, t * 32 + u * 16, n * 32), p, dv[n]);
+                        dk[n] = mma(columns_of<T, G::LD>(tile_q, t * 32 + u * 16, n * 32), ds, dk[n]);
+                    }
+                }
+            }
+        }
+    }
+
+    float back_k = a.scale, back_v = 1.f;
+    if constexpr (FACTORED<T>) {
+        back_v = exp2f(-SHIFT);
+        back_k *= back_v / factor;
+    }
+    bool fine = true;
+    if (there) {
+        T *to_k = row<T>(a.dk, b, j, g), *to_v = row<T>(a.dv, b, j, g);
+#pragma unroll
+        for (int n = 0; n < DP / 32; ++n)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                int d = n * 32 + r * 8 + hf * 4, e = r * 4;
+                if (d < a.d) {
+                    put4(to_k + d, dk[n][e] * back_k, dk[n][e + 1] * back_k, dk[n][e + 2] * back_k,
+                         dk[n][e + 3] * back_k);
+                    put4(to_v + d, dv[n][e] * back_v, dv[n][e + 1] * back_v, dv[n][e + 2] * back_v,
+                         dv[n][e + 3] * back_v);
+                }
+#pragma unroll
+                for (int x = e; x < e + 4; ++x)
+                    fine &= fabsf(dk[n][x]) <= 3.4028235e38f && fabsf(dv[n][x]) <= 3.4028235e38f;
+            }
+    }
+    uint64_t bad = __ballot(!fine);
+    for (uint64_t rows = (bad | bad >> 32) & 0xffffffffull; rows; rows &= rows - 1)
+        dkv_row<T>(a, b, g, key0 + __builtin_ctzll(rows));
+}
+
+template <typename T, int DP>
+void launch_backward(const Args& a, const int2* key_ranges, int key_n, const int2* query_ranges,
+                     int query_n, float* factors, int factors_n, hipStream_t stream) {
+    int64_t rows = (int64_t)a.b * a.hq * factors_n;
+    int tiles_q = (a.sq + 127) / 128, tiles_k = (a.sk + 127) / 128;
+    int64_t blocks_q = (int64_t)a.b * a.hq * tiles_q, blocks_k = (int64_t)a.b * a.hkv * tiles_k;
+    TORCH_CHECK(rows <= INT_MAX && blocks_k <= INT_MAX, "too many rows for one launch");
+    hipLaunchKernelGGL(delta_kernel<T>, dim3((unsigned)rows), dim3(256), 0, stream, a, factors_n,
+                       factors);
+    hipLaunchKernelGGL((dq_kernel<T, DP, 4>), dim3((unsigned)blocks_q), dim3(256), 0, stream, a,
+                       key_ranges, key_n, tiles_q, factors, factors_n);
+    hipLaunchKernelGGL((dkv_kernel<T, DP, 4>), dim3((unsigned)blocks_k), dim3(256), 0, stream, a,
+                       query_ranges, query_n, tiles_k, factors, factors_n);
+}
+
 // f of the head size, as the constant of its padded width
 template <typename F>
 void for_width(int d, F f) {
@@ -826,11 +1199,25 @@ std::vector<torch::Tensor> attention_backward(torch::Tensor dout, torch::Tensor 
     a.lse = lse.data_ptr<float>();
     a.delta = delta.data_ptr<float>();
     hipStream_t stream = at::hip::getCurrentHIPStream();
+    if (dq.numel() == 0) return {dq, dk.zero_(), dv.zero_()};
+    const int factors_n = (a.sq + FACTOR_ROWS - 1) / FACTOR_ROWS;
+    auto factors = torch::empty({a.b, a.hq, factors_n}, lse.options());
+    torch::Tensor keys, queries;  // ranges of documents
+    const int2 *key_ranges = nullptr, *query_ranges = nullptr;
+    if (documents) {
+        keys = ranges_for(a, 0, q, stream);
+        queries = a.sq == a.sk ? keys : ranges_for(a, a.sk - a.sq, q, stream);
+        key_ranges = (const int2*)keys.data_ptr<int>();
+        query_ranges = (const int2*)queries.data_ptr<int>();
+    }
     for_type(q.scalar_type(), [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
-        launch_rows<T, DELTA>(a, stream);
-        launch_rows<T, DQ>(a, stream);
-        launch_rows<T, DKV>(a, stream);
+        for_width(a.d, [&](auto width) {
+            launch_backward<T, decltype(width)::value>(
+                a, key_ranges, documents ? (int)keys.size(1) : 0, query_ranges,
+                documents ? (int)queries.size(1) : 0, factors.data_ptr<float>(), factors_n,
+                stream);
+        });
     });
     return {dq, dk, dv};
 }
