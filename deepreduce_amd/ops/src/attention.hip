@@ -34,7 +34,7 @@ struct View {
 };
 
 struct Args {
-    View q, k, v, out, dout, dq, dk, dv;
+    View q, k, v, out, rest, dout, dq, dk, dv;  // rest: what rounding took from out
     float* lse;              // [batch, hq, sq], in log2 units
     float* delta;            // [batch, hq, sq]
     const int* documents;    // [batch, sk] or none
@@ -126,8 +126,11 @@ __device__ void forward_row(const Args& a, int b, int h, int i) {
         }
     }
     T* out = row<T>(a.out, b, i, h);
-    if (lane < a.d) out[lane] = (T)o[0];
-    if (lane + 64 < a.d) out[lane + 64] = (T)o[1];
+    for (int n = 0; n < 2; ++n)
+        if (int d = lane + n * 64; d < a.d) {
+            out[d] = (T)o[n];
+            if (a.rest.at) row<T>(a.rest, b, i, h)[d] = (T)(o[n] - (float)out[d]);
+        }
     if (lane == 0 && a.lse)
         a.lse[((int64_t)b * a.hq + h) * a.sq + i] = total == 0.f ? -INFINITY : base + log2f(total);
 }
@@ -336,6 +339,24 @@ __device__ __forceinline__ float add_halves(float x) {
     return __uint_as_float(s[0]) + __uint_as_float(s[1]);
 }
 
+// sums += (rows y0 .. y0 + 32 of a tile) transposed * c.  In 32 bits the rows'
+// own sum comes first: added one by one, tens of thousands of products would
+// lose more bits than a product of matrices does.
+template <typename T, int DP>
+__device__ __forceinline__ void add_product(const T* tile, int y0, const acc16& c, acc16* sums) {
+    constexpr int LD = Tile<T, DP>::LD;
+    const Frag<T> lo = to_frag<T>(c, 0), hi = to_frag<T>(c, 8);
+#pragma unroll
+    for (int n = 0; n < DP / 32; ++n) {
+        acc16 x = {};
+        if constexpr (sizeof(T) == 2) x = sums[n];
+        x = mma(columns_of<T, LD>(tile, y0, n * 32), lo, x);
+        x = mma(columns_of<T, LD>(tile, y0 + 16, n * 32), hi, x);
+        if constexpr (sizeof(T) == 4) x += sums[n];
+        sums[n] = x;
+    }
+}
+
 // row of register i of a 32x32 result
 __device__ __forceinline__ int row_of(int i) {
     return 8 * (i >> 2) + 4 * ((threadIdx.x & 63) >> 5) + (i & 3);
@@ -384,7 +405,6 @@ constexpr float SHIFT = 12.f;    // probabilities carry a factor 2^12, at most 2
 // One wave's 32 queries against tiles of keys: the running softmax.
 template <typename T, int DP> struct Forward {
     using G = Tile<T, DP>;
-    static constexpr int KT = G::KEYS / 32;
     Frag<T> q[DP / 16];
     acc16 o[DP / 32];
     float top, off, total;  // reference maximum, what exponents lose, this half's sum
@@ -411,17 +431,18 @@ template <typename T, int DP> struct Forward {
         total = 0;
     }
 
-    // keys key0 .. key0 + KEYS; `mixed`: some pairs may be hidden
-    __device__ __forceinline__ void step(const T* k, const T* v, const int* docs, int key0,
-                                         bool mixed, bool causal) {
+    // keys key0 .. key0 + 32 KT, k(t, n) the fragments of their rows; `mixed`:
+    // some pairs may be hidden
+    template <int KT, typename K>
+    __device__ __forceinline__ void step(K k, const T* v, const int* docs, int key0, bool mixed,
+                                         bool causal) {
         const int hf = (threadIdx.x & 63) >> 5;
         acc16 s[KT];
 #pragma unroll
         for (int t = 0; t < KT; ++t) {
             s[t] = acc16{};
 #pragma unroll
-            for (int n = 0; n < DP / 16; ++n)
-                s[t] = mma(rows_of<T, G::LD>(k, t * 32, n * 16), q[n], s[t]);
+            for (int n = 0; n < DP / 16; ++n) s[t] = mma(k(t, n), q[n], s[t]);
         }
         if (scaled) {
             float far = (float)(pos - key0 - 4 * hf);
@@ -465,21 +486,17 @@ template <typename T, int DP> struct Forward {
 #pragma unroll
                 for (int i = 0; i < 16; ++i) o[n][i] *= keep;
         }
+        float sum = 0;  // a tile's first, so that long rows keep their bits
 #pragma unroll
         for (int t = 0; t < KT; ++t) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 s[t][i] = exp2_fast(fmaf(s[t][i], cm, -off));
-                total += s[t][i];
+                sum += s[t][i];
             }
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                Frag<T> p = to_frag<T>(s[t], u * 8);
-#pragma unroll
-                for (int n = 0; n < DP / 32; ++n)
-                    o[n] = mma(columns_of<T, G::LD>(v, t * 32 + u * 16, n * 32), p, o[n]);
-            }
+            add_product<T, DP>(v, t * 32, s[t], o);
         }
+        total += sum;
     }
 
     __device__ __forceinline__ bool finite() const {
@@ -497,6 +514,16 @@ template <typename T>
 __device__ __forceinline__ void put4(T* at, float a, float b, float c, float d) {
     typedef T Four __attribute__((ext_vector_type(4)));
     *(Four*)at = Four{(T)a, (T)b, (T)c, (T)d};
+}
+
+// an output row's four values, and what rounding took from them
+template <typename T>
+__device__ __forceinline__ void put_out(const Args& a, int b, int i, int h, int d, const float* x) {
+    T* out = row<T>(a.out, b, i, h) + d;
+    put4(out, x[0], x[1], x[2], x[3]);
+    if (a.rest.at)
+        put4(row<T>(a.rest, b, i, h) + d, x[0] - (float)(T)x[0], x[1] - (float)(T)x[1],
+             x[2] - (float)(T)x[2], x[3] - (float)(T)x[3]);
 }
 
 // The tiles that a block visits: those whose documents meet its own, in
@@ -600,22 +627,23 @@ void forward_kernel(const Args a, const int2* ranges,
                 if (!meet(r, wave_docs)) continue;
                 mixed |= !one_document(r, wave_docs);
             }
-            f.step(tile_k, tile_v, docs, at, mixed, a.causal);
+            f.template step<N / 32>(
+                [&](int t, int n) { return rows_of<T, G::LD>(tile_k, t * 32, n * 16); }, tile_v,
+                docs, at, mixed, a.causal);
         }
     }
 
     const float total = add_halves(f.total);
     const float inv = total == 0.f ? 0.f : 1.f / total;
     if (there) {
-        T* out = row<T>(a.out, b, i, h);
 #pragma unroll
         for (int n = 0; n < DP / 32; ++n)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 int d = n * 32 + r * 8 + (lane >> 5) * 4;
-                if (d < a.d)
-                    put4(out + d, f.o[n][r * 4] * inv, f.o[n][r * 4 + 1] * inv,
-                         f.o[n][r * 4 + 2] * inv, f.o[n][r * 4 + 3] * inv);
+                float x[4] = {f.o[n][r * 4] * inv, f.o[n][r * 4 + 1] * inv,
+                              f.o[n][r * 4 + 2] * inv, f.o[n][r * 4 + 3] * inv};
+                if (d < a.d) put_out<T>(a, b, i, h, d, x);
             }
         if (a.lse && lane < 32)
             a.lse[((int64_t)b * a.hq + h) * a.sq + i] =
@@ -629,7 +657,186 @@ void forward_kernel(const Args a, const int2* ranges,
         forward_row<T>(a, b, h, row0 + __builtin_ctzll(rows));
 }
 
+// Few queries over many keys: bound by one read of K and V.  A wave takes up
+// to 32 columns, which are the queries of all heads of one key-value head, and
+// one part of the keys; nothing is shared between waves.  K's fragments are
+// rows as they lie in memory and go straight to registers, V passes through
+// shared memory for its columns; both travel a tile ahead.  join_kernel adds
+// the parts up, each with its own exponent.
+template <typename T, int DP>
+__global__ __launch_bounds__(64, DP >= 96 ? 1 : 2) void split_kernel(const Args a, int parts, int keys_each,
+                                                   int column_tiles, float* part_o,
+                                                   float2* part_state) {
+    using G = Tile<T, DP>;
+    constexpr int N = 32;
+    __shared__ alignas(16) T tile_v[N * G::LD];
+    __shared__ alignas(16) int docs[N];
+
+    unsigned id = xcd_order(blockIdx.x, gridDim.x);
+    const int part = id % parts, ct = id / parts % column_tiles;
+    const int g = id / parts / column_tiles % a.hkv, b = id / parts / column_tiles / a.hkv;
+    const int lane = threadIdx.x, hf = lane >> 5, group = a.hq / a.hkv, first = a.sk - a.sq;
+    const int columns = group * a.sq, column = ct * 32 + (lane & 31);
+    const bool there = column < columns;
+    const int h = g * group + (there ? column / a.sq : 0), i = there ? column % a.sq : 0;
+    const int* doc_row = a.documents ? a.documents + b * a.documents_sb : nullptr;
+
+    Forward<T, DP> f;
+    f.begin(a, row<T>(a.q, b, i, h), there, slope_of(a, h));
+    f.scaled = __any(f.scaled);
+    f.pos = i + first;
+    const int doc = there ? doc_row ? doc_row[f.pos] : 0 : -1;
+    f.doc = doc < 0 ? INT_MIN : doc;
+    const int2 own = range_of_wave(doc);
+    int latest = there ? f.pos : 0, earliest = there ? f.pos : a.sk;
+    for (int m = 32; m; m >>= 1) {
+        latest = max(latest, __shfl_xor(latest, m));
+        earliest = min(earliest, __shfl_xor(earliest, m));
+    }
+    int end = min(a.sk, (part + 1) * keys_each);
+    if (a.causal) end = min(end, latest + 1);
+    const T *k = row<T>(a.k, b, 0, g), *v = row<T>(a.v, b, 0, g);
+
+    Frag<T> next_k[DP / 16];
+    Stage<T, DP, N, 64> sv;
+    for (int chunk = part * keys_each; chunk < end; chunk += 64 * N) {
+        // tiles with a key that some query may see, of 64
+        const int tiles = min(64, (end - chunk + N - 1) / N);
+        uint64_t visits = tiles == 64 ? ~0ull : (1ull << tiles) - 1;
+        if (doc_row) {
+            visits = 0;
+            for (int t = 0; t < tiles; t += 2) {
+                int j = chunk + t * N + lane, d = j < end ? doc_row[j] : -1;
+                uint64_t met = __ballot(d >= (own.x & NONE) && d <= own.y);
+                if (met & 0xffffffffull) visits |= 1ull << t;
+                if (met >> 32) visits |= 2ull << t;
+            }
+        }
+        int key_doc = -1;
+        auto fetch = [&](int at) {
+            const bool row_there = at + (lane & 31) < a.sk;
+            const T* kr = k + (int64_t)(row_there ? at + (lane & 31) : at) * a.k.ss;
+#pragma unroll
+            for (int n = 0; n < DP / 16; ++n)
+                next_k[n] = row_frag<T>(kr, n * 16 + hf * 8, a.d, row_there);
+            sv.load(v + (int64_t)at * a.v.ss, a.v.ss, a.sk - at, a.d);
+            int j = at + lane;
+            if (lane < N) key_doc = j < a.sk ? doc_row ? max(doc_row[j], -1) : 0 : -1;
+        };
+        int at = visits ? chunk + __builtin_ctzll(visits) * N : 0;
+        if (visits) fetch(at);
+        while (visits) {
+            visits &= visits - 1;
+            // one wave: its own reads and writes of shared memory keep order
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            sv.store(tile_v);
+            if (lane < N) docs[lane] = key_doc;
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            Frag<T> k_now[DP / 16];
+#pragma unroll
+            for (int n = 0; n < DP / 16; ++n) k_now[n] = next_k[n];
+            const int now = at;
+            if (visits) {
+                at = chunk + __builtin_ctzll(visits) * N;
+                fetch(at);
+            }
+            const bool mixed = doc_row || now + N > a.sk || (a.causal && now + N - 1 > earliest);
+            f.template step<1>([&](int, int n) { return k_now[n]; }, tile_v, docs, now, mixed,
+                               a.causal);
+        }
+    }
+
+    const float total = add_halves(f.total);
+    if (!there) return;
+    const int64_t at = (((int64_t)b * a.hkv + g) * columns + column) * parts + part;
+#pragma unroll
+    for (int n = 0; n < DP / 32; ++n)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            put4(part_o + at * DP + n * 32 + r * 8 + hf * 4, f.o[n][r * 4], f.o[n][r * 4 + 1],
+                 f.o[n][r * 4 + 2], f.o[n][r * 4 + 3]);
+    if (hf == 0) part_state[at] = make_float2(f.off, total);
+}
+
+constexpr int MOST_PARTS = 256;
+
+// One row a block: the parts' exponents and sums first, then their values in
+// 256 / DP shares of the parts.
+template <typename T, int DP>
+__global__ __launch_bounds__(256) void join_kernel(const Args a, int parts, const float* part_o,
+                                                   const float2* part_state) {
+    __shared__ float weight[MOST_PARTS], shared[8], values[256];
+    __shared__ int lost;
+    const int group = a.hq / a.hkv, columns = group * a.sq;
+    const int column = blockIdx.x % columns, g = blockIdx.x / columns % a.hkv;
+    const int b = blockIdx.x / columns / a.hkv, h = g * group + column / a.sq, i = column % a.sq;
+    const int tid = threadIdx.x, wave = tid >> 6;
+    const float2 state = tid < parts ? part_state[(int64_t)blockIdx.x * parts + tid]
+                                     : make_float2(0.f, 0.f);
+    const float exponent = state.y == 0.f ? -INFINITY : state.x;
+    float most = wave_max(exponent);
+    if ((tid & 63) == 0) shared[wave] = most;
+    if (tid == 0) lost = 0;
+    __syncthreads();
+    most = fmaxf(fmaxf(shared[0], shared[1]), fmaxf(shared[2], shared[3]));
+    const float w = state.y == 0.f ? 0.f : exp2_fast(exponent - most);
+    float total = wave_sum(w * state.y);
+    weight[tid] = w;
+    if ((tid & 63) == 0) shared[4 + wave] = total;
+    __syncthreads();
+    total = shared[4] + shared[5] + shared[6] + shared[7];
+    const float inv = total == 0.f ? 0.f : 1.f / total;
+
+    constexpr int SHARES = 256 / DP;
+    const int d = tid % DP, share = tid / DP;
+    float o = 0;
+    if (share < SHARES) {
+        const float* from = part_o + (int64_t)blockIdx.x * parts * DP + d;
+#pragma unroll 4
+        for (int p = share; p < parts; p += SHARES)
+            if (weight[p] != 0.f) o = fmaf(weight[p], from[(int64_t)p * DP], o);
+    }
+    values[tid] = o;
+    __syncthreads();
+    if (tid < a.d) {
+        o = 0;
+        for (int n = 0; n < SHARES; ++n) o += values[n * DP + tid];
+        o *= inv;
+        T* out = row<T>(a.out, b, i, h);
+        out[tid] = (T)o;
+        if (a.rest.at) row<T>(a.rest, b, i, h)[tid] = (T)(o - (float)(T)o);
+        if (!(fabsf(o) <= 3.4028235e38f)) lost = 1;
+    }
+    if (tid == 0 && a.lse)
+        a.lse[((int64_t)b * a.hq + h) * a.sq + i] = total == 0.f ? -INFINITY : most + log2f(total);
+    __syncthreads();
+    if (lost && wave == 0) forward_row<T>(a, b, h, i);  // as in forward_kernel
+}
+
 int padded(int d) { return (d + 31) / 32 * 32; }
+
+// Whether the forward pass is split over the keys: where 64 queries a block
+// give fewer blocks than there are CUs.
+bool split_keys(const Args& a) { return (int64_t)a.b * a.hq * ((a.sq + 63) / 64) < 256; }
+
+template <typename T, int DP>
+void launch_split(const Args& a, const torch::Tensor& like, hipStream_t stream) {
+    int64_t columns = (int64_t)(a.hq / a.hkv) * a.sq, tiles = (columns + 31) / 32;
+    int64_t units = tiles * a.b * a.hkv, rows = (int64_t)a.b * a.hkv * columns;
+    // 8 waves a CU, each with 2 tiles of 32 keys at least
+    int64_t parts = std::min<int64_t>({std::max<int64_t>(1, 2048 / units),
+                                       std::max<int64_t>(1, a.sk / 64), MOST_PARTS});
+    int64_t each = ((a.sk + parts - 1) / parts + 31) / 32 * 32;
+    parts = (a.sk + each - 1) / each;
+    auto f32 = like.options().dtype(torch::kFloat32);
+    auto part_o = torch::empty({rows, parts, DP}, f32), state = torch::empty({rows, parts, 2}, f32);
+    hipLaunchKernelGGL((split_kernel<T, DP>), dim3((unsigned)(units * parts)), dim3(64), 0, stream,
+                       a, (int)parts, (int)each, (int)tiles, part_o.data_ptr<float>(),
+                       (float2*)state.data_ptr<float>());
+    hipLaunchKernelGGL((join_kernel<T, DP>), dim3((unsigned)rows), dim3(256), 0, stream, a,
+                       (int)parts, part_o.data_ptr<float>(),
+                       (const float2*)state.data_ptr<float>());
+}
 
 template <typename T, int DP>
 void launch_forward(const Args& a, const int2* ranges, int ranges_n, hipStream_t stream) {
@@ -666,7 +873,9 @@ template <typename T> constexpr bool FACTORED = std::is_same<T, _Float16>::value
 // rows that saw nothing have probabilities of zero
 __device__ __forceinline__ float usable(float lse) { return lse == -INFINITY ? INFINITY : lse; }
 
-// 64 rows a block, 4 threads a row; one read of dout and out bounds it
+// 64 rows a block, 4 threads a row; one read of dout, out and rest bounds it.
+// Where few keys hold a row, do.v_j and delta nearly cancel: delta takes out
+// with the bits that its rounding lost.
 template <typename T>
 __global__ __launch_bounds__(256) void delta_kernel(const Args a, int tiles, float* factors) {
     int t = blockIdx.x % tiles, h = blockIdx.x / tiles % a.hq, b = blockIdx.x / tiles / a.hq;
@@ -674,11 +883,13 @@ __global__ __launch_bounds__(256) void delta_kernel(const Args a, int tiles, flo
     float sum = 0, most = 0;
     if (i < a.sq) {
         const T *x = row<T>(a.dout, b, i, h), *y = row<T>(a.out, b, i, h);
+        const T* z = a.rest.at ? row<T>(a.rest, b, i, h) : nullptr;
         for (int d = (threadIdx.x & 3) * 8; d < a.d; d += 32) {
-            Frag<T> u = *(const Frag<T>*)(x + d), w = *(const Frag<T>*)(y + d);
+            Frag<T> u = *(const Frag<T>*)(x + d), w = *(const Frag<T>*)(y + d), r = {};
+            if (z) r = *(const Frag<T>*)(z + d);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                sum = fmaf((float)u[e], (float)w[e], sum);
+                sum = fmaf((float)u[e], (float)w[e] + (float)r[e], sum);
                 float size = fabsf((float)u[e]);
                 if (FACTORED<T> && size < INFINITY) most = fmaxf(most, size);
             }
@@ -821,14 +1032,7 @@ void dq_kernel(const Args a, const int2* ranges, int ranges_n, int tiles_q, cons
                 }
 #pragma unroll
                 for (int e = 0; e < 16; ++e) s[e] = exp2_fast(s[e]) * (dp[e] - delta);
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    Frag<T> ds = to_frag<T>(s, u * 8);
-#pragma unroll
-                    for (int n = 0; n < DP / 32; ++n)
-                        acc[n] = mma(columns_of<T, G::LD>(tile_k, t * 32 + u * 16, n * 32), ds,
-                                     acc[n]);
-                }
+                add_product<T, DP>(tile_k, t * 32, s, acc);
             }
         }
     }
@@ -854,7 +1058,7 @@ void dq_kernel(const Args a, const int2* ranges, int ranges_n, int tiles_q, cons
 }
 
 template <typename T, int DP, int WAVES>
-__global__ __launch_bounds__(WAVES * 64, DP >= 96 ? 1 : 2)
+__global__ __launch_bounds__(WAVES * 64, DP >= 96 || (DP == 64 && sizeof(T) == 4) ? 1 : 2)
 void dkv_kernel(const Args a, const int2* ranges, int ranges_n, int tiles_k, const float* factors,
                 int factors_n) {
     using G = Tile<T, DP>;
@@ -999,15 +1203,8 @@ void dkv_kernel(const Args a, const int2* ranges, int ranges_n, int tiles_k, con
                     s[e] = exp2_fast(s[e]);
                     dp[e] *= s[e];
                 }
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    Frag<T> p = to_frag<T>(s, u * 8), ds = to_frag<T>(dp, u * 8);
-#pragma unroll
-                    for (int n = 0; n < DP / 32; ++n) {
-                        dv[n] = mma(columns_of<T, G::LD>(tile_o, t * 32 + u * 16, n * 32), p, dv[n]);
-                        dk[n] = mma(columns_of<T, G::LD>(tile_q, t * 32 + u * 16, n * 32), ds, dk[n]);
-                    }
-                }
+                add_product<T, DP>(tile_o, t * 32, s, dv);
+                add_product<T, DP>(tile_q, t * 32, dp, dk);
             }
         }
     }
@@ -1159,23 +1356,31 @@ std::vector<torch::Tensor> attention_forward(torch::Tensor q, torch::Tensor k, t
     a.q = view(q), a.k = view(k), a.v = view(v), a.out = view(out);
     a.lse = want_lse ? lse.data_ptr<float>() : nullptr;
     hipStream_t stream = at::hip::getCurrentHIPStream();
-    if (out.numel() == 0) return {out, lse};
+    // the backward's delta needs the bits that 16-bit outputs lose
+    auto rest = want_lse && q.element_size() == 2 ? torch::empty_like(out)
+                                                  : torch::empty({0}, q.options());
+    if (rest.numel()) a.rest = view(rest);
+    if (out.numel() == 0) return {out, lse, rest};
+    const bool split = split_keys(a);
     torch::Tensor ranges;
-    if (documents) ranges = ranges_for(a, 0, q, stream);
+    if (documents && !split) ranges = ranges_for(a, 0, q, stream);
     for_type(q.scalar_type(), [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
         for_width(a.d, [&](auto width) {
-            launch_forward<T, decltype(width)::value>(
-                a, documents ? (const int2*)ranges.data_ptr<int>() : nullptr,
-                documents ? (int)ranges.size(1) : 0, stream);
+            if (split)
+                launch_split<T, decltype(width)::value>(a, q, stream);
+            else
+                launch_forward<T, decltype(width)::value>(
+                    a, documents ? (const int2*)ranges.data_ptr<int>() : nullptr,
+                    documents ? (int)ranges.size(1) : 0, stream);
         });
     });
-    return {out, lse};
+    return {out, lse, rest};
 }
 
 std::vector<torch::Tensor> attention_backward(torch::Tensor dout, torch::Tensor q,
                                               torch::Tensor k, torch::Tensor v, torch::Tensor out,
-                                              torch::Tensor lse,
+                                              torch::Tensor rest, torch::Tensor lse,
                                               std::optional<torch::Tensor> documents,
                                               std::optional<torch::Tensor> slopes, bool causal,
                                               double scale) {
@@ -1194,6 +1399,11 @@ std::vector<torch::Tensor> attention_backward(torch::Tensor dout, torch::Tensor 
     auto dk = torch::empty(k.sizes(), k.options());
     auto dv = torch::empty(v.sizes(), v.options());
     auto delta = torch::empty(lse.sizes(), lse.options());
+    TORCH_CHECK(rest.numel() == 0 || (rest.sizes() == q.sizes() && rest.is_contiguous() &&
+                                      rest.device() == q.device() &&
+                                      rest.scalar_type() == q.scalar_type()),
+                "rest must be the forward's");
+    if (rest.numel()) a.rest = view(rest);
     a.q = view(q), a.k = view(k), a.v = view(v), a.out = view(out), a.dout = view(dout);
     a.dq = view(dq), a.dk = view(dk), a.dv = view(dv);
     a.lse = lse.data_ptr<float>();

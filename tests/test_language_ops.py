@@ -214,7 +214,8 @@ def test_attention(device, dtype, shape, docs):
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
 @pytest.mark.parametrize("shape", [(1, 1000, 1000, 2, 1, 64), (1, 700, 1111, 2, 2, 128),
-                                   (2, 1, 5003, 4, 2, 64), (1, 7, 2049, 3, 1, 32)], ids=str)
+                                   (2, 1, 5003, 4, 2, 64), (1, 7, 2049, 3, 1, 32),
+                                   (1, 45, 3001, 4, 2, 96), (40, 2, 131, 12, 4, 128)], ids=str)
 def test_attention_long(dtype, shape):
     b, sq, sk, hq, hkv, d = shape
     q, k, v, dout = attention_inputs(*shape, dtype, "cuda", seed=sum(shape))
