@@ -186,13 +186,11 @@ def attention_forward(q, k, v, documents, slopes, causal, scale, want_lse):
     base = torch.where(lse == float("-inf"), torch.zeros_like(lse), lse)
     p = torch.where(seen, torch.exp(s - base.unsqueeze(-1)), torch.zeros_like(s))
     vf = v.float().transpose(1, 2).repeat_interleave(q.shape[2] // v.shape[2], 1)
-    whole = _masked_product(p, vf, seen).transpose(1, 2).contiguous()
-    out = whole.to(q.dtype)
-    # what the backward needs: the rows' sums, and what rounding took from out
-    return (out, lse, whole - out.float()) if want_lse else (out, None, None)
+    out = _masked_product(p, vf, seen).transpose(1, 2).contiguous().to(q.dtype)
+    return out, lse if want_lse else None
 
 
-def attention_backward(dout, q, k, v, out, rest, lse, documents, slopes, causal, scale):
+def attention_backward(dout, q, k, v, out, lse, documents, slopes, causal, scale):
     s, seen = _attention_parts(q, k, documents, slopes, causal, scale)
     group = q.shape[2] // k.shape[2]
     seen = seen & (lse != float("-inf")).unsqueeze(-1)
@@ -200,8 +198,9 @@ def attention_backward(dout, q, k, v, out, rest, lse, documents, slopes, causal,
     p = torch.where(seen, torch.exp(s - lse.unsqueeze(-1)), zero)
     qf, do = q.float().transpose(1, 2), dout.float().transpose(1, 2)
     kf, vf = (t.float().transpose(1, 2).repeat_interleave(group, 1) for t in (k, v))
-    delta = (do * (out.float() + rest).transpose(1, 2)).sum(-1, keepdim=True)
-    ds = torch.where(seen, p * (torch.matmul(do, vf.transpose(2, 3)) - delta), zero)
+    dp = torch.where(seen, torch.matmul(do, vf.transpose(2, 3)), zero)
+    ds = p * (dp - (p * dp).sum(-1, keepdim=True))
+    ds = torch.where(seen, ds, zero)
     dq = _masked_product(ds, kf, seen) * scale
     back = seen.transpose(2, 3)
     dk = _masked_product(ds.transpose(2, 3), qf, back) * scale

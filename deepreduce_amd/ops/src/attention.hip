@@ -34,7 +34,7 @@ struct View {
 };
 
 struct Args {
-    View q, k, v, out, rest, dout, dq, dk, dv;  // rest: what rounding took from out
+    View q, k, v, out, dout, dq, dk, dv;
     float* lse;              // [batch, hq, sq], in log2 units
     float* delta;            // [batch, hq, sq]
     const int* documents;    // [batch, sk] or none
@@ -126,46 +126,46 @@ __device__ void forward_row(const Args& a, int b, int h, int i) {
         }
     }
     T* out = row<T>(a.out, b, i, h);
-    for (int n = 0; n < 2; ++n)
-        if (int d = lane + n * 64; d < a.d) {
-            out[d] = (T)o[n];
-            if (a.rest.at) row<T>(a.rest, b, i, h)[d] = (T)(o[n] - (float)out[d]);
-        }
+    if (lane < a.d) out[lane] = (T)o[0];
+    if (lane + 64 < a.d) out[lane + 64] = (T)o[1];
     if (lane == 0 && a.lse)
         a.lse[((int64_t)b * a.hq + h) * a.sq + i] = total == 0.f ? -INFINITY : base + log2f(total);
 }
 
+// also leaves the row's delta, from probabilities of 32 bits
 template <typename T>
 __device__ void dq_row(const Args& a, int b, int h, int i) {
     const int lane = threadIdx.x & 63, g = h / (a.hq / a.hkv), pos = i + a.sk - a.sq;
     const float slope = slope_of(a, h);
     const int64_t at = ((int64_t)b * a.hq + h) * a.sq + i;
-    const float lse = a.lse[at], delta = a.delta[at];
+    const float lse = a.lse[at];
     const T *q = row<T>(a.q, b, i, h), *dout = row<T>(a.dout, b, i, h);
-    float acc[2] = {0, 0};
-    const int end = a.causal ? pos + 1 : a.sk;
-    if (lse != -INFINITY)
-        for (int j0 = 0; j0 < end; j0 += 64) {
-            int j = j0 + lane;
-            bool seen = j < end && visible(a, b, pos, j);
-            uint64_t any = __ballot(seen);
-            float ds = 0;
-            if (seen) {
-                float s = dot(q, row<T>(a.k, b, j, g), a.d) * (a.scale * LOG2E) -
-                          slope * abs(pos - j);
-                ds = exp2_fast(s - lse) * (dot(dout, row<T>(a.v, b, j, g), a.d) - delta);
-            }
-            for (; any; any &= any - 1) {
-                int n = __builtin_ctzll(any);
-                float w = __shfl(ds, n);
-                const T* k = row<T>(a.k, b, j0 + n, g);
-                if (lane < a.d) acc[0] = fmaf(w, (float)k[lane], acc[0]);
-                if (lane + 64 < a.d) acc[1] = fmaf(w, (float)k[lane + 64], acc[1]);
-            }
+    float acc[2] = {0, 0}, delta = 0;
+    const int end = lse == -INFINITY ? 0 : a.causal ? pos + 1 : a.sk;
+    auto p_of = [&](int j) {
+        return exp2_fast(dot(q, row<T>(a.k, b, j, g), a.d) * (a.scale * LOG2E) -
+                         slope * abs(pos - j) - lse);
+    };
+    for (int j = lane; j < end; j += 64)
+        if (visible(a, b, pos, j))
+            delta = fmaf(p_of(j), dot(dout, row<T>(a.v, b, j, g), a.d), delta);
+    delta = wave_sum(delta);
+    for (int j0 = 0; j0 < end; j0 += 64) {
+        int j = j0 + lane;
+        bool seen = j < end && visible(a, b, pos, j);
+        float ds = seen ? p_of(j) * (dot(dout, row<T>(a.v, b, j, g), a.d) - delta) : 0.f;
+        for (uint64_t any = __ballot(seen); any; any &= any - 1) {
+            int n = __builtin_ctzll(any);
+            float w = __shfl(ds, n);
+            const T* k = row<T>(a.k, b, j0 + n, g);
+            if (lane < a.d) acc[0] = fmaf(w, (float)k[lane], acc[0]);
+            if (lane + 64 < a.d) acc[1] = fmaf(w, (float)k[lane + 64], acc[1]);
         }
+    }
     T* dq = row<T>(a.dq, b, i, h);
     if (lane < a.d) dq[lane] = (T)(acc[0] * a.scale);
     if (lane + 64 < a.d) dq[lane + 64] = (T)(acc[1] * a.scale);
+    if (lane == 0) a.delta[at] = delta;
 }
 
 template <typename T>
@@ -516,16 +516,6 @@ __device__ __forceinline__ void put4(T* at, float a, float b, float c, float d) 
     *(Four*)at = Four{(T)a, (T)b, (T)c, (T)d};
 }
 
-// an output row's four values, and what rounding took from them
-template <typename T>
-__device__ __forceinline__ void put_out(const Args& a, int b, int i, int h, int d, const float* x) {
-    T* out = row<T>(a.out, b, i, h) + d;
-    put4(out, x[0], x[1], x[2], x[3]);
-    if (a.rest.at)
-        put4(row<T>(a.rest, b, i, h) + d, x[0] - (float)(T)x[0], x[1] - (float)(T)x[1],
-             x[2] - (float)(T)x[2], x[3] - (float)(T)x[3]);
-}
-
 // The tiles that a block visits: those whose documents meet its own, in
 // order, THREADS candidates at a time.
 template <int THREADS> struct Visits {
@@ -636,14 +626,15 @@ void forward_kernel(const Args a, const int2* ranges,
     const float total = add_halves(f.total);
     const float inv = total == 0.f ? 0.f : 1.f / total;
     if (there) {
+        T* out = row<T>(a.out, b, i, h);
 #pragma unroll
         for (int n = 0; n < DP / 32; ++n)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 int d = n * 32 + r * 8 + (lane >> 5) * 4;
-                float x[4] = {f.o[n][r * 4] * inv, f.o[n][r * 4 + 1] * inv,
-                              f.o[n][r * 4 + 2] * inv, f.o[n][r * 4 + 3] * inv};
-                if (d < a.d) put_out<T>(a, b, i, h, d, x);
+                if (d < a.d)
+                    put4(out + d, f.o[n][r * 4] * inv, f.o[n][r * 4 + 1] * inv,
+                         f.o[n][r * 4 + 2] * inv, f.o[n][r * 4 + 3] * inv);
             }
         if (a.lse && lane < 32)
             a.lse[((int64_t)b * a.hq + h) * a.sq + i] =
@@ -802,9 +793,7 @@ __global__ __launch_bounds__(256) void join_kernel(const Args a, int parts, cons
         o = 0;
         for (int n = 0; n < SHARES; ++n) o += values[n * DP + tid];
         o *= inv;
-        T* out = row<T>(a.out, b, i, h);
-        out[tid] = (T)o;
-        if (a.rest.at) row<T>(a.rest, b, i, h)[tid] = (T)(o - (float)(T)o);
+        row<T>(a.out, b, i, h)[tid] = (T)o;
         if (!(fabsf(o) <= 3.4028235e38f)) lost = 1;
     }
     if (tid == 0 && a.lse)
@@ -870,12 +859,16 @@ constexpr int FACTOR_ROWS = 64;
 
 template <typename T> constexpr bool FACTORED = std::is_same<T, _Float16>::value;
 
+// delta from 16-bit outputs is off by their roundings and those of their
+// probabilities, which shows where few keys hold a row and do.v_j - delta
+// nearly cancels.  The sum of P (do.v_j - delta), which would be 0, says by
+// how much: dq is set right with the sum of P k, and dk takes the right delta.
+template <typename T> constexpr bool CORRECTED = sizeof(T) == 2;
+
 // rows that saw nothing have probabilities of zero
 __device__ __forceinline__ float usable(float lse) { return lse == -INFINITY ? INFINITY : lse; }
 
-// 64 rows a block, 4 threads a row; one read of dout, out and rest bounds it.
-// Where few keys hold a row, do.v_j and delta nearly cancel: delta takes out
-// with the bits that its rounding lost.
+// 64 rows a block, 4 threads a row; one read of dout and out bounds it
 template <typename T>
 __global__ __launch_bounds__(256) void delta_kernel(const Args a, int tiles, float* factors) {
     int t = blockIdx.x % tiles, h = blockIdx.x / tiles % a.hq, b = blockIdx.x / tiles / a.hq;
@@ -883,13 +876,11 @@ __global__ __launch_bounds__(256) void delta_kernel(const Args a, int tiles, flo
     float sum = 0, most = 0;
     if (i < a.sq) {
         const T *x = row<T>(a.dout, b, i, h), *y = row<T>(a.out, b, i, h);
-        const T* z = a.rest.at ? row<T>(a.rest, b, i, h) : nullptr;
         for (int d = (threadIdx.x & 3) * 8; d < a.d; d += 32) {
-            Frag<T> u = *(const Frag<T>*)(x + d), w = *(const Frag<T>*)(y + d), r = {};
-            if (z) r = *(const Frag<T>*)(z + d);
+            Frag<T> u = *(const Frag<T>*)(x + d), w = *(const Frag<T>*)(y + d);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                sum = fmaf((float)u[e], (float)w[e] + (float)r[e], sum);
+                sum = fmaf((float)u[e], (float)w[e], sum);
                 float size = fabsf((float)u[e]);
                 if (FACTORED<T> && size < INFINITY) most = fmaxf(most, size);
             }
@@ -911,7 +902,7 @@ __global__ __launch_bounds__(256) void delta_kernel(const Args a, int tiles, flo
 }
 
 template <typename T, int DP, int WAVES>
-__global__ __launch_bounds__(WAVES * 64, DP == 128 ? 1 : 2)
+__global__ __launch_bounds__(WAVES * 64, DP >= 96 ? 1 : 2)
 void dq_kernel(const Args a, const int2* ranges, int ranges_n, int tiles_q, const float* factors,
                int factors_n) {
     using G = Tile<T, DP>;
@@ -939,15 +930,14 @@ void dq_kernel(const Args a, const int2* ranges, int ranges_n, int tiles_q, cons
         dout[n] = row_frag<T>(row<T>(a.dout, b, there ? i : 0, h), n * 16 + hf * 8, a.d, there);
         if (a.scale < 0) q[n] = -q[n];
     }
-    acc16 acc[DP / 32];
+    acc16 acc[DP / 32], mean[DP / 32];  // mean: sum of P k
 #pragma unroll
-    for (int n = 0; n < DP / 32; ++n) acc[n] = acc16{};
+    for (int n = 0; n < DP / 32; ++n) acc[n] = acc16{}, mean[n] = acc16{};
     const float delta = there ? a.delta[at_row] : 0.f;
-    float off = there ? usable(a.lse[at_row]) : INFINITY, back = a.scale;
+    float off = there ? usable(a.lse[at_row]) : INFINITY, rest = 0, factor = 1.f;
     if constexpr (FACTORED<T>) {
-        float f = factors[((int64_t)b * a.hq + h) * factors_n + min(i, a.sq - 1) / FACTOR_ROWS];
-        off -= SHIFT + log2f(f);
-        back *= exp2f(-SHIFT) / f;
+        factor = factors[((int64_t)b * a.hq + h) * factors_n + min(i, a.sq - 1) / FACTOR_ROWS];
+        off -= SHIFT;
     }
 
     const int seen = there ? doc_row ? doc_row[pos] : 0 : -1;
@@ -1030,14 +1020,38 @@ void dq_kernel(const Args a, const int2* ranges, int ranges_n, int tiles_q, cons
                         }
                     }
                 }
+                float sum = 0;
 #pragma unroll
-                for (int e = 0; e < 16; ++e) s[e] = exp2_fast(s[e]) * (dp[e] - delta);
-                add_product<T, DP>(tile_k, t * 32, s, acc);
+                for (int e = 0; e < 16; ++e) {
+                    s[e] = exp2_fast(s[e]);
+                    if constexpr (FACTORED<T>)
+                        dp[e] = s[e] * fmaf(dp[e], factor, -delta * factor);
+                    else
+                        dp[e] = s[e] * (dp[e] - delta);
+                    sum += dp[e];
+                }
+                add_product<T, DP>(tile_k, t * 32, dp, acc);
+                if constexpr (CORRECTED<T>) {
+                    rest += sum;
+                    add_product<T, DP>(tile_k, t * 32, s, mean);
+                }
             }
         }
     }
 
     bool fine = true;
+    float back = a.scale;
+    if constexpr (FACTORED<T>) back *= exp2f(-SHIFT) / factor;
+    if constexpr (CORRECTED<T>) {
+        rest = add_halves(rest);
+        fine = fabsf(rest) <= 3.4028235e38f;
+        float by = FACTORED<T> ? rest * exp2f(-SHIFT) : rest;
+#pragma unroll
+        for (int n = 0; n < DP / 32; ++n)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[n][e] = fmaf(-by, mean[n][e], acc[n][e]);
+        if (there && hf == 0) a.delta[at_row] = FACTORED<T> ? delta + by / factor : delta + rest;
+    }
     if (there) {
         T* dq = row<T>(a.dq, b, i, h);
 #pragma unroll
@@ -1052,7 +1066,7 @@ void dq_kernel(const Args a, const int2* ranges, int ranges_n, int tiles_q, cons
                 for (int e = 0; e < 4; ++e) fine &= fabsf(acc[n][r * 4 + e]) <= 3.4028235e38f;
             }
     }
-    uint64_t bad = __ballot(!fine);
+    uint64_t bad = __ballot(there && !fine);
     for (uint64_t rows = (bad | bad >> 32) & 0xffffffffull; rows; rows &= rows - 1)
         dq_row<T>(a, b, h, row0 + __builtin_ctzll(rows));
 }
@@ -1356,11 +1370,7 @@ std::vector<torch::Tensor> attention_forward(torch::Tensor q, torch::Tensor k, t
     a.q = view(q), a.k = view(k), a.v = view(v), a.out = view(out);
     a.lse = want_lse ? lse.data_ptr<float>() : nullptr;
     hipStream_t stream = at::hip::getCurrentHIPStream();
-    // the backward's delta needs the bits that 16-bit outputs lose
-    auto rest = want_lse && q.element_size() == 2 ? torch::empty_like(out)
-                                                  : torch::empty({0}, q.options());
-    if (rest.numel()) a.rest = view(rest);
-    if (out.numel() == 0) return {out, lse, rest};
+    if (out.numel() == 0) return {out, lse};
     const bool split = split_keys(a);
     torch::Tensor ranges;
     if (documents && !split) ranges = ranges_for(a, 0, q, stream);
@@ -1375,12 +1385,12 @@ std::vector<torch::Tensor> attention_forward(torch::Tensor q, torch::Tensor k, t
                     documents ? (int)ranges.size(1) : 0, stream);
         });
     });
-    return {out, lse, rest};
+    return {out, lse};
 }
 
 std::vector<torch::Tensor> attention_backward(torch::Tensor dout, torch::Tensor q,
                                               torch::Tensor k, torch::Tensor v, torch::Tensor out,
-                                              torch::Tensor rest, torch::Tensor lse,
+                                              torch::Tensor lse,
                                               std::optional<torch::Tensor> documents,
                                               std::optional<torch::Tensor> slopes, bool causal,
                                               double scale) {
@@ -1399,11 +1409,6 @@ std::vector<torch::Tensor> attention_backward(torch::Tensor dout, torch::Tensor 
     auto dk = torch::empty(k.sizes(), k.options());
     auto dv = torch::empty(v.sizes(), v.options());
     auto delta = torch::empty(lse.sizes(), lse.options());
-    TORCH_CHECK(rest.numel() == 0 || (rest.sizes() == q.sizes() && rest.is_contiguous() &&
-                                      rest.device() == q.device() &&
-                                      rest.scalar_type() == q.scalar_type()),
-                "rest must be the forward's");
-    if (rest.numel()) a.rest = view(rest);
     a.q = view(q), a.k = view(k), a.v = view(v), a.out = view(out), a.dout = view(dout);
     a.dq = view(dq), a.dk = view(dk), a.dv = view(dv);
     a.lse = lse.data_ptr<float>();

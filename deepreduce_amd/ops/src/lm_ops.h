@@ -19,7 +19,7 @@ std::vector<torch::Tensor> attention_forward(torch::Tensor q, torch::Tensor k, t
                                              double scale, bool want_lse);
 std::vector<torch::Tensor> attention_backward(torch::Tensor dout, torch::Tensor q,
                                               torch::Tensor k, torch::Tensor v, torch::Tensor out,
-                                              torch::Tensor rest, torch::Tensor lse,
+                                              torch::Tensor lse,
                                               std::optional<torch::Tensor> documents,
                                               std::optional<torch::Tensor> slopes, bool causal,
                                               double scale);
