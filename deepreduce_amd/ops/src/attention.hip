@@ -249,7 +249,7 @@ __device__ __forceinline__ acc16 mma(f32x8 a, f32x8 b, acc16 c) {
     return c;
 }
 
-constexpr int RANGE = 64;            // positions whose documents share a range
+constexpr int RANGE = 32;            // positions whose documents share a range
 constexpr int NONE = 0x7fffffff;
 
 template <typename T, int DP> struct Tile {
@@ -260,26 +260,38 @@ template <typename T, int DP> struct Tile {
 };
 
 // Rows of one tile on their way from memory to shared memory, through
-// registers so that they travel while the tile before is worked on.
+// registers so that they travel while the tile before is worked on.  Buffer
+// loads take the tile's address from scalar registers and give zero behind
+// its end, so a load costs no address and no comparison.
 template <typename T, int DP, int ROWS, int THREADS> struct Stage {
     using G = Tile<T, DP>;
     static constexpr int N = ROWS * G::VECS / THREADS;
     static_assert(N * THREADS == ROWS * G::VECS, "threads share a tile's vectors evenly");
-    uint4 r[N];
+    typedef unsigned raw4 __attribute__((ext_vector_type(4)));
+    raw4 r[N];
+    int offset[N];   // of this thread's vectors, in bytes; the end for those behind d
+    int row_bytes, d_bytes;
 
-    __device__ __forceinline__ void load(const T* base, int64_t stride, int rows, int d) {
+    __device__ __forceinline__ Stage(int64_t stride, int d)
+        : row_bytes((int)stride * (int)sizeof(T)), d_bytes(d * (int)sizeof(T)) {
 #pragma unroll
         for (int n = 0; n < N; ++n) {
             int v = threadIdx.x + n * THREADS, y = v / G::VECS, x = (v % G::VECS) * G::PER;
-            r[n] = make_uint4(0, 0, 0, 0);
-            if (y < rows && x < d) r[n] = *(const uint4*)(base + y * stride + x);
+            offset[n] = x < d ? y * row_bytes + x * (int)sizeof(T) : 0x7fffffff - 15;
         }
+    }
+    __device__ __forceinline__ void load(const T* base, int rows) {
+        auto buffer = __builtin_amdgcn_make_buffer_rsrc(
+            (void*)base, 0, (min(rows, ROWS) - 1) * row_bytes + d_bytes, 0x00027000);
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+            r[n] = __builtin_amdgcn_raw_buffer_load_b128(buffer, offset[n], 0, 0);
     }
     __device__ __forceinline__ void store(T* tile) const {
 #pragma unroll
         for (int n = 0; n < N; ++n) {
             int v = threadIdx.x + n * THREADS, y = v / G::VECS, x = (v % G::VECS) * G::PER;
-            *(uint4*)(tile + y * G::LD + x) = r[n];
+            *(raw4*)(tile + y * G::LD + x) = r[n];
         }
     }
 };
@@ -362,18 +374,9 @@ __device__ __forceinline__ int row_of(int i) {
     return 8 * (i >> 2) + 4 * ((threadIdx.x & 63) >> 5) + (i & 3);
 }
 
-// The documents of RANGE positions: x is the least of those that are not
+// The documents of some positions: x is the least of those that are not
 // negative (NONE without one), with the top bit set if there are negative
 // ones too, y the largest.
-__device__ __forceinline__ int2 range_of_wave(int doc) {
-    int lo = doc < 0 ? NONE : doc, hi = doc;
-    for (int m = 32; m; m >>= 1) {
-        lo = min(lo, __shfl_xor(lo, m));
-        hi = max(hi, __shfl_xor(hi, m));
-    }
-    if (__any(doc < 0)) lo |= 0x80000000;
-    return make_int2(__builtin_amdgcn_readfirstlane(lo), __builtin_amdgcn_readfirstlane(hi));
-}
 __device__ __forceinline__ bool meet(int2 a, int2 b) {
     return max(a.x & NONE, b.x & NONE) <= min(a.y, b.y);
 }
@@ -381,14 +384,51 @@ __device__ __forceinline__ bool meet(int2 a, int2 b) {
 __device__ __forceinline__ bool one_document(int2 a, int2 b) {
     return a.x == a.y && b.x == b.y && a.x == b.x;
 }
+__device__ __forceinline__ int2 both(int2 a, int2 b) {
+    return make_int2(min(a.x & NONE, b.x & NONE) | ((a.x | b.x) & INT_MIN), max(a.y, b.y));
+}
 
-// ranges [batch, count] of the positions from `first` on
-__global__ __launch_bounds__(64) void ranges_kernel(const int* documents, int64_t sb, int first,
-                                                    int end, int count, int2* ranges) {
-    int t = blockIdx.x % count, b = blockIdx.x / count;
-    int at = first + t * RANGE + threadIdx.x;
-    int2 r = range_of_wave(at < end ? documents[b * sb + at] : -1);
-    if (threadIdx.x == 0) ranges[blockIdx.x] = r;
+// ranges of RANGE positions each, [batch, count], from position `first` on
+struct Ranges {
+    const int2* at;  // none without documents
+    int count;
+
+    __device__ __forceinline__ int2 of(int b, int n) const {
+        return n < count ? at[(int64_t)b * count + n] : make_int2(-1, -1);
+    }
+};
+
+__global__ __launch_bounds__(256) void ranges_kernel(const int* documents, int64_t sb, int first,
+                                                     int end, int count, int64_t all,
+                                                     int2* ranges) {
+    int64_t n = (int64_t)blockIdx.x * (256 / RANGE) + threadIdx.x / RANGE;
+    if (n >= all) return;
+    int at = first + (int)(n % count) * RANGE + threadIdx.x % RANGE;
+    int doc = at < end ? documents[n / count * sb + at] : -1;
+    int2 r = make_int2(doc < 0 ? -1 : doc, doc);
+    for (int m = RANGE / 2; m; m >>= 1)
+        r = both(r, make_int2(__shfl_xor(r.x, m), __shfl_xor(r.y, m)));
+    if (threadIdx.x % RANGE == 0) ranges[n] = r;
+}
+
+// The next 64 tiles, a bit each: `block` those that some position of the
+// block may see, `wave` some of the wave, `whole` those that all of the wave
+// see wholly as far as documents go.  Every wave looks at all 64, one each
+// lane, so that nothing passes between waves.
+struct Visits {
+    uint64_t block, wave, whole;
+};
+template <int SIZE>
+__device__ __forceinline__ Visits visits_of(const Ranges& r, int b, int first, int n, int2 block,
+                                            int2 wave) {
+    const uint64_t all = n >= 64 ? ~0ull : (1ull << n) - 1;
+    if (!r.at) return {all, all, all};
+    const int t = first + (threadIdx.x & 63);
+    int2 x = r.of(b, t * (SIZE / RANGE));
+#pragma unroll
+    for (int m = 1; m < SIZE / RANGE; ++m) x = both(x, r.of(b, t * (SIZE / RANGE) + m));
+    return {__ballot(meet(x, block)) & all, __ballot(meet(x, wave)) & all,
+            __ballot(one_document(x, wave)) & all};
 }
 
 // Workgroups go round the 8 XCDs: neighbours in the order returned run on one
@@ -402,15 +442,43 @@ constexpr float HEADROOM = 3.f;  // how far (log2) a score may pass the referenc
 constexpr float SHIFT = 12.f;    // probabilities carry a factor 2^12, at most 2^15 in all:
                                  // in fp16 the small ones keep their bits
 
+// x[i] = -inf for the keys of other documents, key 32 t + row_of(i); docs of a
+// tile's keys, with -1 behind the last
+__device__ __forceinline__ void hide_documents(acc16& x, const int* docs, int t, int doc) {
+    const int hf = (threadIdx.x & 63) >> 5;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        int4 d = *(const int4*)(docs + t * 32 + r * 8 + 4 * hf);
+        x[r * 4] = d.x == doc ? x[r * 4] : -INFINITY;
+        x[r * 4 + 1] = d.y == doc ? x[r * 4 + 1] : -INFINITY;
+        x[r * 4 + 2] = d.z == doc ? x[r * 4 + 2] : -INFINITY;
+        x[r * 4 + 3] = d.w == doc ? x[r * 4 + 3] : -INFINITY;
+    }
+}
+// ... and for those whose row is past `last`, both counted from the tile's start
+__device__ __forceinline__ void hide_past(acc16& x, int t, int last) {
+    const int l = last - t * 32 - 4 * ((threadIdx.x & 63) >> 5);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] = 8 * (i >> 2) + (i & 3) > l ? -INFINITY : x[i];
+}
+
+// ... or before `begin`
+__device__ __forceinline__ void hide_before(acc16& x, int t, int begin) {
+    const int l = begin - t * 32 - 4 * ((threadIdx.x & 63) >> 5);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] = 8 * (i >> 2) + (i & 3) < l ? -INFINITY : x[i];
+}
+
 // One wave's 32 queries against tiles of keys: the running softmax.
 template <typename T, int DP> struct Forward {
     using G = Tile<T, DP>;
     Frag<T> q[DP / 16];
     acc16 o[DP / 32];
-    float top, off, total;  // reference maximum, what exponents lose, this half's sum
+    float off, total;       // what exponents lose (the reference maximum less SHIFT), this
+                            // half's sum
+    bool fresh;             // nothing seen yet
     float c;                // score factor, in units of log2
     float slope;
-    bool scaled;            // scores are scaled before the maximum is taken
     int doc;                // the lane's query's document, INT_MIN for none
     int pos;                // its position
 
@@ -418,7 +486,6 @@ template <typename T, int DP> struct Forward {
         const int hf = (threadIdx.x & 63) >> 5;
         slope = slope_;
         c = fabsf(a.scale) * LOG2E;
-        scaled = slope != 0.f || c == 0.f;
 #pragma unroll
         for (int n = 0; n < DP / 16; ++n) {
             q[n] = row_frag<T>(row, n * 16 + hf * 8, a.d, there);
@@ -426,16 +493,16 @@ template <typename T, int DP> struct Forward {
         }
 #pragma unroll
         for (int n = 0; n < DP / 32; ++n) o[n] = acc16{};
-        top = -INFINITY;
-        off = -SHIFT;
+        fresh = true;
+        off = 0;
         total = 0;
     }
 
-    // keys key0 .. key0 + 32 KT, k(t, n) the fragments of their rows; `mixed`:
-    // some pairs may be hidden
+    // keys key0 .. key0 + 32 KT, k(t, n) the fragments of their rows; some may
+    // be hidden by their documents or lie past the query
     template <int KT, typename K>
-    __device__ __forceinline__ void step(K k, const T* v, const int* docs, int key0, bool mixed,
-                                         bool causal) {
+    __device__ __forceinline__ void step(K k, const T* v, const int* docs, int key0,
+                                         bool biased, bool by_document, bool by_position) {
         const int hf = (threadIdx.x & 63) >> 5;
         acc16 s[KT];
 #pragma unroll
@@ -444,54 +511,56 @@ template <typename T, int DP> struct Forward {
 #pragma unroll
             for (int n = 0; n < DP / 16; ++n) s[t] = mma(k(t, n), q[n], s[t]);
         }
-        if (scaled) {
-            float far = (float)(pos - key0 - 4 * hf);
+        if (biased) {
+            const float far = (float)(pos - key0 - 4 * hf);
 #pragma unroll
             for (int t = 0; t < KT; ++t)
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
-                    s[t][i] = s[t][i] * c -
-                              slope * fabsf(far - (float)(t * 32 + 8 * (i >> 2) + (i & 3)));
-        }
-        const float cm = scaled ? 1.f : c;
-        if (mixed) {
+                    s[t][i] = fmaf(s[t][i], c,
+                                   fmaf(-slope, fabsf(far - (float)(t * 32 + 8 * (i >> 2) + (i & 3))),
+                                        -off));
+        } else {
 #pragma unroll
             for (int t = 0; t < KT; ++t)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    int at = t * 32 + r * 8 + 4 * hf;
-                    int4 d = *(const int4*)(docs + at);
-                    const int kd[4] = {d.x, d.y, d.z, d.w};
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        bool hidden = kd[e] != doc || (causal && key0 + at + e > pos);
-                        s[t][r * 4 + e] = hidden ? -INFINITY : s[t][r * 4 + e];
-                    }
-                }
+                for (int i = 0; i < 16; ++i) s[t][i] = fmaf(s[t][i], c, -off);
         }
+        if (by_document)
+#pragma unroll
+            for (int t = 0; t < KT; ++t) hide_documents(s[t], docs, t, doc);
+        if (by_position)
+#pragma unroll
+            for (int t = 0; t < KT; ++t) hide_past(s[t], t, pos - key0);
         float most = -INFINITY;
 #pragma unroll
         for (int t = 0; t < KT; ++t)
 #pragma unroll
             for (int i = 0; i < 16; i += 2) most = fmaxf(most, fmaxf(s[t][i], s[t][i + 1]));
-        most = max_halves(most) * cm;
-        if (__any(most > top + HEADROOM)) {
-            float next = fmaxf(top, most);
-            float keep = next == top ? 1.f : exp2_fast(top - next);
-            top = next;
-            off = (top == -INFINITY ? 0.f : top) - SHIFT;
+        most = max_halves(most);
+        if (__any(most > (fresh ? -INFINITY : SHIFT + HEADROOM))) {
+            float by = fresh ? most == -INFINITY ? 0.f : most - SHIFT : fmaxf(most - SHIFT, 0.f);
+            const float next = off + by;
+            by = next - off;  // as far as off really went
+            const float keep = fresh ? 1.f : exp2_fast(-by);
+            fresh = fresh && most == -INFINITY;
+            off = next;
             total *= keep;
 #pragma unroll
             for (int n = 0; n < DP / 32; ++n)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) o[n][i] *= keep;
+#pragma unroll
+            for (int t = 0; t < KT; ++t)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[t][i] -= by;
         }
         float sum = 0;  // a tile's first, so that long rows keep their bits
 #pragma unroll
         for (int t = 0; t < KT; ++t) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                s[t][i] = exp2_fast(fmaf(s[t][i], cm, -off));
+                s[t][i] = exp2_fast(s[t][i]);
                 sum += s[t][i];
             }
             add_product<T, DP>(v, t * 32, s[t], o);
@@ -516,51 +585,23 @@ __device__ __forceinline__ void put4(T* at, float a, float b, float c, float d) 
     *(Four*)at = Four{(T)a, (T)b, (T)c, (T)d};
 }
 
-// The tiles that a block visits: those whose documents meet its own, in
-// order, THREADS candidates at a time.
-template <int THREADS> struct Visits {
-    int list[THREADS];
-    int counts[THREADS / 64];
-
-    __device__ __forceinline__ int fill(int first, int end, int size, const int2* ranges,
-                                        int2 own) {
-        int t = first + threadIdx.x;
-        bool there = t < end && meet(ranges[t * size / RANGE], own);
-        uint64_t all = __ballot(there);
-        int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-        __syncthreads();
-        if (lane == 0) counts[wave] = __popcll(all);
-        __syncthreads();
-        int before = 0, n = 0;
-        for (int w = 0; w < THREADS / 64; ++w) {
-            if (w < wave) before += counts[w];
-            n += counts[w];
-        }
-        if (there) list[before + __popcll(all & ((1ull << lane) - 1))] = t;
-        __syncthreads();
-        return n;
-    }
-};
-
 // 32 queries for each wave, all heads and keys.  The block's waves share the
 // tiles of K and V; block tiles of one head are neighbours on one XCD, whose
 // L2 then serves the head's keys once.
 template <typename T, int DP, int WAVES>
 __global__ __launch_bounds__(WAVES * 64, DP == 128 && (WAVES == 2 || sizeof(T) == 4) ? 1 : 2)
-void forward_kernel(const Args a, const int2* ranges,
-                                                                int ranges_n, int tiles_q) {
+void forward_kernel(const Args a, const Ranges keys, const Ranges queries, int tiles_q) {
     using G = Tile<T, DP>;
     constexpr int THREADS = WAVES * 64, N = G::KEYS;
     __shared__ alignas(16) T tile_k[N * G::LD], tile_v[N * G::LD];
     __shared__ alignas(16) int docs[N];
-    __shared__ int2 own[WAVES];
-    __shared__ Visits<THREADS> visits;
 
     unsigned id = xcd_order(blockIdx.x, gridDim.x);
     int qt = id % tiles_q, h = id / tiles_q % a.hq, b = id / tiles_q / a.hq;
     if (a.causal) qt = tiles_q - 1 - qt;  // the longest first
-    const int g = h / (a.hq / a.hkv), lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int first = a.sk - a.sq, row0 = qt * WAVES * 32 + wave * 32;
+    const int g = h / (a.hq / a.hkv), lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int first = a.sk - a.sq, row0 = (qt * WAVES + wave) * 32;
     const int i = row0 + (lane & 31);
     const bool there = i < a.sq;
     const int* doc_row = a.documents ? a.documents + b * a.documents_sb : nullptr;
@@ -568,58 +609,48 @@ void forward_kernel(const Args a, const int2* ranges,
     Forward<T, DP> f;
     f.begin(a, row<T>(a.q, b, there ? i : 0, h), there, slope_of(a, h));
     f.pos = i + first;
-    int doc = there ? doc_row ? doc_row[f.pos] : 0 : -1;
+    const int doc = there ? doc_row ? doc_row[f.pos] : 0 : -1;
     f.doc = doc < 0 ? INT_MIN : doc;
-    const int2 wave_docs = range_of_wave(doc);
-    int2 block_docs = wave_docs;
+    int2 wave_docs{}, block_docs{};
     if (doc_row) {
-        if (lane == 0) own[wave] = wave_docs;
-        __syncthreads();
-        for (int w = 0; w < WAVES; ++w) {
-            block_docs.x = min(block_docs.x & NONE, own[w].x & NONE);
-            block_docs.y = max(block_docs.y, own[w].y);
-        }
+        wave_docs = queries.of(b, qt * WAVES + wave);
+        block_docs = queries.of(b, qt * WAVES);
+        for (int w = 1; w < WAVES; ++w) block_docs = both(block_docs, queries.of(b, qt * WAVES + w));
     }
     const int wave_first = row0 + first, wave_last = min(row0 + 31, a.sq - 1) + first;
     int end = a.sk;
     if (a.causal) end = min(end, (qt + 1) * WAVES * 32 + first);
     const int tiles = (end + N - 1) / N;
+    const bool biased = f.slope != 0.f;
     const T *k = row<T>(a.k, b, 0, g), *v = row<T>(a.v, b, 0, g);
 
-    Stage<T, DP, N, THREADS> sk, sv;
-    for (int chunk = 0; chunk < tiles; chunk += THREADS) {
-        int n = min(THREADS, tiles - chunk);
-        if (doc_row) n = visits.fill(chunk, tiles, N, ranges + (int64_t)b * ranges_n, block_docs);
-        auto tile_at = [&](int m) { return (doc_row ? visits.list[m] : chunk + m) * N; };
-        int key0 = n ? tile_at(0) : 0, key_doc = -1;
-        auto fetch = [&](int at) {
-            sk.load(k + (int64_t)at * a.k.ss, a.k.ss, a.sk - at, a.d);
-            sv.load(v + (int64_t)at * a.v.ss, a.v.ss, a.sk - at, a.d);
-            int j = at + threadIdx.x;
+    Stage<T, DP, N, THREADS> sk(a.k.ss, a.d), sv(a.v.ss, a.d);
+    for (int chunk = 0; chunk < tiles; chunk += 64) {
+        Visits visits = visits_of<N>(keys, b, chunk, tiles - chunk, block_docs, wave_docs);
+        int next = 0, key_doc = -1;
+        auto fetch = [&] {
+            next = (chunk + __builtin_ctzll(visits.block)) * N;
+            sk.load(k + (int64_t)next * a.k.ss, a.sk - next);
+            sv.load(v + (int64_t)next * a.v.ss, a.sk - next);
+            int j = next + threadIdx.x;
             if ((int)threadIdx.x < N) key_doc = j < a.sk ? doc_row ? max(doc_row[j], -1) : 0 : -1;
         };
-        if (n) fetch(key0);
-        for (int m = 0; m < n; ++m) {
+        if (visits.block) fetch();
+        while (visits.block) {
             __syncthreads();
             sk.store(tile_k);
             sv.store(tile_v);
             if ((int)threadIdx.x < N) docs[threadIdx.x] = key_doc;
             __syncthreads();
-            const int at = key0;
-            if (m + 1 < n) {
-                key0 = tile_at(m + 1);
-                fetch(key0);
-            }
-            bool mixed = at + N > a.sk || (a.causal && at + N - 1 > wave_first);
-            if (a.causal && at > wave_last) continue;
-            if (doc_row) {
-                int2 r = ranges[(int64_t)b * ranges_n + at / RANGE];
-                if (!meet(r, wave_docs)) continue;
-                mixed |= !one_document(r, wave_docs);
-            }
+            const uint64_t bit = visits.block & -visits.block;
+            const int at = next;
+            visits.block ^= bit;
+            if (visits.block) fetch();
+            if (!(visits.wave & bit) || (a.causal && at > wave_last)) continue;
             f.template step<N / 32>(
                 [&](int t, int n) { return rows_of<T, G::LD>(tile_k, t * 32, n * 16); }, tile_v,
-                docs, at, mixed, a.causal);
+                docs, at, biased, !(visits.whole & bit) || at + N > a.sk,
+                a.causal && at + N - 1 > wave_first);
         }
     }
 
@@ -674,11 +705,15 @@ __global__ __launch_bounds__(64, DP >= 96 ? 1 : 2) void split_kernel(const Args 
 
     Forward<T, DP> f;
     f.begin(a, row<T>(a.q, b, i, h), there, slope_of(a, h));
-    f.scaled = __any(f.scaled);
+    const bool biased = __any(f.slope != 0.f);
     f.pos = i + first;
     const int doc = there ? doc_row ? doc_row[f.pos] : 0 : -1;
     f.doc = doc < 0 ? INT_MIN : doc;
-    const int2 own = range_of_wave(doc);
+    int least = doc < 0 ? NONE : doc, largest = doc;
+    for (int m = 16; m; m >>= 1) {
+        least = min(least, __shfl_xor(least, m));
+        largest = max(largest, __shfl_xor(largest, m));
+    }
     int latest = there ? f.pos : 0, earliest = there ? f.pos : a.sk;
     for (int m = 32; m; m >>= 1) {
         latest = max(latest, __shfl_xor(latest, m));
@@ -689,7 +724,7 @@ __global__ __launch_bounds__(64, DP >= 96 ? 1 : 2) void split_kernel(const Args 
     const T *k = row<T>(a.k, b, 0, g), *v = row<T>(a.v, b, 0, g);
 
     Frag<T> next_k[DP / 16];
-    Stage<T, DP, N, 64> sv;
+    Stage<T, DP, N, 64> sv(a.v.ss, a.d);
     for (int chunk = part * keys_each; chunk < end; chunk += 64 * N) {
         // tiles with a key that some query may see, of 64
         const int tiles = min(64, (end - chunk + N - 1) / N);
@@ -698,7 +733,7 @@ __global__ __launch_bounds__(64, DP >= 96 ? 1 : 2) void split_kernel(const Args 
             visits = 0;
             for (int t = 0; t < tiles; t += 2) {
                 int j = chunk + t * N + lane, d = j < end ? doc_row[j] : -1;
-                uint64_t met = __ballot(d >= (own.x & NONE) && d <= own.y);
+                uint64_t met = __ballot(d >= least && d <= largest);
                 if (met & 0xffffffffull) visits |= 1ull << t;
                 if (met >> 32) visits |= 2ull << t;
             }
@@ -710,7 +745,7 @@ __global__ __launch_bounds__(64, DP >= 96 ? 1 : 2) void split_kernel(const Args 
 #pragma unroll
             for (int n = 0; n < DP / 16; ++n)
                 next_k[n] = row_frag<T>(kr, n * 16 + hf * 8, a.d, row_there);
-            sv.load(v + (int64_t)at * a.v.ss, a.v.ss, a.sk - at, a.d);
+            sv.load(v + (int64_t)at * a.v.ss, a.sk - at);
             int j = at + lane;
             if (lane < N) key_doc = j < a.sk ? doc_row ? max(doc_row[j], -1) : 0 : -1;
         };
@@ -731,9 +766,8 @@ __global__ __launch_bounds__(64, DP >= 96 ? 1 : 2) void split_kernel(const Args 
                 at = chunk + __builtin_ctzll(visits) * N;
                 fetch(at);
             }
-            const bool mixed = doc_row || now + N > a.sk || (a.causal && now + N - 1 > earliest);
-            f.template step<1>([&](int, int n) { return k_now[n]; }, tile_v, docs, now, mixed,
-                               a.causal);
+            f.template step<1>([&](int, int n) { return k_now[n]; }, tile_v, docs, now, biased,
+                               doc_row || now + N > a.sk, a.causal && now + N - 1 > earliest);
         }
     }
 
@@ -828,7 +862,8 @@ void launch_split(const Args& a, const torch::Tensor& like, hipStream_t stream) 
 }
 
 template <typename T, int DP>
-void launch_forward(const Args& a, const int2* ranges, int ranges_n, hipStream_t stream) {
+void launch_forward(const Args& a, const Ranges& keys, const Ranges& queries,
+                    hipStream_t stream) {
     // 128 queries a block share a tile; with few blocks 64 spread wider
     int64_t heads = (int64_t)a.b * a.hq;
     bool wide = heads * ((a.sq + 127) / 128) >= 512;
@@ -837,10 +872,10 @@ void launch_forward(const Args& a, const int2* ranges, int ranges_n, hipStream_t
     TORCH_CHECK(blocks <= INT_MAX, "too many rows for one launch");
     if (wide)
         hipLaunchKernelGGL((forward_kernel<T, DP, 4>), dim3((unsigned)blocks), dim3(256), 0,
-                           stream, a, ranges, ranges_n, tiles_q);
+                           stream, a, keys, queries, tiles_q);
     else
         hipLaunchKernelGGL((forward_kernel<T, DP, 2>), dim3((unsigned)blocks), dim3(128), 0,
-                           stream, a, ranges, ranges_n, tiles_q);
+                           stream, a, keys, queries, tiles_q);
 }
 
 // ---------------------------------------------------------------------------
@@ -903,20 +938,19 @@ __global__ __launch_bounds__(256) void delta_kernel(const Args a, int tiles, flo
 
 template <typename T, int DP, int WAVES>
 __global__ __launch_bounds__(WAVES * 64, DP >= 96 ? 1 : 2)
-void dq_kernel(const Args a, const int2* ranges, int ranges_n, int tiles_q, const float* factors,
-               int factors_n) {
+void dq_kernel(const Args a, const Ranges keys, const Ranges queries, int tiles_q,
+               const float* factors, int factors_n) {
     using G = Tile<T, DP>;
     constexpr int THREADS = WAVES * 64, N = G::KEYS;
     __shared__ alignas(16) T tile_k[N * G::LD], tile_v[N * G::LD];
     __shared__ alignas(16) int docs[N];
-    __shared__ int2 own[WAVES];
-    __shared__ Visits<THREADS> visits;
 
     unsigned id = xcd_order(blockIdx.x, gridDim.x);
     int qt = id % tiles_q, h = id / tiles_q % a.hq, b = id / tiles_q / a.hq;
     if (a.causal) qt = tiles_q - 1 - qt;
-    const int g = h / (a.hq / a.hkv), lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int hf = lane >> 5, first = a.sk - a.sq, row0 = qt * WAVES * 32 + wave * 32;
+    const int g = h / (a.hq / a.hkv), lane = threadIdx.x & 63, hf = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int first = a.sk - a.sq, row0 = (qt * WAVES + wave) * 32;
     const int i = row0 + (lane & 31), pos = i + first;
     const bool there = i < a.sq;
     const int* doc_row = a.documents ? a.documents + b * a.documents_sb : nullptr;
@@ -942,15 +976,11 @@ void dq_kernel(const Args a, const int2* ranges, int ranges_n, int tiles_q, cons
 
     const int seen = there ? doc_row ? doc_row[pos] : 0 : -1;
     const int doc = seen < 0 ? INT_MIN : seen;
-    const int2 wave_docs = range_of_wave(seen);
-    int2 block_docs = wave_docs;
+    int2 wave_docs{}, block_docs{};
     if (doc_row) {
-        if (lane == 0) own[wave] = wave_docs;
-        __syncthreads();
-        for (int w = 0; w < WAVES; ++w) {
-            block_docs.x = min(block_docs.x & NONE, own[w].x & NONE);
-            block_docs.y = max(block_docs.y, own[w].y);
-        }
+        wave_docs = queries.of(b, qt * WAVES + wave);
+        block_docs = queries.of(b, qt * WAVES);
+        for (int w = 1; w < WAVES; ++w) block_docs = both(block_docs, queries.of(b, qt * WAVES + w));
     }
     const int wave_first = row0 + first, wave_last = min(row0 + 31, a.sq - 1) + first;
     int end = a.sk;
@@ -958,37 +988,31 @@ void dq_kernel(const Args a, const int2* ranges, int ranges_n, int tiles_q, cons
     const int tiles = (end + N - 1) / N;
     const T *k = row<T>(a.k, b, 0, g), *v = row<T>(a.v, b, 0, g);
 
-    Stage<T, DP, N, THREADS> sk, sv;
-    for (int chunk = 0; chunk < tiles; chunk += THREADS) {
-        int n = min(THREADS, tiles - chunk);
-        if (doc_row) n = visits.fill(chunk, tiles, N, ranges + (int64_t)b * ranges_n, block_docs);
-        auto tile_at = [&](int m) { return (doc_row ? visits.list[m] : chunk + m) * N; };
-        int key0 = n ? tile_at(0) : 0, key_doc = -1;
-        auto fetch = [&](int at) {
-            sk.load(k + (int64_t)at * a.k.ss, a.k.ss, a.sk - at, a.d);
-            sv.load(v + (int64_t)at * a.v.ss, a.v.ss, a.sk - at, a.d);
-            int j = at + threadIdx.x;
+    Stage<T, DP, N, THREADS> sk(a.k.ss, a.d), sv(a.v.ss, a.d);
+    for (int chunk = 0; chunk < tiles; chunk += 64) {
+        Visits visits = visits_of<N>(keys, b, chunk, tiles - chunk, block_docs, wave_docs);
+        int next = 0, key_doc = -1;
+        auto fetch = [&] {
+            next = (chunk + __builtin_ctzll(visits.block)) * N;
+            sk.load(k + (int64_t)next * a.k.ss, a.sk - next);
+            sv.load(v + (int64_t)next * a.v.ss, a.sk - next);
+            int j = next + threadIdx.x;
             if ((int)threadIdx.x < N) key_doc = j < a.sk ? doc_row ? max(doc_row[j], -1) : 0 : -1;
         };
-        if (n) fetch(key0);
-        for (int m = 0; m < n; ++m) {
+        if (visits.block) fetch();
+        while (visits.block) {
             __syncthreads();
             sk.store(tile_k);
             sv.store(tile_v);
             if ((int)threadIdx.x < N) docs[threadIdx.x] = key_doc;
             __syncthreads();
-            const int at = key0;
-            if (m + 1 < n) {
-                key0 = tile_at(m + 1);
-                fetch(key0);
-            }
-            bool mixed = at + N > a.sk || (a.causal && at + N - 1 > wave_first);
-            if (a.causal && at > wave_last) continue;
-            if (doc_row) {
-                int2 r = ranges[(int64_t)b * ranges_n + at / RANGE];
-                if (!meet(r, wave_docs)) continue;
-                mixed |= !one_document(r, wave_docs);
-            }
+            const uint64_t bit = visits.block & -visits.block;
+            const int at = next;
+            visits.block ^= bit;
+            if (visits.block) fetch();
+            if (!(visits.wave & bit) || (a.causal && at > wave_last)) continue;
+            const bool by_document = !(visits.whole & bit) || at + N > a.sk;
+            const bool by_position = a.causal && at + N - 1 > wave_first;
 #pragma unroll
             for (int t = 0; t < N / 32; ++t) {
                 acc16 s = {}, dp = {};
@@ -999,27 +1023,17 @@ void dq_kernel(const Args a, const int2* ranges, int ranges_n, int tiles_q, cons
                 for (int n = 0; n < DP / 16; ++n)
                     dp = mma(rows_of<T, G::LD>(tile_v, t * 32, n * 16), dout[n], dp);
                 if (slope != 0.f) {
-                    float far = (float)(pos - at - t * 32 - 4 * hf);
+                    const float far = (float)(pos - at - t * 32 - 4 * hf);
 #pragma unroll
                     for (int e = 0; e < 16; ++e)
-                        s[e] = fmaf(s[e], c, -off - slope * fabsf(far - (float)(8 * (e >> 2) + (e & 3))));
+                        s[e] = fmaf(s[e], c,
+                                    fmaf(-slope, fabsf(far - (float)(8 * (e >> 2) + (e & 3))), -off));
                 } else {
 #pragma unroll
                     for (int e = 0; e < 16; ++e) s[e] = fmaf(s[e], c, -off);
                 }
-                if (mixed) {
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        int j = t * 32 + r * 8 + 4 * hf;
-                        int4 d = *(const int4*)(docs + j);
-                        const int kd[4] = {d.x, d.y, d.z, d.w};
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            bool hidden = kd[e] != doc || (a.causal && at + j + e > pos);
-                            s[r * 4 + e] = hidden ? -INFINITY : s[r * 4 + e];
-                        }
-                    }
-                }
+                if (by_document) hide_documents(s, docs, t, doc);
+                if (by_position) hide_past(s, t, pos - at);
                 float sum = 0;
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
@@ -1073,20 +1087,19 @@ void dq_kernel(const Args a, const int2* ranges, int ranges_n, int tiles_q, cons
 
 template <typename T, int DP, int WAVES>
 __global__ __launch_bounds__(WAVES * 64, DP >= 96 || (DP == 64 && sizeof(T) == 4) ? 1 : 2)
-void dkv_kernel(const Args a, const int2* ranges, int ranges_n, int tiles_k, const float* factors,
-                int factors_n) {
+void dkv_kernel(const Args a, const Ranges keys, const Ranges queries, int tiles_k,
+                const float* factors, int factors_n) {
     using G = Tile<T, DP>;
     constexpr int THREADS = WAVES * 64, N = G::KEYS;  // N queries a tile
     __shared__ alignas(16) T tile_q[N * G::LD], tile_o[N * G::LD];
     __shared__ alignas(16) int docs[N];
     __shared__ alignas(16) float lses[N], deltas[N];
-    __shared__ int2 own[WAVES];
-    __shared__ Visits<THREADS> visits;
 
     unsigned id = xcd_order(blockIdx.x, gridDim.x);
     const int kt = id % tiles_k, g = id / tiles_k % a.hkv, b = id / tiles_k / a.hkv;
-    const int group = a.hq / a.hkv, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int hf = lane >> 5, first = a.sk - a.sq, block0 = kt * WAVES * 32;
+    const int group = a.hq / a.hkv, lane = threadIdx.x & 63, hf = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int first = a.sk - a.sq, block0 = kt * WAVES * 32;
     const int key0 = block0 + wave * 32, j = key0 + (lane & 31);
     const bool there = j < a.sk;
     const int* doc_row = a.documents ? a.documents + b * a.documents_sb : nullptr;
@@ -1107,32 +1120,27 @@ void dkv_kernel(const Args a, const int2* ranges, int ranges_n, int tiles_k, con
 
     const int seen = there ? doc_row ? doc_row[j] : 0 : -1;
     const int doc = seen < 0 ? INT_MIN : seen;
-    const int2 wave_docs = range_of_wave(seen);
-    int2 block_docs = wave_docs;
+    int2 wave_docs{}, block_docs{};
     if (doc_row) {
-        if (lane == 0) own[wave] = wave_docs;
-        __syncthreads();
-        for (int w = 0; w < WAVES; ++w) {
-            block_docs.x = min(block_docs.x & NONE, own[w].x & NONE);
-            block_docs.y = max(block_docs.y, own[w].y);
-        }
+        wave_docs = keys.of(b, kt * WAVES + wave);
+        block_docs = keys.of(b, kt * WAVES);
+        for (int w = 1; w < WAVES; ++w) block_docs = both(block_docs, keys.of(b, kt * WAVES + w));
     }
     const int wave_last = min(key0 + 31, a.sk - 1);
     const int tiles = (a.sq + N - 1) / N;
     const int begin = a.causal ? max(0, block0 - first) / N : 0;
 
-    Stage<T, DP, N, THREADS> sq, so;
-    for (int chunk = begin; chunk < tiles; chunk += THREADS) {
-        int n = min(THREADS, tiles - chunk);
-        if (doc_row) n = visits.fill(chunk, tiles, N, ranges + (int64_t)b * ranges_n, block_docs);
-        auto tile_at = [&](int m) { return (doc_row ? visits.list[m] : chunk + m) * N; };
+    Stage<T, DP, N, THREADS> sq(a.q.ss, a.d), so(a.dout.ss, a.d);
+    for (int chunk = begin; chunk < tiles; chunk += 64) {
+        const Visits visits = visits_of<N>(queries, b, chunk, tiles - chunk, block_docs, wave_docs);
+        if (!visits.block) continue;
+        uint64_t left = visits.block;
         int next = 0, next_h = g * group, query_doc = -1;
         float lse = 0, delta = 0, next_factor = 1.f;
-        auto fetch = [&](int m) {
-            next_h = g * group + m / n;
-            next = tile_at(m % n);
-            sq.load(row<T>(a.q, b, next, next_h), a.q.ss, a.sq - next, a.d);
-            so.load(row<T>(a.dout, b, next, next_h), a.dout.ss, a.sq - next, a.d);
+        auto fetch = [&] {
+            next = (chunk + __builtin_ctzll(left)) * N;
+            sq.load(row<T>(a.q, b, next, next_h), a.sq - next);
+            so.load(row<T>(a.dout, b, next, next_h), a.sq - next);
             if ((int)threadIdx.x < N) {
                 int i = next + threadIdx.x;
                 int64_t at = ((int64_t)b * a.hq + next_h) * a.sq + i;
@@ -1143,8 +1151,8 @@ void dkv_kernel(const Args a, const int2* ranges, int ranges_n, int tiles_k, con
             if constexpr (FACTORED<T>)
                 next_factor = factors[((int64_t)b * a.hq + next_h) * factors_n + next / FACTOR_ROWS];
         };
-        if (n) fetch(0);
-        for (int m = 0; m < n * group; ++m) {
+        fetch();
+        while (left) {
             __syncthreads();
             sq.store(tile_q);
             so.store(tile_o);
@@ -1154,16 +1162,18 @@ void dkv_kernel(const Args a, const int2* ranges, int ranges_n, int tiles_k, con
                 deltas[threadIdx.x] = delta;
             }
             __syncthreads();
+            const uint64_t bit = left & -left;
             const int at = next, h = next_h;
             const float tile_factor = next_factor;
-            if (m + 1 < n * group) fetch(m + 1);
-            bool mixed = a.causal && at + first < wave_last;
-            if (a.causal && at + first + N - 1 < key0) continue;
-            if (doc_row) {
-                int2 r = ranges[(int64_t)b * ranges_n + at / RANGE];
-                if (!meet(r, wave_docs)) continue;
-                mixed |= !one_document(r, wave_docs);
+            left ^= bit;
+            if (!left && next_h + 1 < (g + 1) * group) {  // the next head of the group
+                left = visits.block;
+                ++next_h;
             }
+            if (left) fetch();
+            if (!(visits.wave & bit) || (a.causal && at + first + N - 1 < key0)) continue;
+            const bool by_document = !(visits.whole & bit);
+            const bool by_position = a.causal && at + first < wave_last;
             if constexpr (FACTORED<T>) {
                 // larger gradients than before: dk's sums go to their factor
                 if (!begun || tile_factor < factor) {
@@ -1176,7 +1186,7 @@ void dkv_kernel(const Args a, const int2* ranges, int ranges_n, int tiles_k, con
                     begun = true;
                 }
             }
-            const float slope = slope_of(a, h);
+            const float slope = slope_of(a, h), far = (float)(at + first + 4 * hf - j);
 #pragma unroll
             for (int t = 0; t < N / 32; ++t) {
                 acc16 s = {}, dp = {};
@@ -1195,23 +1205,16 @@ void dkv_kernel(const Args a, const int2* ranges, int ranges_n, int tiles_k, con
                         float off = l[e];
                         if constexpr (FACTORED<T>) off -= SHIFT;
                         if (slope != 0.f)
-                            off = fmaf(slope, fabsf((float)(at + first + i + e - j)), off);
+                            off = fmaf(slope, fabsf(far + (float)(t * 32 + r * 8 + e)), off);
                         s[r * 4 + e] = fmaf(s[r * 4 + e], c, -off);
                         if constexpr (FACTORED<T>)
                             dp[r * 4 + e] = fmaf(dp[r * 4 + e], factor, -dl[e] * factor);
                         else
                             dp[r * 4 + e] -= dl[e];
                     }
-                    if (mixed) {
-                        int4 d = *(const int4*)(docs + i);
-                        const int qd[4] = {d.x, d.y, d.z, d.w};
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            bool hidden = qd[e] != doc || (a.causal && j > at + first + i + e);
-                            s[r * 4 + e] = hidden ? -INFINITY : s[r * 4 + e];
-                        }
-                    }
                 }
+                if (by_document) hide_documents(s, docs, t, doc);
+                if (by_position) hide_before(s, t, j - at - first);
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
                     s[e] = exp2_fast(s[e]);
@@ -1253,8 +1256,8 @@ void dkv_kernel(const Args a, const int2* ranges, int ranges_n, int tiles_k, con
 }
 
 template <typename T, int DP>
-void launch_backward(const Args& a, const int2* key_ranges, int key_n, const int2* query_ranges,
-                     int query_n, float* factors, int factors_n, hipStream_t stream) {
+void launch_backward(const Args& a, const Ranges& keys, const Ranges& queries, float* factors,
+                     int factors_n, hipStream_t stream) {
     int64_t rows = (int64_t)a.b * a.hq * factors_n;
     int tiles_q = (a.sq + 127) / 128, tiles_k = (a.sk + 127) / 128;
     int64_t blocks_q = (int64_t)a.b * a.hq * tiles_q, blocks_k = (int64_t)a.b * a.hkv * tiles_k;
@@ -1262,9 +1265,9 @@ void launch_backward(const Args& a, const int2* key_ranges, int key_n, const int
     hipLaunchKernelGGL(delta_kernel<T>, dim3((unsigned)rows), dim3(256), 0, stream, a, factors_n,
                        factors);
     hipLaunchKernelGGL((dq_kernel<T, DP, 4>), dim3((unsigned)blocks_q), dim3(256), 0, stream, a,
-                       key_ranges, key_n, tiles_q, factors, factors_n);
+                       keys, queries, tiles_q, factors, factors_n);
     hipLaunchKernelGGL((dkv_kernel<T, DP, 4>), dim3((unsigned)blocks_k), dim3(256), 0, stream, a,
-                       query_ranges, query_n, tiles_k, factors, factors_n);
+                       keys, queries, tiles_k, factors, factors_n);
 }
 
 // f of the head size, as the constant of its padded width
@@ -1278,16 +1281,30 @@ void for_width(int d, F f) {
     }
 }
 
-// [batch, count] ranges of the positions from `first` on, for a launch
-torch::Tensor ranges_for(const Args& a, int first, const torch::Tensor& like, hipStream_t stream) {
-    int count = (a.sk - first + RANGE - 1) / RANGE;
-    auto r = torch::empty({a.b, count, 2}, like.options().dtype(torch::kInt32));
-    if (a.b * (int64_t)count)
-        hipLaunchKernelGGL(ranges_kernel, dim3((unsigned)(a.b * count)), dim3(64), 0, stream,
-                           a.documents, a.documents_sb, first, a.sk, count,
-                           (int2*)r.data_ptr<int>());
-    return r;
-}
+// The ranges of the keys' documents and of the queries', which are the same
+// where both begin at a multiple of RANGE.
+struct DocumentRanges {
+    torch::Tensor buffer[2];
+    Ranges keys{}, queries{};
+
+    DocumentRanges(const Args& a, const torch::Tensor& like, hipStream_t stream) {
+        if (!a.documents) return;
+        keys = fill(0, a, 0, like, stream);
+        const int first = a.sk - a.sq;
+        if (first) queries = fill(1, a, first, like, stream);
+        else queries = keys;
+    }
+    Ranges fill(int n, const Args& a, int first, const torch::Tensor& like, hipStream_t stream) {
+        const int count = (a.sk - first + RANGE - 1) / RANGE;
+        const int64_t all = (int64_t)a.b * count;
+        buffer[n] = torch::empty({all, 2}, like.options().dtype(torch::kInt32));
+        int2* at = (int2*)buffer[n].data_ptr<int>();
+        constexpr int EACH = 256 / RANGE;
+        hipLaunchKernelGGL(ranges_kernel, dim3((unsigned)((all + EACH - 1) / EACH)), dim3(256), 0,
+                           stream, a.documents, a.documents_sb, first, a.sk, count, all, at);
+        return {at, count};
+    }
+};
 
 // ---------------------------------------------------------------------------
 
@@ -1295,10 +1312,12 @@ View view(const torch::Tensor& t) {
     return {t.data_ptr(), t.stride(0), t.stride(1), t.stride(2)};
 }
 
-// d contiguous and every head at a 16-byte address, by a copy where it is not
+// d contiguous, every head at a 16-byte address and a tile of 64 rows within
+// the 31 bits of a buffer load's offset, by a copy where it is not
 torch::Tensor aligned(const torch::Tensor& t) {
     int64_t per = 16 / t.element_size();
-    bool fine = (uintptr_t)t.data_ptr() % 16 == 0 && t.stride(3) == 1;
+    bool fine = (uintptr_t)t.data_ptr() % 16 == 0 && t.stride(3) == 1 &&
+                t.stride(1) * t.element_size() < (1 << 24);
     for (int d = 0; d < 3; ++d) fine = fine && t.stride(d) % per == 0;
     return fine ? t : t.clone(at::MemoryFormat::Contiguous);
 }
@@ -1371,18 +1390,16 @@ std::vector<torch::Tensor> attention_forward(torch::Tensor q, torch::Tensor k, t
     a.lse = want_lse ? lse.data_ptr<float>() : nullptr;
     hipStream_t stream = at::hip::getCurrentHIPStream();
     if (out.numel() == 0) return {out, lse};
-    const bool split = split_keys(a);
-    torch::Tensor ranges;
-    if (documents && !split) ranges = ranges_for(a, 0, q, stream);
     for_type(q.scalar_type(), [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
         for_width(a.d, [&](auto width) {
-            if (split)
-                launch_split<T, decltype(width)::value>(a, q, stream);
-            else
-                launch_forward<T, decltype(width)::value>(
-                    a, documents ? (const int2*)ranges.data_ptr<int>() : nullptr,
-                    documents ? (int)ranges.size(1) : 0, stream);
+            constexpr int DP = decltype(width)::value;
+            if (split_keys(a)) {
+                launch_split<T, DP>(a, q, stream);
+            } else {
+                DocumentRanges ranges(a, q, stream);
+                launch_forward<T, DP>(a, ranges.keys, ranges.queries, stream);
+            }
         });
     });
     return {out, lse};
@@ -1417,21 +1434,13 @@ std::vector<torch::Tensor> attention_backward(torch::Tensor dout, torch::Tensor 
     if (dq.numel() == 0) return {dq, dk.zero_(), dv.zero_()};
     const int factors_n = (a.sq + FACTOR_ROWS - 1) / FACTOR_ROWS;
     auto factors = torch::empty({a.b, a.hq, factors_n}, lse.options());
-    torch::Tensor keys, queries;  // ranges of documents
-    const int2 *key_ranges = nullptr, *query_ranges = nullptr;
-    if (documents) {
-        keys = ranges_for(a, 0, q, stream);
-        queries = a.sq == a.sk ? keys : ranges_for(a, a.sk - a.sq, q, stream);
-        key_ranges = (const int2*)keys.data_ptr<int>();
-        query_ranges = (const int2*)queries.data_ptr<int>();
-    }
+    DocumentRanges ranges(a, q, stream);
     for_type(q.scalar_type(), [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
         for_width(a.d, [&](auto width) {
-            launch_backward<T, decltype(width)::value>(
-                a, key_ranges, documents ? (int)keys.size(1) : 0, query_ranges,
-                documents ? (int)queries.size(1) : 0, factors.data_ptr<float>(), factors_n,
-                stream);
+            launch_backward<T, decltype(width)::value>(a, ranges.keys, ranges.queries,
+                                                       factors.data_ptr<float>(), factors_n,
+                                                       stream);
         });
     });
     return {dq, dk, dv};
