@@ -256,7 +256,6 @@ template <typename T, int DP> struct Tile {
     static constexpr int PER = 16 / sizeof(T);
     static constexpr int LD = DP + PER;  // rows 16 bytes apart of a multiple of the banks
     static constexpr int VECS = DP / PER;
-    static constexpr int KEYS = sizeof(T) == 2 ? 64 : 32;
 };
 
 // Rows of one tile on their way from memory to shared memory, through
@@ -270,13 +269,13 @@ template <typename T, int DP, int ROWS, int THREADS> struct Stage {
     typedef unsigned raw4 __attribute__((ext_vector_type(4)));
     raw4 r[N];
     int offset[N];   // of this thread's vectors, in bytes; the end for those behind d
-    int row_bytes, d_bytes;
+    int row_bytes, d_bytes, tid;
 
-    __device__ __forceinline__ Stage(int64_t stride, int d)
-        : row_bytes((int)stride * (int)sizeof(T)), d_bytes(d * (int)sizeof(T)) {
+    __device__ __forceinline__ Stage(int64_t stride, int d, int tid)
+        : row_bytes((int)stride * (int)sizeof(T)), d_bytes(d * (int)sizeof(T)), tid(tid) {
 #pragma unroll
         for (int n = 0; n < N; ++n) {
-            int v = threadIdx.x + n * THREADS, y = v / G::VECS, x = (v % G::VECS) * G::PER;
+            int v = tid + n * THREADS, y = v / G::VECS, x = (v % G::VECS) * G::PER;
             offset[n] = x < d ? y * row_bytes + x * (int)sizeof(T) : 0x7fffffff - 15;
         }
     }
@@ -290,7 +289,7 @@ template <typename T, int DP, int ROWS, int THREADS> struct Stage {
     __device__ __forceinline__ void store(T* tile) const {
 #pragma unroll
         for (int n = 0; n < N; ++n) {
-            int v = threadIdx.x + n * THREADS, y = v / G::VECS, x = (v % G::VECS) * G::PER;
+            int v = tid + n * THREADS, y = v / G::VECS, x = (v % G::VECS) * G::PER;
             *(raw4*)(tile + y * G::LD + x) = r[n];
         }
     }
@@ -429,6 +428,48 @@ __device__ __forceinline__ Visits visits_of(const Ranges& r, int b, int first, i
     for (int m = 1; m < SIZE / RANGE; ++m) x = both(x, r.of(b, t * (SIZE / RANGE) + m));
     return {__ballot(meet(x, block)) & all, __ballot(meet(x, wave)) & all,
             __ballot(one_document(x, wave)) & all};
+}
+
+// A block of ROWS * SHARES waves: ROWS waves of 32 rows each share their tiles,
+// and SHARES such groups take the block's tiles in turn, with a tile each at a
+// time, and add their sums up at the end.  Shares put more waves on few rows.
+__device__ __forceinline__ uint64_t bit_of(uint64_t bits, int n) {
+    for (; n; --n) bits &= bits - 1;
+    return bits & -bits;
+}
+template <int N> __device__ __forceinline__ uint64_t without(uint64_t bits) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) bits &= bits - 1;
+    return bits;
+}
+
+// With 4 shares a wave fetches its tile alone: 32 rows keep it in registers.
+template <typename T, int SHARES>
+constexpr int tile_rows = SHARES == 4 || sizeof(T) == 4 ? 32 : 64;
+
+// the shares' tiles and, at the end, the sums they leave for the first
+template <typename T, int DP, int N, int SHARES, int FLOATS> union Shared {
+    alignas(16) T tiles[SHARES][2][N * Tile<T, DP>::LD];
+    alignas(16) float boxes[FLOATS ? FLOATS : 4];
+};
+
+// a wave's sums for another: [32 DP / 64] floats a lane, lanes next to each other
+template <int DP>
+__device__ __forceinline__ void leave(float* box, const acc16* x) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int n = 0; n < DP / 32; ++n)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) box[(n * 16 + i) * 64 + lane] = x[n][i];
+}
+template <int DP>
+__device__ __forceinline__ void take(const float* box, float mine, float theirs, acc16* x) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int n = 0; n < DP / 32; ++n)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            x[n][i] = fmaf(box[(n * 16 + i) * 64 + lane], theirs, x[n][i] * mine);
 }
 
 // Workgroups go round the 8 XCDs: neighbours in the order returned run on one
@@ -588,20 +629,25 @@ __device__ __forceinline__ void put4(T* at, float a, float b, float c, float d) 
 // 32 queries for each wave, all heads and keys.  The block's waves share the
 // tiles of K and V; block tiles of one head are neighbours on one XCD, whose
 // L2 then serves the head's keys once.
-template <typename T, int DP, int WAVES>
-__global__ __launch_bounds__(WAVES * 64, DP == 128 && (WAVES == 2 || sizeof(T) == 4) ? 1 : 2)
+template <typename T, int DP, int ROWS, int SHARES>
+__global__ __launch_bounds__(ROWS * SHARES * 64, (DP == 128 && (ROWS < 4 || sizeof(T) == 4)) || SHARES == 4 ? 1 : 2)
 void forward_kernel(const Args a, const Ranges keys, const Ranges queries, int tiles_q) {
     using G = Tile<T, DP>;
-    constexpr int THREADS = WAVES * 64, N = G::KEYS;
-    __shared__ alignas(16) T tile_k[N * G::LD], tile_v[N * G::LD];
-    __shared__ alignas(16) int docs[N];
+    constexpr int BOX = (DP / 2 + 2) * 64;  // o, off and total
+    constexpr int THREADS = ROWS * 64, N = tile_rows<T, SHARES>;
+    __shared__ Shared<T, DP, N, SHARES, (SHARES - 1) * ROWS * BOX> shared;
+    __shared__ alignas(16) int tile_docs[SHARES][N];
 
     unsigned id = xcd_order(blockIdx.x, gridDim.x);
     int qt = id % tiles_q, h = id / tiles_q % a.hq, b = id / tiles_q / a.hq;
     if (a.causal) qt = tiles_q - 1 - qt;  // the longest first
     const int g = h / (a.hq / a.hkv), lane = threadIdx.x & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int first = a.sk - a.sq, row0 = (qt * WAVES + wave) * 32;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % ROWS;
+    const int share = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) / ROWS;
+    const int tid = threadIdx.x - share * THREADS;
+    T *tile_k = shared.tiles[share][0], *tile_v = shared.tiles[share][1];
+    int* docs = tile_docs[share];
+    const int first = a.sk - a.sq, row0 = (qt * ROWS + wave) * 32;
     const int i = row0 + (lane & 31);
     const bool there = i < a.sq;
     const int* doc_row = a.documents ? a.documents + b * a.documents_sb : nullptr;
@@ -613,38 +659,41 @@ void forward_kernel(const Args a, const Ranges keys, const Ranges queries, int t
     f.doc = doc < 0 ? INT_MIN : doc;
     int2 wave_docs{}, block_docs{};
     if (doc_row) {
-        wave_docs = queries.of(b, qt * WAVES + wave);
-        block_docs = queries.of(b, qt * WAVES);
-        for (int w = 1; w < WAVES; ++w) block_docs = both(block_docs, queries.of(b, qt * WAVES + w));
+        wave_docs = queries.of(b, qt * ROWS + wave);
+        block_docs = queries.of(b, qt * ROWS);
+        for (int w = 1; w < ROWS; ++w) block_docs = both(block_docs, queries.of(b, qt * ROWS + w));
     }
     const int wave_first = row0 + first, wave_last = min(row0 + 31, a.sq - 1) + first;
     int end = a.sk;
-    if (a.causal) end = min(end, (qt + 1) * WAVES * 32 + first);
+    if (a.causal) end = min(end, (qt + 1) * ROWS * 32 + first);
     const int tiles = (end + N - 1) / N;
     const bool biased = f.slope != 0.f;
     const T *k = row<T>(a.k, b, 0, g), *v = row<T>(a.v, b, 0, g);
 
-    Stage<T, DP, N, THREADS> sk(a.k.ss, a.d), sv(a.v.ss, a.d);
+    Stage<T, DP, N, THREADS> sk(a.k.ss, a.d, tid), sv(a.v.ss, a.d, tid);
     for (int chunk = 0; chunk < tiles; chunk += 64) {
         Visits visits = visits_of<N>(keys, b, chunk, tiles - chunk, block_docs, wave_docs);
+        uint64_t mine = 0;
         int next = 0, key_doc = -1;
         auto fetch = [&] {
-            next = (chunk + __builtin_ctzll(visits.block)) * N;
+            mine = bit_of(visits.block, share);
+            if (!mine) return;
+            next = (chunk + __builtin_ctzll(mine)) * N;
             sk.load(k + (int64_t)next * a.k.ss, a.sk - next);
             sv.load(v + (int64_t)next * a.v.ss, a.sk - next);
-            int j = next + threadIdx.x;
-            if ((int)threadIdx.x < N) key_doc = j < a.sk ? doc_row ? max(doc_row[j], -1) : 0 : -1;
+            int j = next + tid;
+            if (tid < N) key_doc = j < a.sk ? doc_row ? max(doc_row[j], -1) : 0 : -1;
         };
         if (visits.block) fetch();
         while (visits.block) {
             __syncthreads();
             sk.store(tile_k);
             sv.store(tile_v);
-            if ((int)threadIdx.x < N) docs[threadIdx.x] = key_doc;
+            if (tid < N) docs[tid] = key_doc;
             __syncthreads();
-            const uint64_t bit = visits.block & -visits.block;
+            const uint64_t bit = mine;
             const int at = next;
-            visits.block ^= bit;
+            visits.block = without<SHARES>(visits.block);
             if (visits.block) fetch();
             if (!(visits.wave & bit) || (a.causal && at > wave_last)) continue;
             f.template step<N / 32>(
@@ -654,7 +703,28 @@ void forward_kernel(const Args a, const Ranges keys, const Ranges queries, int t
         }
     }
 
-    const float total = add_halves(f.total);
+    float total = add_halves(f.total);
+    if constexpr (SHARES > 1) {
+        float* box = shared.boxes + wave * BOX;
+        __syncthreads();
+        if (share) {
+            float* to = box + (share - 1) * ROWS * BOX;
+            leave<DP>(to, f.o);
+            to[DP / 2 * 64 + lane] = f.off;
+            to[(DP / 2 + 1) * 64 + lane] = total;
+        }
+        __syncthreads();
+        if (share) return;
+        for (int n = 0; n < SHARES - 1; ++n, box += ROWS * BOX) {
+            const float off = box[DP / 2 * 64 + lane], sum = box[(DP / 2 + 1) * 64 + lane];
+            const float top = total == 0.f ? off : sum == 0.f ? f.off : fmaxf(f.off, off);
+            const float keep = total == 0.f ? 0.f : exp2_fast(f.off - top);
+            const float add = sum == 0.f ? 0.f : exp2_fast(off - top);
+            take<DP>(box, keep, add, f.o);
+            total = total * keep + sum * add;
+            f.off = top;
+        }
+    }
     const float inv = total == 0.f ? 0.f : 1.f / total;
     if (there) {
         T* out = row<T>(a.out, b, i, h);
@@ -724,7 +794,7 @@ __global__ __launch_bounds__(64, DP >= 96 ? 1 : 2) void split_kernel(const Args 
     const T *k = row<T>(a.k, b, 0, g), *v = row<T>(a.v, b, 0, g);
 
     Frag<T> next_k[DP / 16];
-    Stage<T, DP, N, 64> sv(a.v.ss, a.d);
+    Stage<T, DP, N, 64> sv(a.v.ss, a.d, lane);
     for (int chunk = part * keys_each; chunk < end; chunk += 64 * N) {
         // tiles with a key that some query may see, of 64
         const int tiles = min(64, (end - chunk + N - 1) / N);
@@ -838,6 +908,25 @@ __global__ __launch_bounds__(256) void join_kernel(const Args a, int parts, cons
 
 int padded(int d) { return (d + 31) / 32 * 32; }
 
+// The shape of the blocks for `length` rows of each of `heads`: 4 waves of 32
+// rows that share their tiles where that gives two blocks a CU; else 2 of them
+// and 2 shares, or 1 and 4.
+template <typename F>
+void for_shape(int64_t heads, int length, F f) {
+    auto blocks = [&](int rows) { return heads * ((length + rows - 1) / rows); };
+    TORCH_CHECK(blocks(32) <= INT_MAX, "too many rows for one launch");
+    auto go = [&](auto rows, auto shares) {
+        const int each = 32 * decltype(rows)::value;
+        f(rows, shares, (length + each - 1) / each, (unsigned)blocks(each));
+    };
+    if (blocks(128) >= 512)
+        go(std::integral_constant<int, 4>{}, std::integral_constant<int, 1>{});
+    else if (blocks(64) >= 256)
+        go(std::integral_constant<int, 2>{}, std::integral_constant<int, 2>{});
+    else
+        go(std::integral_constant<int, 1>{}, std::integral_constant<int, 4>{});
+}
+
 // Whether the forward pass is split over the keys: where 64 queries a block
 // give fewer blocks than there are CUs.
 bool split_keys(const Args& a) { return (int64_t)a.b * a.hq * ((a.sq + 63) / 64) < 256; }
@@ -864,18 +953,11 @@ void launch_split(const Args& a, const torch::Tensor& like, hipStream_t stream) 
 template <typename T, int DP>
 void launch_forward(const Args& a, const Ranges& keys, const Ranges& queries,
                     hipStream_t stream) {
-    // 128 queries a block share a tile; with few blocks 64 spread wider
-    int64_t heads = (int64_t)a.b * a.hq;
-    bool wide = heads * ((a.sq + 127) / 128) >= 512;
-    int rows = wide ? 128 : 64, tiles_q = (a.sq + rows - 1) / rows;
-    int64_t blocks = heads * tiles_q;
-    TORCH_CHECK(blocks <= INT_MAX, "too many rows for one launch");
-    if (wide)
-        hipLaunchKernelGGL((forward_kernel<T, DP, 4>), dim3((unsigned)blocks), dim3(256), 0,
-                           stream, a, keys, queries, tiles_q);
-    else
-        hipLaunchKernelGGL((forward_kernel<T, DP, 2>), dim3((unsigned)blocks), dim3(128), 0,
-                           stream, a, keys, queries, tiles_q);
+    for_shape((int64_t)a.b * a.hq, a.sq, [&](auto rows, auto shares, int tiles, unsigned blocks) {
+        constexpr int ROWS = decltype(rows)::value, SHARES = decltype(shares)::value;
+        hipLaunchKernelGGL((forward_kernel<T, DP, ROWS, SHARES>), dim3(blocks),
+                           dim3(ROWS * SHARES * 64), 0, stream, a, keys, queries, tiles);
+    });
 }
 
 // ---------------------------------------------------------------------------
@@ -936,21 +1018,26 @@ __global__ __launch_bounds__(256) void delta_kernel(const Args a, int tiles, flo
     }
 }
 
-template <typename T, int DP, int WAVES>
-__global__ __launch_bounds__(WAVES * 64, DP >= 96 ? 1 : 2)
+template <typename T, int DP, int ROWS, int SHARES>
+__global__ __launch_bounds__(ROWS * SHARES * 64, DP >= 96 || SHARES == 4 ? 1 : 2)
 void dq_kernel(const Args a, const Ranges keys, const Ranges queries, int tiles_q,
                const float* factors, int factors_n) {
     using G = Tile<T, DP>;
-    constexpr int THREADS = WAVES * 64, N = G::KEYS;
-    __shared__ alignas(16) T tile_k[N * G::LD], tile_v[N * G::LD];
-    __shared__ alignas(16) int docs[N];
+    constexpr int BOX = (CORRECTED<T> ? DP + 1 : DP / 2) * 64;  // acc, mean and rest
+    constexpr int THREADS = ROWS * 64, N = tile_rows<T, SHARES>;
+    __shared__ Shared<T, DP, N, SHARES, (SHARES - 1) * ROWS * BOX> shared;
+    __shared__ alignas(16) int tile_docs[SHARES][N];
 
     unsigned id = xcd_order(blockIdx.x, gridDim.x);
     int qt = id % tiles_q, h = id / tiles_q % a.hq, b = id / tiles_q / a.hq;
     if (a.causal) qt = tiles_q - 1 - qt;
     const int g = h / (a.hq / a.hkv), lane = threadIdx.x & 63, hf = lane >> 5;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int first = a.sk - a.sq, row0 = (qt * WAVES + wave) * 32;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % ROWS;
+    const int share = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) / ROWS;
+    const int tid = threadIdx.x - share * THREADS;
+    T *tile_k = shared.tiles[share][0], *tile_v = shared.tiles[share][1];
+    int* docs = tile_docs[share];
+    const int first = a.sk - a.sq, row0 = (qt * ROWS + wave) * 32;
     const int i = row0 + (lane & 31), pos = i + first;
     const bool there = i < a.sq;
     const int* doc_row = a.documents ? a.documents + b * a.documents_sb : nullptr;
@@ -978,37 +1065,40 @@ void dq_kernel(const Args a, const Ranges keys, const Ranges queries, int tiles_
     const int doc = seen < 0 ? INT_MIN : seen;
     int2 wave_docs{}, block_docs{};
     if (doc_row) {
-        wave_docs = queries.of(b, qt * WAVES + wave);
-        block_docs = queries.of(b, qt * WAVES);
-        for (int w = 1; w < WAVES; ++w) block_docs = both(block_docs, queries.of(b, qt * WAVES + w));
+        wave_docs = queries.of(b, qt * ROWS + wave);
+        block_docs = queries.of(b, qt * ROWS);
+        for (int w = 1; w < ROWS; ++w) block_docs = both(block_docs, queries.of(b, qt * ROWS + w));
     }
     const int wave_first = row0 + first, wave_last = min(row0 + 31, a.sq - 1) + first;
     int end = a.sk;
-    if (a.causal) end = min(end, (qt + 1) * WAVES * 32 + first);
+    if (a.causal) end = min(end, (qt + 1) * ROWS * 32 + first);
     const int tiles = (end + N - 1) / N;
     const T *k = row<T>(a.k, b, 0, g), *v = row<T>(a.v, b, 0, g);
 
-    Stage<T, DP, N, THREADS> sk(a.k.ss, a.d), sv(a.v.ss, a.d);
+    Stage<T, DP, N, THREADS> sk(a.k.ss, a.d, tid), sv(a.v.ss, a.d, tid);
     for (int chunk = 0; chunk < tiles; chunk += 64) {
         Visits visits = visits_of<N>(keys, b, chunk, tiles - chunk, block_docs, wave_docs);
+        uint64_t mine = 0;
         int next = 0, key_doc = -1;
         auto fetch = [&] {
-            next = (chunk + __builtin_ctzll(visits.block)) * N;
+            mine = bit_of(visits.block, share);
+            if (!mine) return;
+            next = (chunk + __builtin_ctzll(mine)) * N;
             sk.load(k + (int64_t)next * a.k.ss, a.sk - next);
             sv.load(v + (int64_t)next * a.v.ss, a.sk - next);
-            int j = next + threadIdx.x;
-            if ((int)threadIdx.x < N) key_doc = j < a.sk ? doc_row ? max(doc_row[j], -1) : 0 : -1;
+            int j = next + tid;
+            if (tid < N) key_doc = j < a.sk ? doc_row ? max(doc_row[j], -1) : 0 : -1;
         };
         if (visits.block) fetch();
         while (visits.block) {
             __syncthreads();
             sk.store(tile_k);
             sv.store(tile_v);
-            if ((int)threadIdx.x < N) docs[threadIdx.x] = key_doc;
+            if (tid < N) docs[tid] = key_doc;
             __syncthreads();
-            const uint64_t bit = visits.block & -visits.block;
+            const uint64_t bit = mine;
             const int at = next;
-            visits.block ^= bit;
+            visits.block = without<SHARES>(visits.block);
             if (visits.block) fetch();
             if (!(visits.wave & bit) || (a.causal && at > wave_last)) continue;
             const bool by_document = !(visits.whole & bit) || at + N > a.sk;
@@ -1053,6 +1143,28 @@ void dq_kernel(const Args a, const Ranges keys, const Ranges queries, int tiles_
         }
     }
 
+    if constexpr (SHARES > 1) {
+        float* box = shared.boxes + wave * BOX;
+        __syncthreads();
+        if (share) {
+            float* to = box + (share - 1) * ROWS * BOX;
+            leave<DP>(to, acc);
+            if constexpr (CORRECTED<T>) {
+                leave<DP>(to + DP / 2 * 64, mean);
+                to[DP * 64 + lane] = rest;
+            }
+        }
+        __syncthreads();
+        if (share) return;
+        for (int n = 0; n < SHARES - 1; ++n, box += ROWS * BOX) {
+            take<DP>(box, 1.f, 1.f, acc);
+            if constexpr (CORRECTED<T>) {
+                take<DP>(box + DP / 2 * 64, 1.f, 1.f, mean);
+                rest += box[DP * 64 + lane];
+            }
+        }
+    }
+
     bool fine = true;
     float back = a.scale;
     if constexpr (FACTORED<T>) back *= exp2f(-SHIFT) / factor;
@@ -1085,21 +1197,27 @@ void dq_kernel(const Args a, const Ranges keys, const Ranges queries, int tiles_
         dq_row<T>(a, b, h, row0 + __builtin_ctzll(rows));
 }
 
-template <typename T, int DP, int WAVES>
-__global__ __launch_bounds__(WAVES * 64, DP >= 96 || (DP == 64 && sizeof(T) == 4) ? 1 : 2)
+template <typename T, int DP, int ROWS, int SHARES>
+__global__ __launch_bounds__(ROWS * SHARES * 64, DP >= 96 || (DP == 64 && sizeof(T) == 4) || SHARES == 4 ? 1 : 2)
 void dkv_kernel(const Args a, const Ranges keys, const Ranges queries, int tiles_k,
                 const float* factors, int factors_n) {
     using G = Tile<T, DP>;
-    constexpr int THREADS = WAVES * 64, N = G::KEYS;  // N queries a tile
-    __shared__ alignas(16) T tile_q[N * G::LD], tile_o[N * G::LD];
-    __shared__ alignas(16) int docs[N];
-    __shared__ alignas(16) float lses[N], deltas[N];
+    constexpr int THREADS = ROWS * 64, N = tile_rows<T, SHARES>;  // queries a tile
+    constexpr int BOX = DP * 64;  // dk and dv
+    __shared__ Shared<T, DP, N, SHARES, (SHARES - 1) * ROWS * BOX> shared;
+    __shared__ alignas(16) int tile_docs[SHARES][N];
+    __shared__ alignas(16) float tile_lses[SHARES][N], tile_deltas[SHARES][N];
 
     unsigned id = xcd_order(blockIdx.x, gridDim.x);
     const int kt = id % tiles_k, g = id / tiles_k % a.hkv, b = id / tiles_k / a.hkv;
     const int group = a.hq / a.hkv, lane = threadIdx.x & 63, hf = lane >> 5;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int first = a.sk - a.sq, block0 = kt * WAVES * 32;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % ROWS;
+    const int share = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) / ROWS;
+    const int tid = threadIdx.x - share * THREADS;
+    T *tile_q = shared.tiles[share][0], *tile_o = shared.tiles[share][1];
+    int* docs = tile_docs[share];
+    float *lses = tile_lses[share], *deltas = tile_deltas[share];
+    const int first = a.sk - a.sq, block0 = kt * ROWS * 32;
     const int key0 = block0 + wave * 32, j = key0 + (lane & 31);
     const bool there = j < a.sk;
     const int* doc_row = a.documents ? a.documents + b * a.documents_sb : nullptr;
@@ -1122,27 +1240,29 @@ void dkv_kernel(const Args a, const Ranges keys, const Ranges queries, int tiles
     const int doc = seen < 0 ? INT_MIN : seen;
     int2 wave_docs{}, block_docs{};
     if (doc_row) {
-        wave_docs = keys.of(b, kt * WAVES + wave);
-        block_docs = keys.of(b, kt * WAVES);
-        for (int w = 1; w < WAVES; ++w) block_docs = both(block_docs, keys.of(b, kt * WAVES + w));
+        wave_docs = keys.of(b, kt * ROWS + wave);
+        block_docs = keys.of(b, kt * ROWS);
+        for (int w = 1; w < ROWS; ++w) block_docs = both(block_docs, keys.of(b, kt * ROWS + w));
     }
     const int wave_last = min(key0 + 31, a.sk - 1);
     const int tiles = (a.sq + N - 1) / N;
     const int begin = a.causal ? max(0, block0 - first) / N : 0;
 
-    Stage<T, DP, N, THREADS> sq(a.q.ss, a.d), so(a.dout.ss, a.d);
+    Stage<T, DP, N, THREADS> sq(a.q.ss, a.d, tid), so(a.dout.ss, a.d, tid);
     for (int chunk = begin; chunk < tiles; chunk += 64) {
         const Visits visits = visits_of<N>(queries, b, chunk, tiles - chunk, block_docs, wave_docs);
         if (!visits.block) continue;
-        uint64_t left = visits.block;
+        uint64_t left = visits.block, mine = 0;
         int next = 0, next_h = g * group, query_doc = -1;
         float lse = 0, delta = 0, next_factor = 1.f;
         auto fetch = [&] {
-            next = (chunk + __builtin_ctzll(left)) * N;
+            mine = bit_of(left, share);
+            if (!mine) return;
+            next = (chunk + __builtin_ctzll(mine)) * N;
             sq.load(row<T>(a.q, b, next, next_h), a.sq - next);
             so.load(row<T>(a.dout, b, next, next_h), a.sq - next);
-            if ((int)threadIdx.x < N) {
-                int i = next + threadIdx.x;
+            if (tid < N) {
+                int i = next + tid;
                 int64_t at = ((int64_t)b * a.hq + next_h) * a.sq + i;
                 lse = i < a.sq ? usable(a.lse[at]) : INFINITY;
                 delta = i < a.sq ? a.delta[at] : 0.f;
@@ -1156,16 +1276,16 @@ void dkv_kernel(const Args a, const Ranges keys, const Ranges queries, int tiles
             __syncthreads();
             sq.store(tile_q);
             so.store(tile_o);
-            if ((int)threadIdx.x < N) {
-                docs[threadIdx.x] = query_doc;
-                lses[threadIdx.x] = lse;
-                deltas[threadIdx.x] = delta;
+            if (tid < N) {
+                docs[tid] = query_doc;
+                lses[tid] = lse;
+                deltas[tid] = delta;
             }
             __syncthreads();
-            const uint64_t bit = left & -left;
+            const uint64_t bit = mine;
             const int at = next, h = next_h;
             const float tile_factor = next_factor;
-            left ^= bit;
+            left = without<SHARES>(left);
             if (!left && next_h + 1 < (g + 1) * group) {  // the next head of the group
                 left = visits.block;
                 ++next_h;
@@ -1231,6 +1351,24 @@ void dkv_kernel(const Args a, const Ranges keys, const Ranges queries, int tiles
         back_v = exp2f(-SHIFT);
         back_k *= back_v / factor;
     }
+#pragma unroll
+    for (int n = 0; n < DP / 32; ++n)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) dk[n][e] *= back_k, dv[n][e] *= back_v;
+    if constexpr (SHARES > 1) {
+        float* box = shared.boxes + wave * BOX;
+        __syncthreads();
+        if (share) {
+            leave<DP>(box + (share - 1) * ROWS * BOX, dk);
+            leave<DP>(box + (share - 1) * ROWS * BOX + BOX / 2, dv);
+        }
+        __syncthreads();
+        if (share) return;
+        for (int n = 0; n < SHARES - 1; ++n, box += ROWS * BOX) {
+            take<DP>(box, 1.f, 1.f, dk);
+            take<DP>(box + BOX / 2, 1.f, 1.f, dv);
+        }
+    }
     bool fine = true;
     if (there) {
         T *to_k = row<T>(a.dk, b, j, g), *to_v = row<T>(a.dv, b, j, g);
@@ -1240,17 +1378,15 @@ void dkv_kernel(const Args a, const Ranges keys, const Ranges queries, int tiles
             for (int r = 0; r < 4; ++r) {
                 int d = n * 32 + r * 8 + hf * 4, e = r * 4;
                 if (d < a.d) {
-                    put4(to_k + d, dk[n][e] * back_k, dk[n][e + 1] * back_k, dk[n][e + 2] * back_k,
-                         dk[n][e + 3] * back_k);
-                    put4(to_v + d, dv[n][e] * back_v, dv[n][e + 1] * back_v, dv[n][e + 2] * back_v,
-                         dv[n][e + 3] * back_v);
+                    put4(to_k + d, dk[n][e], dk[n][e + 1], dk[n][e + 2], dk[n][e + 3]);
+                    put4(to_v + d, dv[n][e], dv[n][e + 1], dv[n][e + 2], dv[n][e + 3]);
                 }
 #pragma unroll
                 for (int x = e; x < e + 4; ++x)
                     fine &= fabsf(dk[n][x]) <= 3.4028235e38f && fabsf(dv[n][x]) <= 3.4028235e38f;
             }
     }
-    uint64_t bad = __ballot(!fine);
+    uint64_t bad = __ballot(there && !fine);
     for (uint64_t rows = (bad | bad >> 32) & 0xffffffffull; rows; rows &= rows - 1)
         dkv_row<T>(a, b, g, key0 + __builtin_ctzll(rows));
 }
@@ -1259,15 +1395,21 @@ template <typename T, int DP>
 void launch_backward(const Args& a, const Ranges& keys, const Ranges& queries, float* factors,
                      int factors_n, hipStream_t stream) {
     int64_t rows = (int64_t)a.b * a.hq * factors_n;
-    int tiles_q = (a.sq + 127) / 128, tiles_k = (a.sk + 127) / 128;
-    int64_t blocks_q = (int64_t)a.b * a.hq * tiles_q, blocks_k = (int64_t)a.b * a.hkv * tiles_k;
-    TORCH_CHECK(rows <= INT_MAX && blocks_k <= INT_MAX, "too many rows for one launch");
+    TORCH_CHECK(rows <= INT_MAX, "too many rows for one launch");
     hipLaunchKernelGGL(delta_kernel<T>, dim3((unsigned)rows), dim3(256), 0, stream, a, factors_n,
                        factors);
-    hipLaunchKernelGGL((dq_kernel<T, DP, 4>), dim3((unsigned)blocks_q), dim3(256), 0, stream, a,
-                       keys, queries, tiles_q, factors, factors_n);
-    hipLaunchKernelGGL((dkv_kernel<T, DP, 4>), dim3((unsigned)blocks_k), dim3(256), 0, stream, a,
-                       keys, queries, tiles_k, factors, factors_n);
+    for_shape((int64_t)a.b * a.hq, a.sq, [&](auto rows, auto shares, int tiles, unsigned blocks) {
+        constexpr int ROWS = decltype(rows)::value, SHARES = decltype(shares)::value;
+        hipLaunchKernelGGL((dq_kernel<T, DP, ROWS, SHARES>), dim3(blocks),
+                           dim3(ROWS * SHARES * 64), 0, stream, a, keys, queries, tiles, factors,
+                           factors_n);
+    });
+    for_shape((int64_t)a.b * a.hkv, a.sk, [&](auto rows, auto shares, int tiles, unsigned blocks) {
+        constexpr int ROWS = decltype(rows)::value, SHARES = decltype(shares)::value;
+        hipLaunchKernelGGL((dkv_kernel<T, DP, ROWS, SHARES>), dim3(blocks),
+                           dim3(ROWS * SHARES * 64), 0, stream, a, keys, queries, tiles, factors,
+                           factors_n);
+    });
 }
 
 // f of the head size, as the constant of its padded width
