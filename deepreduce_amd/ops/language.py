@@ -37,18 +37,19 @@ def _check(ok: bool, message: str) -> None:
 class _Attention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, documents, slopes, causal, scale):
-        out, lse = _attention_forward(q, k, v, documents, slopes, causal, scale, True)
-        ctx.save_for_backward(q, k, v, out, lse, documents, slopes)
+        out, lse, *ranges = _attention_forward(q, k, v, documents, slopes, causal, scale, True)
+        ctx.save_for_backward(q, k, v, out, lse, documents, slopes, *ranges)
         ctx.options = (causal, scale)
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
-        q, k, v, out, lse, documents, slopes = ctx.saved_tensors
+        q, k, v, out, lse, documents, slopes, *ranges = ctx.saved_tensors
         hip = _hip(q)
         backward = hip.attention_backward if hip else _ref.attention_backward
-        dq, dk, dv = backward(dout, q, k, v, out, lse, documents, slopes, *ctx.options)
+        dq, dk, dv = backward(
+            dout, q, k, v, out, lse, ranges, documents, slopes, *ctx.options)
         return dq, dk, dv, None, None, None, None
 
 

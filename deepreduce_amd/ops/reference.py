@@ -190,7 +190,7 @@ def attention_forward(q, k, v, documents, slopes, causal, scale, want_lse):
     return out, lse if want_lse else None
 
 
-def attention_backward(dout, q, k, v, out, lse, documents, slopes, causal, scale):
+def attention_backward(dout, q, k, v, out, lse, ranges, documents, slopes, causal, scale):
     s, seen = _attention_parts(q, k, documents, slopes, causal, scale)
     group = q.shape[2] // k.shape[2]
     seen = seen & (lse != float("-inf")).unsqueeze(-1)

@@ -21,6 +21,7 @@
 #include <c10/core/DeviceGuard.h>
 #include <hip/hip_runtime.h>
 #include <algorithm>
+#include <cmath>
 
 namespace {
 
@@ -43,6 +44,7 @@ struct Args {
     int b, sq, sk, hq, hkv, d;
     int causal;
     float scale;
+    float c;                 // the scores' factor in log2 units, not 0: hidden ones stay -inf
 };
 
 template <typename T>
@@ -510,6 +512,26 @@ __device__ __forceinline__ void hide_before(acc16& x, int t, int begin) {
     for (int i = 0; i < 16; ++i) x[i] = 8 * (i >> 2) + (i & 3) < l ? -INFINITY : x[i];
 }
 
+// products to the exponents of their probabilities; far: how far the query lies
+// behind the tile's first key of this half
+template <int KT>
+__device__ __forceinline__ void exponents(acc16* s, float c, float off, float slope, float far) {
+    if (slope != 0.f) {
+#pragma unroll
+        for (int t = 0; t < KT; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                s[t][i] = fmaf(s[t][i], c,
+                               fmaf(-slope, fabsf(far - (float)(t * 32 + 8 * (i >> 2) + (i & 3))),
+                                    -off));
+    } else {
+#pragma unroll
+        for (int t = 0; t < KT; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[t][i] = fmaf(s[t][i], c, -off);
+    }
+}
+
 // One wave's 32 queries against tiles of keys: the running softmax.
 template <typename T, int DP> struct Forward {
     using G = Tile<T, DP>;
@@ -526,7 +548,7 @@ template <typename T, int DP> struct Forward {
     __device__ __forceinline__ void begin(const Args& a, const T* row, bool there, float slope_) {
         const int hf = (threadIdx.x & 63) >> 5;
         slope = slope_;
-        c = fabsf(a.scale) * LOG2E;
+        c = a.c;
 #pragma unroll
         for (int n = 0; n < DP / 16; ++n) {
             q[n] = row_frag<T>(row, n * 16 + hf * 8, a.d, there);
@@ -543,7 +565,7 @@ template <typename T, int DP> struct Forward {
     // be hidden by their documents or lie past the query
     template <int KT, typename K>
     __device__ __forceinline__ void step(K k, const T* v, const int* docs, int key0,
-                                         bool biased, bool by_document, bool by_position) {
+                                         bool by_document, bool by_position) {
         const int hf = (threadIdx.x & 63) >> 5;
         acc16 s[KT];
 #pragma unroll
@@ -552,21 +574,7 @@ template <typename T, int DP> struct Forward {
 #pragma unroll
             for (int n = 0; n < DP / 16; ++n) s[t] = mma(k(t, n), q[n], s[t]);
         }
-        if (biased) {
-            const float far = (float)(pos - key0 - 4 * hf);
-#pragma unroll
-            for (int t = 0; t < KT; ++t)
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    s[t][i] = fmaf(s[t][i], c,
-                                   fmaf(-slope, fabsf(far - (float)(t * 32 + 8 * (i >> 2) + (i & 3))),
-                                        -off));
-        } else {
-#pragma unroll
-            for (int t = 0; t < KT; ++t)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) s[t][i] = fmaf(s[t][i], c, -off);
-        }
+        exponents<KT>(s, c, off, slope, (float)(pos - key0 - 4 * hf));
         if (by_document)
 #pragma unroll
             for (int t = 0; t < KT; ++t) hide_documents(s[t], docs, t, doc);
@@ -630,7 +638,7 @@ __device__ __forceinline__ void put4(T* at, float a, float b, float c, float d) 
 // tiles of K and V; block tiles of one head are neighbours on one XCD, whose
 // L2 then serves the head's keys once.
 template <typename T, int DP, int ROWS, int SHARES>
-__global__ __launch_bounds__(ROWS * SHARES * 64, (DP == 128 && (ROWS < 4 || sizeof(T) == 4)) || SHARES == 4 ? 1 : 2)
+__global__ __launch_bounds__(ROWS * SHARES * 64, (DP >= 96 && SHARES > 1) || (DP == 128 && sizeof(T) == 4) || SHARES == 4 ? 1 : 2)
 void forward_kernel(const Args a, const Ranges keys, const Ranges queries, int tiles_q) {
     using G = Tile<T, DP>;
     constexpr int BOX = (DP / 2 + 2) * 64;  // o, off and total
@@ -667,7 +675,6 @@ void forward_kernel(const Args a, const Ranges keys, const Ranges queries, int t
     int end = a.sk;
     if (a.causal) end = min(end, (qt + 1) * ROWS * 32 + first);
     const int tiles = (end + N - 1) / N;
-    const bool biased = f.slope != 0.f;
     const T *k = row<T>(a.k, b, 0, g), *v = row<T>(a.v, b, 0, g);
 
     Stage<T, DP, N, THREADS> sk(a.k.ss, a.d, tid), sv(a.v.ss, a.d, tid);
@@ -698,7 +705,7 @@ void forward_kernel(const Args a, const Ranges keys, const Ranges queries, int t
             if (!(visits.wave & bit) || (a.causal && at > wave_last)) continue;
             f.template step<N / 32>(
                 [&](int t, int n) { return rows_of<T, G::LD>(tile_k, t * 32, n * 16); }, tile_v,
-                docs, at, biased, !(visits.whole & bit) || at + N > a.sk,
+                docs, at, !(visits.whole & bit) || at + N > a.sk,
                 a.causal && at + N - 1 > wave_first);
         }
     }
@@ -775,7 +782,6 @@ __global__ __launch_bounds__(64, DP >= 96 ? 1 : 2) void split_kernel(const Args 
 
     Forward<T, DP> f;
     f.begin(a, row<T>(a.q, b, i, h), there, slope_of(a, h));
-    const bool biased = __any(f.slope != 0.f);
     f.pos = i + first;
     const int doc = there ? doc_row ? doc_row[f.pos] : 0 : -1;
     f.doc = doc < 0 ? INT_MIN : doc;
@@ -836,7 +842,7 @@ __global__ __launch_bounds__(64, DP >= 96 ? 1 : 2) void split_kernel(const Args 
                 at = chunk + __builtin_ctzll(visits) * N;
                 fetch(at);
             }
-            f.template step<1>([&](int, int n) { return k_now[n]; }, tile_v, docs, now, biased,
+            f.template step<1>([&](int, int n) { return k_now[n]; }, tile_v, docs, now,
                                doc_row || now + N > a.sk, a.causal && now + N - 1 > earliest);
         }
     }
@@ -888,8 +894,10 @@ __global__ __launch_bounds__(256) void join_kernel(const Args a, int parts, cons
     if (share < SHARES) {
         const float* from = part_o + (int64_t)blockIdx.x * parts * DP + d;
 #pragma unroll 4
-        for (int p = share; p < parts; p += SHARES)
-            if (weight[p] != 0.f) o = fmaf(weight[p], from[(int64_t)p * DP], o);
+        for (int p = share; p < parts; p += SHARES) {
+            const float w = weight[p], x = from[(int64_t)p * DP];
+            o = w == 0.f ? o : fmaf(w, x, o);
+        }
     }
     values[tid] = o;
     __syncthreads();
@@ -927,9 +935,9 @@ void for_shape(int64_t heads, int length, F f) {
         go(std::integral_constant<int, 1>{}, std::integral_constant<int, 4>{});
 }
 
-// Whether the forward pass is split over the keys: where 64 queries a block
+// Whether the forward pass is split over the keys: where 32 queries a block
 // give fewer blocks than there are CUs.
-bool split_keys(const Args& a) { return (int64_t)a.b * a.hq * ((a.sq + 63) / 64) < 256; }
+bool split_keys(const Args& a) { return (int64_t)a.b * a.hq * ((a.sq + 31) / 32) < 256; }
 
 template <typename T, int DP>
 void launch_split(const Args& a, const torch::Tensor& like, hipStream_t stream) {
@@ -961,18 +969,18 @@ void launch_forward(const Args& a, const Ranges& keys, const Ranges& queries,
 }
 
 // ---------------------------------------------------------------------------
-// Backward.  delta and the queries' gradient, whose waves hold 32 queries as
-// the forward's do; then the keys' and values', whose waves hold 32 keys and
-// go over the queries of all heads that share them.  Scores are formed again
+// Backward.  First the queries' gradient, whose waves hold 32 queries as the
+// forward's do, and their delta; then the keys' and values', whose waves hold
+// 32 keys and go over the queries of all heads that share them.  Scores are formed again
 // in both (7 products where 5 would do), so that nothing is added across
 // blocks: results repeat bit by bit and no buffer of gradients is needed.
 //
 // dS is rounded to the inputs' type for its products.  In fp16 it first gets
-// a factor, a power of two that puts its queries' largest dout near 2^-4 and
-// P's 2^12 with it, so that gradients of any size keep their bits.
+// a factor, a power of two that puts the largest dout of 32 queries near 2^-4
+// and P's 2^12 with it, so that gradients of any size keep their bits.
 // ---------------------------------------------------------------------------
 
-constexpr int FACTOR_ROWS = 64;
+constexpr int FACTOR_ROWS = 32;
 
 template <typename T> constexpr bool FACTORED = std::is_same<T, _Float16>::value;
 
@@ -985,43 +993,10 @@ template <typename T> constexpr bool CORRECTED = sizeof(T) == 2;
 // rows that saw nothing have probabilities of zero
 __device__ __forceinline__ float usable(float lse) { return lse == -INFINITY ? INFINITY : lse; }
 
-// 64 rows a block, 4 threads a row; one read of dout and out bounds it
-template <typename T>
-__global__ __launch_bounds__(256) void delta_kernel(const Args a, int tiles, float* factors) {
-    int t = blockIdx.x % tiles, h = blockIdx.x / tiles % a.hq, b = blockIdx.x / tiles / a.hq;
-    int i = t * FACTOR_ROWS + (threadIdx.x >> 2);
-    float sum = 0, most = 0;
-    if (i < a.sq) {
-        const T *x = row<T>(a.dout, b, i, h), *y = row<T>(a.out, b, i, h);
-        for (int d = (threadIdx.x & 3) * 8; d < a.d; d += 32) {
-            Frag<T> u = *(const Frag<T>*)(x + d), w = *(const Frag<T>*)(y + d);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                sum = fmaf((float)u[e], (float)w[e], sum);
-                float size = fabsf((float)u[e]);
-                if (FACTORED<T> && size < INFINITY) most = fmaxf(most, size);
-            }
-        }
-    }
-    sum += __shfl_xor(sum, 1);
-    sum += __shfl_xor(sum, 2);
-    if (i < a.sq && (threadIdx.x & 3) == 0) a.delta[((int64_t)b * a.hq + h) * a.sq + i] = sum;
-    if constexpr (FACTORED<T>) {
-        __shared__ float shared[4];
-        most = wave_max(most);
-        if ((threadIdx.x & 63) == 0) shared[threadIdx.x >> 6] = most;
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            for (int w = 1; w < 4; ++w) most = fmaxf(most, shared[w]);
-            factors[blockIdx.x] = most == 0.f ? 1.f : exp2f(-4.f - ceilf(log2f(most)));
-        }
-    }
-}
-
 template <typename T, int DP, int ROWS, int SHARES>
-__global__ __launch_bounds__(ROWS * SHARES * 64, DP >= 96 || SHARES == 4 ? 1 : 2)
+__global__ __launch_bounds__(ROWS * SHARES * 64, DP >= 96 || SHARES > 1 ? 1 : 2)
 void dq_kernel(const Args a, const Ranges keys, const Ranges queries, int tiles_q,
-               const float* factors, int factors_n) {
+               float* factors, int factors_n) {
     using G = Tile<T, DP>;
     constexpr int BOX = (CORRECTED<T> ? DP + 1 : DP / 2) * 64;  // acc, mean and rest
     constexpr int THREADS = ROWS * 64, N = tile_rows<T, SHARES>;
@@ -1043,22 +1018,34 @@ void dq_kernel(const Args a, const Ranges keys, const Ranges queries, int tiles_
     const int* doc_row = a.documents ? a.documents + b * a.documents_sb : nullptr;
     const int64_t at_row = ((int64_t)b * a.hq + h) * a.sq + i;
 
-    const float c = fabsf(a.scale) * LOG2E, slope = slope_of(a, h);
+    const float c = a.c, slope = slope_of(a, h);
     Frag<T> q[DP / 16], dout[DP / 16];
+    float delta = 0, most = 0;
 #pragma unroll
     for (int n = 0; n < DP / 16; ++n) {
         q[n] = row_frag<T>(row<T>(a.q, b, there ? i : 0, h), n * 16 + hf * 8, a.d, there);
         dout[n] = row_frag<T>(row<T>(a.dout, b, there ? i : 0, h), n * 16 + hf * 8, a.d, there);
+        const Frag<T> out =
+            row_frag<T>(row<T>(a.out, b, there ? i : 0, h), n * 16 + hf * 8, a.d, there);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float x = (float)dout[n][e];
+            delta = fmaf(x, (float)out[e], delta);
+            if (FACTORED<T>) most = fabsf(x) < INFINITY ? fmaxf(most, fabsf(x)) : most;
+        }
         if (a.scale < 0) q[n] = -q[n];
     }
+    delta = add_halves(delta);
     acc16 acc[DP / 32], mean[DP / 32];  // mean: sum of P k
 #pragma unroll
     for (int n = 0; n < DP / 32; ++n) acc[n] = acc16{}, mean[n] = acc16{};
-    const float delta = there ? a.delta[at_row] : 0.f;
     float off = there ? usable(a.lse[at_row]) : INFINITY, rest = 0, factor = 1.f;
     if constexpr (FACTORED<T>) {
-        factor = factors[((int64_t)b * a.hq + h) * factors_n + min(i, a.sq - 1) / FACTOR_ROWS];
+        most = wave_max(most);
+        factor = most == 0.f ? 1.f : exp2f(-4.f - ceilf(log2f(most)));
         off -= SHIFT;
+        if (lane == 0 && row0 < a.sq)
+            factors[((int64_t)b * a.hq + h) * factors_n + row0 / FACTOR_ROWS] = factor;
     }
 
     const int seen = there ? doc_row ? doc_row[pos] : 0 : -1;
@@ -1112,16 +1099,7 @@ void dq_kernel(const Args a, const Ranges keys, const Ranges queries, int tiles_
 #pragma unroll
                 for (int n = 0; n < DP / 16; ++n)
                     dp = mma(rows_of<T, G::LD>(tile_v, t * 32, n * 16), dout[n], dp);
-                if (slope != 0.f) {
-                    const float far = (float)(pos - at - t * 32 - 4 * hf);
-#pragma unroll
-                    for (int e = 0; e < 16; ++e)
-                        s[e] = fmaf(s[e], c,
-                                    fmaf(-slope, fabsf(far - (float)(8 * (e >> 2) + (e & 3))), -off));
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) s[e] = fmaf(s[e], c, -off);
-                }
+                exponents<1>(&s, c, off, slope, (float)(pos - at - t * 32 - 4 * hf));
                 if (by_document) hide_documents(s, docs, t, doc);
                 if (by_position) hide_past(s, t, pos - at);
                 float sum = 0;
@@ -1176,8 +1154,9 @@ void dq_kernel(const Args a, const Ranges keys, const Ranges queries, int tiles_
         for (int n = 0; n < DP / 32; ++n)
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[n][e] = fmaf(-by, mean[n][e], acc[n][e]);
-        if (there && hf == 0) a.delta[at_row] = FACTORED<T> ? delta + by / factor : delta + rest;
+        delta += FACTORED<T> ? by / factor : rest;
     }
+    if (there && hf == 0) a.delta[at_row] = delta;
     if (there) {
         T* dq = row<T>(a.dq, b, i, h);
 #pragma unroll
@@ -1222,7 +1201,7 @@ void dkv_kernel(const Args a, const Ranges keys, const Ranges queries, int tiles
     const bool there = j < a.sk;
     const int* doc_row = a.documents ? a.documents + b * a.documents_sb : nullptr;
 
-    const float c = fabsf(a.scale) * LOG2E;
+    const float c = a.c;
     Frag<T> k[DP / 16], v[DP / 16];
 #pragma unroll
     for (int n = 0; n < DP / 16; ++n) {
@@ -1264,12 +1243,16 @@ void dkv_kernel(const Args a, const Ranges keys, const Ranges queries, int tiles
             if (tid < N) {
                 int i = next + tid;
                 int64_t at = ((int64_t)b * a.hq + next_h) * a.sq + i;
-                lse = i < a.sq ? usable(a.lse[at]) : INFINITY;
+                lse = i < a.sq ? usable(a.lse[at]) - (FACTORED<T> ? SHIFT : 0.f) : INFINITY;
                 delta = i < a.sq ? a.delta[at] : 0.f;
                 query_doc = i < a.sq ? doc_row ? max(doc_row[i + first], -1) : 0 : -1;
             }
-            if constexpr (FACTORED<T>)
-                next_factor = factors[((int64_t)b * a.hq + next_h) * factors_n + next / FACTOR_ROWS];
+            if constexpr (FACTORED<T>) {
+                const float* f = factors + ((int64_t)b * a.hq + next_h) * factors_n;
+                next_factor = f[next / FACTOR_ROWS];
+                for (int n = FACTOR_ROWS; n < N && next + n < a.sq; n += FACTOR_ROWS)
+                    next_factor = fminf(next_factor, f[(next + n) / FACTOR_ROWS]);
+            }
         };
         fetch();
         while (left) {
@@ -1307,6 +1290,7 @@ void dkv_kernel(const Args a, const Ranges keys, const Ranges queries, int tiles
                 }
             }
             const float slope = slope_of(a, h), far = (float)(at + first + 4 * hf - j);
+            const float by_slope = slope / c;
 #pragma unroll
             for (int t = 0; t < N / 32; ++t) {
                 acc16 s = {}, dp = {};
@@ -1316,29 +1300,26 @@ void dkv_kernel(const Args a, const Ranges keys, const Ranges queries, int tiles
 #pragma unroll
                 for (int n = 0; n < DP / 16; ++n)
                     dp = mma(rows_of<T, G::LD>(tile_o, t * 32, n * 16), v[n], dp);
+                if (slope != 0.f)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        s[e] = fmaf(-by_slope,
+                                    fabsf(far + (float)(t * 32 + 8 * (e >> 2) + (e & 3))), s[e]);
+                if (by_document) hide_documents(s, docs, t, doc);
+                if (by_position) hide_before(s, t, j - at - first);
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const int i = t * 32 + r * 8 + 4 * hf;
                     const f32x4 l = *(const f32x4*)(lses + i), dl = *(const f32x4*)(deltas + i);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        float off = l[e];
-                        if constexpr (FACTORED<T>) off -= SHIFT;
-                        if (slope != 0.f)
-                            off = fmaf(slope, fabsf(far + (float)(t * 32 + r * 8 + e)), off);
-                        s[r * 4 + e] = fmaf(s[r * 4 + e], c, -off);
+                        const int x = r * 4 + e;
+                        s[x] = exp2_fast(fmaf(s[x], c, -l[e]));
                         if constexpr (FACTORED<T>)
-                            dp[r * 4 + e] = fmaf(dp[r * 4 + e], factor, -dl[e] * factor);
+                            dp[x] = s[x] * fmaf(dp[x], factor, -dl[e] * factor);
                         else
-                            dp[r * 4 + e] -= dl[e];
+                            dp[x] = s[x] * (dp[x] - dl[e]);
                     }
-                }
-                if (by_document) hide_documents(s, docs, t, doc);
-                if (by_position) hide_before(s, t, j - at - first);
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    s[e] = exp2_fast(s[e]);
-                    dp[e] *= s[e];
                 }
                 add_product<T, DP>(tile_o, t * 32, s, dv);
                 add_product<T, DP>(tile_q, t * 32, dp, dk);
@@ -1394,10 +1375,6 @@ void dkv_kernel(const Args a, const Ranges keys, const Ranges queries, int tiles
 template <typename T, int DP>
 void launch_backward(const Args& a, const Ranges& keys, const Ranges& queries, float* factors,
                      int factors_n, hipStream_t stream) {
-    int64_t rows = (int64_t)a.b * a.hq * factors_n;
-    TORCH_CHECK(rows <= INT_MAX, "too many rows for one launch");
-    hipLaunchKernelGGL(delta_kernel<T>, dim3((unsigned)rows), dim3(256), 0, stream, a, factors_n,
-                       factors);
     for_shape((int64_t)a.b * a.hq, a.sq, [&](auto rows, auto shares, int tiles, unsigned blocks) {
         constexpr int ROWS = decltype(rows)::value, SHARES = decltype(shares)::value;
         hipLaunchKernelGGL((dq_kernel<T, DP, ROWS, SHARES>), dim3(blocks),
@@ -1429,12 +1406,26 @@ struct DocumentRanges {
     torch::Tensor buffer[2];
     Ranges keys{}, queries{};
 
-    DocumentRanges(const Args& a, const torch::Tensor& like, hipStream_t stream) {
+    // `known`: those that the forward pass has left, or nothing
+    DocumentRanges(const Args& a, const std::vector<torch::Tensor>& known,
+                   const torch::Tensor& like, hipStream_t stream) {
         if (!a.documents) return;
-        keys = fill(0, a, 0, like, stream);
         const int first = a.sk - a.sq;
-        if (first) queries = fill(1, a, first, like, stream);
-        else queries = keys;
+        if (!known.empty()) {
+            TORCH_CHECK(known.size() == (first ? 2 : 1), "ranges must be the forward's");
+            keys = over(known[0], a, 0);
+            queries = first ? over(known[1], a, first) : keys;
+            return;
+        }
+        keys = fill(0, a, 0, like, stream);
+        queries = first ? fill(1, a, first, like, stream) : keys;
+    }
+    static Ranges over(const torch::Tensor& t, const Args& a, int first) {
+        const int count = (a.sk - first + RANGE - 1) / RANGE;
+        TORCH_CHECK(t.is_cuda() && t.scalar_type() == torch::kInt32 && t.is_contiguous() &&
+                        t.numel() == (int64_t)a.b * count * 2,
+                    "ranges must be the forward's");
+        return {(const int2*)t.data_ptr<int>(), count};
     }
     Ranges fill(int n, const Args& a, int first, const torch::Tensor& like, hipStream_t stream) {
         const int count = (a.sk - first + RANGE - 1) / RANGE;
@@ -1503,6 +1494,7 @@ Args args_for(const torch::Tensor& q, const torch::Tensor& k, const torch::Tenso
     }
     a.causal = causal;
     a.scale = (float)scale;
+    a.c = std::max(std::fabs(a.scale) * LOG2E, 1e-30f);
     return a;
 }
 
@@ -1532,6 +1524,7 @@ std::vector<torch::Tensor> attention_forward(torch::Tensor q, torch::Tensor k, t
     a.lse = want_lse ? lse.data_ptr<float>() : nullptr;
     hipStream_t stream = at::hip::getCurrentHIPStream();
     if (out.numel() == 0) return {out, lse};
+    std::vector<torch::Tensor> results = {out, lse};
     for_type(q.scalar_type(), [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
         for_width(a.d, [&](auto width) {
@@ -1539,17 +1532,20 @@ std::vector<torch::Tensor> attention_forward(torch::Tensor q, torch::Tensor k, t
             if (split_keys(a)) {
                 launch_split<T, DP>(a, q, stream);
             } else {
-                DocumentRanges ranges(a, q, stream);
+                DocumentRanges ranges(a, {}, q, stream);
                 launch_forward<T, DP>(a, ranges.keys, ranges.queries, stream);
+                for (auto& r : ranges.buffer)
+                    if (r.defined()) results.push_back(r);
             }
         });
     });
-    return {out, lse};
+    return results;
 }
 
 std::vector<torch::Tensor> attention_backward(torch::Tensor dout, torch::Tensor q,
                                               torch::Tensor k, torch::Tensor v, torch::Tensor out,
                                               torch::Tensor lse,
+                                              std::vector<torch::Tensor> known_ranges,
                                               std::optional<torch::Tensor> documents,
                                               std::optional<torch::Tensor> slopes, bool causal,
                                               double scale) {
@@ -1575,8 +1571,9 @@ std::vector<torch::Tensor> attention_backward(torch::Tensor dout, torch::Tensor 
     hipStream_t stream = at::hip::getCurrentHIPStream();
     if (dq.numel() == 0) return {dq, dk.zero_(), dv.zero_()};
     const int factors_n = (a.sq + FACTOR_ROWS - 1) / FACTOR_ROWS;
-    auto factors = torch::empty({a.b, a.hq, factors_n}, lse.options());
-    DocumentRanges ranges(a, q, stream);
+    const bool factored = q.scalar_type() == torch::kFloat16;
+    auto factors = torch::empty({factored ? (int64_t)a.b * a.hq * factors_n : 0}, lse.options());
+    DocumentRanges ranges(a, known_ranges, q, stream);
     for_type(q.scalar_type(), [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
         for_width(a.d, [&](auto width) {

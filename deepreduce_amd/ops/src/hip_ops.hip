@@ -3251,6 +3251,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           "global 2-norm of many tensors, and the tensors scaled to at most max_norm (HIP)");
     m.def("rotary", &rotary, "rotary positions of one or two tensors (HIP)");
     m.def("attention_forward", &attention_forward,
-          "attention with documents, distance bias and causality -> (out, lse) (HIP)");
+          "attention with documents, distance bias and causality -> (out, lse, document ranges if it made any) (HIP)");
     m.def("attention_backward", &attention_backward, "its gradient -> (dq, dk, dv) (HIP)");
 }

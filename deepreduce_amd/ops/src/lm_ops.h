@@ -20,6 +20,7 @@ std::vector<torch::Tensor> attention_forward(torch::Tensor q, torch::Tensor k, t
 std::vector<torch::Tensor> attention_backward(torch::Tensor dout, torch::Tensor q,
                                               torch::Tensor k, torch::Tensor v, torch::Tensor out,
                                               torch::Tensor lse,
+                                              std::vector<torch::Tensor> ranges,
                                               std::optional<torch::Tensor> documents,
                                               std::optional<torch::Tensor> slopes, bool causal,
                                               double scale);

@@ -298,6 +298,16 @@ def test_attention_large_scores(device):
 
 
 @pytest.mark.parametrize("device", BOTH)
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("scale", [0.0, -0.3])
+def test_attention_scale(device, dtype, scale):
+    q, k, v, dout = attention_inputs(1, 75, 75, 2, 1, 64, dtype, device)
+    documents = DOCS["packed"](1, 75).to(device)
+    check_attention(q, k, v, dout, documents, torch.tensor([0.2, 0.0], device=device), True, scale)
+    check_attention(q[:, -1:], k, v, dout[:, -1:], documents, None, True, scale)
+
+
+@pytest.mark.parametrize("device", BOTH)
 def test_attention_without_rows(device):
     for b, sq, sk in ((0, 4, 4), (2, 0, 5), (2, 0, 0)):
         q, k, v, dout = attention_inputs(b, sq, sk, 2, 1, 16, torch.float32, device)
