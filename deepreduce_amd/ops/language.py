@@ -18,7 +18,7 @@ from . import reference as _ref
 TYPES = (torch.float32, torch.bfloat16, torch.float16)
 
 
-def _hip(t: torch.Tensor):
+def _hip(t):
     """The extension if `t` is on a GPU, None on the CPU."""
     from deepreduce_amd import ops
 
@@ -35,28 +35,20 @@ def _check(ok: bool, message: str) -> None:
 # --------------------------------------------------------------------------
 
 class _Attention(torch.autograd.Function):
+    """The CPU path; the extension has its own."""
+
     @staticmethod
     def forward(ctx, q, k, v, documents, slopes, causal, scale):
-        out, lse, *ranges = _attention_forward(q, k, v, documents, slopes, causal, scale, True)
-        ctx.save_for_backward(q, k, v, out, lse, documents, slopes, *ranges)
+        out, lse = _ref.attention_forward(q, k, v, documents, slopes, causal, scale)
+        ctx.save_for_backward(q, k, v, lse, documents, slopes)
         ctx.options = (causal, scale)
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
-        q, k, v, out, lse, documents, slopes, *ranges = ctx.saved_tensors
-        hip = _hip(q)
-        backward = hip.attention_backward if hip else _ref.attention_backward
-        dq, dk, dv = backward(
-            dout, q, k, v, out, lse, ranges, documents, slopes, *ctx.options)
-        return dq, dk, dv, None, None, None, None
-
-
-def _attention_forward(q, k, v, documents, slopes, causal, scale, want_lse):
-    hip = _hip(q)
-    forward = hip.attention_forward if hip else _ref.attention_forward
-    return forward(q, k, v, documents, slopes, causal, scale, want_lse)
+        grads = _ref.attention_backward(dout, *ctx.saved_tensors, *ctx.options)
+        return (*grads, None, None, None, None)
 
 
 def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
@@ -79,6 +71,9 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     causal: a query sees no later position.
     scale: factor of the scores, D ** -0.5 by default.
     """
+    hip = _hip(q)
+    if hip:
+        return hip.attention(q, k, v, documents, slopes, causal, scale)
     _check(all(t.dim() == 4 for t in (q, k, v)),
            "attention: q, k and v must be [batch, length, heads, head size]")
     _check(q.dtype in TYPES, f"attention: q must be float32, bfloat16 or float16, got {q.dtype}")
@@ -100,20 +95,14 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
         _check(documents.dtype == torch.int32 and documents.shape == (b, sk)
                and documents.device == q.device,
                f"attention: documents must be int32 [{b}, {sk}] on q's device")
-        if sk > 1 and documents.stride(1) != 1:
-            documents = documents.contiguous()
     if slopes is not None:
         _check(slopes.dtype == torch.float32 and slopes.shape == (hq,)
                and slopes.device == q.device,
                f"attention: slopes must be float32 [{hq}] on q's device")
         _check(not slopes.requires_grad, "attention: slopes are constants and get no gradient")
-        slopes = slopes.contiguous()
     scale = d ** -0.5 if scale is None else float(scale)
     _check(math.isfinite(scale), "attention: scale must be finite")
-    causal = bool(causal)
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        return _Attention.apply(q, k, v, documents, slopes, causal, scale)
-    return _attention_forward(q, k, v, documents, slopes, causal, scale, False)[0]
+    return _Attention.apply(q, k, v, documents, slopes, bool(causal), scale)
 
 
 # --------------------------------------------------------------------------
@@ -146,26 +135,20 @@ def rotary_frequencies(dim: int, base: float = 10000.0, factor: float = 1.0,
     return f.to(device)
 
 
-def _rotate(xs, positions, frequencies, interleaved, inverse):
-    hip = _hip(xs[0])
-    rotate = hip.rotary if hip else _ref.rotary
-    return rotate(xs, positions, frequencies, interleaved, inverse)
-
-
 class _Rotary(torch.autograd.Function):
+    """The CPU path; the extension has its own."""
+
     @staticmethod
     def forward(ctx, q, k, positions, frequencies, interleaved):
         ctx.save_for_backward(positions, frequencies)
         ctx.interleaved = interleaved
-        return tuple(_rotate([q, k], positions, frequencies, interleaved, False))
+        return tuple(_ref.rotary([q, k], positions, frequencies, interleaved, False))
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dq, dk):
-        positions, frequencies = ctx.saved_tensors
-        need = [d for d, n in zip((dq, dk), ctx.needs_input_grad) if n]
-        got = iter(_rotate(need, positions, frequencies, ctx.interleaved, True))
-        return tuple(next(got) if n else None for n in ctx.needs_input_grad[:2]) + (None,) * 3
+        grads = _ref.rotary([dq, dk], *ctx.saved_tensors, ctx.interleaved, True)
+        return (*grads, None, None, None)
 
 
 def rotary(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor,
@@ -179,6 +162,9 @@ def rotary(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor,
     (2 i, 2 i + 1) if interleaved.  Angles are formed in 64 bits, so far
     positions keep theirs.  Differentiable in q and k.
     """
+    hip = _hip(q)
+    if hip:
+        return tuple(hip.rotary(q, k, positions, frequencies, interleaved))
     _check(q.dim() == 4 and k.dim() == 4 and q.shape[:2] == k.shape[:2]
            and q.shape[3] == k.shape[3],
            f"rotary: q {tuple(q.shape)} and k {tuple(k.shape)} must be "
@@ -196,27 +182,24 @@ def rotary(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor,
            f"rotary: frequencies must be float64 with 1 to {d // 2} values")
     _check(not frequencies.requires_grad, "rotary: frequencies are constants and get no gradient")
     _check(d % 2 == 0 and d <= 1024, f"rotary: the head size must be even and at most 1024, got {d}")
-    positions = positions.expand(b, s)
-    frequencies = frequencies.contiguous()
-    interleaved = bool(interleaved)
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad):
-        return _Rotary.apply(q, k, positions, frequencies, interleaved)
-    return tuple(_rotate([q, k], positions, frequencies, interleaved, False))
+    return _Rotary.apply(q, k, positions.expand(b, s), frequencies, bool(interleaved))
 
 
 # --------------------------------------------------------------------------
 # the global gradient norm, and clipping
 # --------------------------------------------------------------------------
 
-def _gradients(tensors, name: str) -> list[torch.Tensor]:
+def _list(tensors) -> list[torch.Tensor]:
     grads = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
-    _check(len(grads) > 0, f"{name}: no tensors")
-    device = grads[0].device
+    _check(len(grads) > 0, "no tensors")
+    return grads
+
+
+def _check_gradients(grads, name: str) -> None:
     for t in grads:
-        if t.dtype not in TYPES or t.layout != torch.strided or t.device != device:
+        if t.dtype not in TYPES or t.layout != torch.strided or t.device != grads[0].device:
             raise ValueError(f"{name}: takes dense float32, bfloat16 or float16 tensors of one "
                              f"device, got {t.layout} {t.dtype} on {t.device}")
-    return grads
 
 
 def grad_norm(tensors) -> torch.Tensor:
@@ -225,9 +208,12 @@ def grad_norm(tensors) -> torch.Tensor:
     Tensors of any shape, order and mixture of float32, bfloat16 and float16.
     Squares are added in 64 bits, in a fixed order.  No gradient flows back.
     """
-    grads = _gradients(tensors, "grad_norm")
+    grads = _list(tensors)
     hip = _hip(grads[0])
-    return (hip.grad_norm if hip else _ref.grad_norm)([t.detach() for t in grads])
+    if hip:
+        return hip.grad_norm(grads)
+    _check_gradients(grads, "grad_norm")
+    return _ref.grad_norm([t.detach() for t in grads])
 
 
 def clip_grad_norm(tensors, max_norm: float, out=None, dtype: torch.dtype | None = None):
@@ -239,19 +225,24 @@ def clip_grad_norm(tensors, max_norm: float, out=None, dtype: torch.dtype | None
     infinite or NaN enters the product as it is: NaN reaches every value.  No
     gradient flows back.
     """
-    grads = _gradients(tensors, "clip_grad_norm")
+    grads, outs = _list(tensors), None if out is None else _list(out)
     max_norm = float(max_norm)
+    _check(dtype is None or dtype in TYPES,
+           f"clip_grad_norm: dtype must be float32, bfloat16 or float16, got {dtype}")
+    hip = _hip(grads[0])
+    if hip:
+        return hip.clip_grad_norm(grads, max_norm, outs, dtype)
+    _check_gradients(grads, "clip_grad_norm")
     _check(max_norm >= 0, f"clip_grad_norm: max_norm must be 0 or more, got {max_norm}")
-    _check(dtype is None or (out is None and dtype in TYPES),
-           "clip_grad_norm: dtype must be float32, bfloat16 or float16, without out")
-    if out is None:
+    _check(dtype is None or out is None, "clip_grad_norm: dtype is for new tensors, without out")
+    if outs is None:
         outs = [torch.empty_like(t, dtype=dtype, requires_grad=False) for t in grads]
-    else:
-        outs = _gradients(out, "clip_grad_norm")
-        _check(len(outs) == len(grads) and all(o.shape == t.shape for o, t in zip(outs, grads))
-               and outs[0].device == grads[0].device,
-               "clip_grad_norm: out must hold a tensor of each one's shape and device")
-    norm = _clip(grads, outs, max_norm)
+    _check_gradients(outs, "clip_grad_norm")
+    _check(len(outs) == len(grads) and all(o.shape == t.shape for o, t in zip(outs, grads))
+           and outs[0].device == grads[0].device,
+           "clip_grad_norm: out must hold a tensor of each one's shape and device")
+    _check_apart(grads, outs)
+    norm = _ref.clip_grad_norm([t.detach() for t in grads], [t.detach() for t in outs], max_norm)
     if out is not None:
         torch.autograd.graph.increment_version(outs)
     return outs, norm
@@ -259,22 +250,8 @@ def clip_grad_norm(tensors, max_norm: float, out=None, dtype: torch.dtype | None
 
 def clip_grad_norm_(tensors, max_norm: float) -> torch.Tensor:
     """`clip_grad_norm` in place; returns the norm that the tensors had."""
-    grads = _gradients(tensors, "clip_grad_norm_")
+    grads = _list(tensors)
     return clip_grad_norm(grads, max_norm, out=grads)[1]
-
-
-def _clip(grads, outs, max_norm):
-    hip = _hip(grads[0])
-    grads, outs = [t.detach() for t in grads], [t.detach() for t in outs]
-    if hip:
-        try:
-            return hip.clip_grad_norm(grads, outs, max_norm)
-        except RuntimeError as e:
-            if "share memory" in str(e) or "shares memory" in str(e):
-                raise ValueError(f"clip_grad_norm: {str(e).splitlines()[0]}") from None
-            raise
-    _check_apart(grads, outs)
-    return _ref.clip_grad_norm(grads, outs, max_norm)
 
 
 def _check_apart(grads, outs):

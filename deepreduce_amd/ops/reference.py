@@ -179,7 +179,7 @@ def _masked_product(w, x, seen):
     return y
 
 
-def attention_forward(q, k, v, documents, slopes, causal, scale, want_lse):
+def attention_forward(q, k, v, documents, slopes, causal, scale):
     s, seen = _attention_parts(q, k, documents, slopes, causal, scale)
     s = s.masked_fill(~seen, float("-inf"))
     lse = torch.logsumexp(s, -1) if s.shape[-1] else s.sum(-1) - float("inf")
@@ -187,10 +187,10 @@ def attention_forward(q, k, v, documents, slopes, causal, scale, want_lse):
     p = torch.where(seen, torch.exp(s - base.unsqueeze(-1)), torch.zeros_like(s))
     vf = v.float().transpose(1, 2).repeat_interleave(q.shape[2] // v.shape[2], 1)
     out = _masked_product(p, vf, seen).transpose(1, 2).contiguous().to(q.dtype)
-    return out, lse if want_lse else None
+    return out, lse
 
 
-def attention_backward(dout, q, k, v, out, lse, ranges, documents, slopes, causal, scale):
+def attention_backward(dout, q, k, v, lse, documents, slopes, causal, scale):
     s, seen = _attention_parts(q, k, documents, slopes, causal, scale)
     group = q.shape[2] // k.shape[2]
     seen = seen & (lse != float("-inf")).unsqueeze(-1)

@@ -1456,12 +1456,13 @@ torch::Tensor aligned(const torch::Tensor& t) {
 }
 
 Args args_for(const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& v,
-              const std::optional<torch::Tensor>& documents,
-              const std::optional<torch::Tensor>& slopes, bool causal, double scale) {
+              const torch::Tensor& documents, const torch::Tensor& slopes, bool causal,
+              double scale) {
     for (auto* t : {&q, &k, &v})
-        TORCH_CHECK(t->is_cuda() && t->dim() == 4 && t->device() == q.device() &&
-                        t->scalar_type() == q.scalar_type(),
-                    "q, k and v must be 4-D GPU tensors of one type and device");
+        TORCH_CHECK_VALUE(t->is_cuda() && t->dim() == 4 && t->device() == q.device() &&
+                              t->scalar_type() == q.scalar_type(),
+                          "attention: q, k and v must be [batch, length, heads, head size] of one "
+                          "type on one device");
     Args a{};
     a.b = (int)q.size(0);
     a.sq = (int)q.size(1);
@@ -1469,28 +1470,36 @@ Args args_for(const torch::Tensor& q, const torch::Tensor& k, const torch::Tenso
     a.d = (int)q.size(3);
     a.sk = (int)k.size(1);
     a.hkv = (int)k.size(2);
-    TORCH_CHECK(k.sizes() == v.sizes() && k.size(0) == a.b && k.size(3) == a.d,
-                "k and v must be [batch, length, heads, d] like q");
-    TORCH_CHECK(a.d >= 8 && a.d <= MOST_D && a.d % 8 == 0,
-                "the head size must be a multiple of 8 from 8 to 128");
-    TORCH_CHECK(a.hkv >= 1 && a.hq % a.hkv == 0, "kv heads must divide the query heads");
-    TORCH_CHECK(a.sq <= a.sk, "there are more queries than keys");
-    TORCH_CHECK(k.size(1) < (1 << 30), "too many keys");
-    if (documents) {
-        TORCH_CHECK(documents->is_cuda() && documents->device() == q.device() &&
-                        documents->scalar_type() == torch::kInt32 && documents->dim() == 2 &&
-                        documents->size(0) == a.b && documents->size(1) == a.sk &&
-                        (documents->stride(1) == 1 || a.sk <= 1),
-                    "documents must be int32 [batch, keys]");
-        a.documents = documents->data_ptr<int>();
-        a.documents_sb = documents->stride(0);
+    TORCH_CHECK_VALUE(k.sizes() == v.sizes() && k.size(0) == a.b && k.size(3) == a.d,
+                      "attention: q ", q.sizes(), ", k ", k.sizes(), " and v ", v.sizes(),
+                      " do not fit");
+    TORCH_CHECK_VALUE(a.d >= 8 && a.d <= MOST_D && a.d % 8 == 0,
+                      "attention: the head size must be a multiple of 8 from 8 to 128, got ", a.d);
+    TORCH_CHECK_VALUE(a.hkv >= 1 && a.hq % a.hkv == 0, "attention: ", a.hkv,
+                      " key-value heads do not divide ", a.hq, " query heads");
+    TORCH_CHECK_VALUE(q.size(1) <= k.size(1), "attention: ", q.size(1), " queries over ",
+                      k.size(1), " keys; queries are the last positions");
+    TORCH_CHECK_VALUE(k.size(1) < (1 << 30), "attention: too many keys");
+    TORCH_CHECK_VALUE(std::isfinite(scale), "attention: scale must be finite");
+    if (documents.defined()) {
+        TORCH_CHECK_VALUE(documents.device() == q.device() &&
+                              documents.scalar_type() == torch::kInt32 && documents.dim() == 2 &&
+                              documents.size(0) == a.b && documents.size(1) == a.sk,
+                          "attention: documents must be int32 [", a.b, ", ", a.sk,
+                          "] on q's device");
+        TORCH_CHECK(documents.stride(1) == 1 || a.sk <= 1, "documents have gaps");
+        a.documents = documents.data_ptr<int>();
+        a.documents_sb = documents.stride(0);
     }
-    if (slopes) {
-        TORCH_CHECK(slopes->is_cuda() && slopes->device() == q.device() &&
-                        slopes->scalar_type() == torch::kFloat32 && slopes->dim() == 1 &&
-                        slopes->size(0) == a.hq && slopes->is_contiguous(),
-                    "slopes must be float32 [query heads]");
-        a.slopes = slopes->data_ptr<float>();
+    if (slopes.defined()) {
+        TORCH_CHECK_VALUE(slopes.device() == q.device() &&
+                              slopes.scalar_type() == torch::kFloat32 && slopes.dim() == 1 &&
+                              slopes.size(0) == a.hq,
+                          "attention: slopes must be float32 [", a.hq, "] on q's device");
+        TORCH_CHECK_VALUE(!slopes.requires_grad(),
+                          "attention: slopes are constants and get no gradient");
+        TORCH_CHECK(slopes.is_contiguous(), "slopes have gaps");
+        a.slopes = slopes.data_ptr<float>();
     }
     a.causal = causal;
     a.scale = (float)scale;
@@ -1504,15 +1513,15 @@ void for_type(torch::ScalarType type, F f) {
         case torch::kFloat32: f((float*)nullptr); break;
         case torch::kBFloat16: f((__bf16*)nullptr); break;
         case torch::kFloat16: f((_Float16*)nullptr); break;
-        default: TORCH_CHECK(false, "attention takes float32, bfloat16 or float16");
+        default:
+            TORCH_CHECK_VALUE(false, "attention: takes float32, bfloat16 or float16, got ", type);
     }
 }
 
-}  // namespace
-
+// out, the rows' sums if `want_lse`, and the ranges of documents if it made any
 std::vector<torch::Tensor> attention_forward(torch::Tensor q, torch::Tensor k, torch::Tensor v,
-                                             std::optional<torch::Tensor> documents,
-                                             std::optional<torch::Tensor> slopes, bool causal,
+                                             const torch::Tensor& documents,
+                                             const torch::Tensor& slopes, bool causal,
                                              double scale, bool want_lse) {
     Args a = args_for(q, k, v, documents, slopes, causal, scale);
     c10::DeviceGuard guard(q.device());
@@ -1545,9 +1554,9 @@ std::vector<torch::Tensor> attention_forward(torch::Tensor q, torch::Tensor k, t
 std::vector<torch::Tensor> attention_backward(torch::Tensor dout, torch::Tensor q,
                                               torch::Tensor k, torch::Tensor v, torch::Tensor out,
                                               torch::Tensor lse,
-                                              std::vector<torch::Tensor> known_ranges,
-                                              std::optional<torch::Tensor> documents,
-                                              std::optional<torch::Tensor> slopes, bool causal,
+                                              const std::vector<torch::Tensor>& known_ranges,
+                                              const torch::Tensor& documents,
+                                              const torch::Tensor& slopes, bool causal,
                                               double scale) {
     Args a = args_for(q, k, v, documents, slopes, causal, scale);
     c10::DeviceGuard guard(q.device());
@@ -1583,4 +1592,55 @@ std::vector<torch::Tensor> attention_backward(torch::Tensor dout, torch::Tensor 
         });
     });
     return {dq, dk, dv};
+}
+
+struct AttentionFunction : torch::autograd::Function<AttentionFunction> {
+    static torch::Tensor forward(torch::autograd::AutogradContext* ctx, const torch::Tensor& q,
+                                 const torch::Tensor& k, const torch::Tensor& v,
+                                 const std::optional<torch::Tensor>& documents,
+                                 const std::optional<torch::Tensor>& slopes, bool causal,
+                                 double scale) {
+        const torch::Tensor none, docs = documents.value_or(none), slope = slopes.value_or(none);
+        auto r = attention_forward(q, k, v, docs, slope, causal, scale, true);
+        torch::autograd::variable_list saved = {q, k, v, docs, slope};
+        saved.insert(saved.end(), r.begin(), r.end());
+        ctx->save_for_backward(saved);
+        ctx->saved_data["causal"] = causal;
+        ctx->saved_data["scale"] = scale;
+        return r[0];
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                   torch::autograd::variable_list grads) {
+        const auto x = ctx->get_saved_variables();
+        torch::autograd::variable_list d;
+        {
+            at::AutoGradMode no(false);
+            d = attention_backward(grads[0], x[0], x[1], x[2], x[5], x[6],
+                                   {x.begin() + 7, x.end()}, x[3], x[4],
+                                   ctx->saved_data["causal"].toBool(),
+                                   ctx->saved_data["scale"].toDouble());
+        }
+        d = once_differentiable(std::move(d), "attention");
+        d.resize(7);
+        return d;
+    }
+};
+
+}  // namespace
+
+torch::Tensor attention(torch::Tensor q, torch::Tensor k, torch::Tensor v,
+                        std::optional<torch::Tensor> documents,
+                        std::optional<torch::Tensor> slopes, bool causal,
+                        std::optional<double> scale) {
+    TORCH_CHECK_VALUE(q.dim() == 4, "attention: q must be [batch, length, heads, head size]");
+    if (documents && documents->dim() == 2 && documents->size(1) > 1 && documents->stride(1) != 1)
+        documents = documents->contiguous();
+    if (slopes) slopes = slopes->contiguous();
+    const double by = scale.value_or(1.0 / std::sqrt((double)q.size(3)));
+    if (at::GradMode::is_enabled() &&
+        (q.requires_grad() || k.requires_grad() || v.requires_grad()))
+        return AttentionFunction::apply(q, k, v, documents, slopes, causal, by);
+    const torch::Tensor none;
+    return attention_forward(q, k, v, documents.value_or(none), slopes.value_or(none), causal, by,
+                             false)[0];
 }

@@ -273,8 +273,8 @@ Kind kind_of(const torch::Tensor& t) {
         case torch::kBFloat16: return BF16;
         case torch::kFloat16: return F16;
         default:
-            TORCH_CHECK(false, "gradients must be float32, bfloat16 or float16, got ",
-                        t.scalar_type());
+            TORCH_CHECK_VALUE(false, "gradients must be float32, bfloat16 or float16, got ",
+                              t.scalar_type());
     }
 }
 
@@ -319,8 +319,8 @@ Plan plan_for(const std::vector<torch::Tensor>& ins, const std::vector<torch::Te
 
 void check_grads(const std::vector<torch::Tensor>& grads) {
     for (auto& t : grads) {
-        TORCH_CHECK(t.is_cuda(), "gradients must be GPU tensors");
-        TORCH_CHECK(t.device() == grads[0].device(), "gradients must be on one device");
+        TORCH_CHECK_VALUE(t.layout() == torch::kStrided, "gradients must be dense tensors");
+        TORCH_CHECK_VALUE(t.device() == grads[0].device(), "gradients must be on one device");
         kind_of(t);
     }
 }
@@ -336,8 +336,9 @@ torch::Tensor partial_sums(const Plan& p, const torch::Tensor& like, hipStream_t
 }  // namespace
 
 torch::Tensor grad_norm(std::vector<torch::Tensor> grads) {
-    TORCH_CHECK(!grads.empty(), "grad_norm needs a tensor");
+    TORCH_CHECK_VALUE(!grads.empty() && grads[0].is_cuda(), "grad_norm: needs GPU tensors");
     check_grads(grads);
+    at::NoGradGuard no_grad;
     c10::DeviceGuard guard(grads[0].device());
     for (auto& t : grads)
         if (!t.is_non_overlapping_and_dense()) t = t.contiguous();
@@ -350,15 +351,27 @@ torch::Tensor grad_norm(std::vector<torch::Tensor> grads) {
     return norm;
 }
 
-torch::Tensor clip_grad_norm(std::vector<torch::Tensor> grads, std::vector<torch::Tensor> outs,
-                             double max_norm) {
-    TORCH_CHECK(!grads.empty(), "clip_grad_norm needs a tensor");
-    TORCH_CHECK(outs.size() == grads.size(), "one output for each gradient");
-    TORCH_CHECK(max_norm >= 0, "max_norm must not be negative");
+std::pair<std::vector<torch::Tensor>, torch::Tensor> clip_grad_norm(
+    std::vector<torch::Tensor> grads, double max_norm,
+    std::optional<std::vector<torch::Tensor>> out, std::optional<torch::ScalarType> dtype) {
+    TORCH_CHECK_VALUE(!grads.empty() && grads[0].is_cuda(), "clip_grad_norm: needs GPU tensors");
+    TORCH_CHECK_VALUE(max_norm >= 0, "clip_grad_norm: max_norm must be 0 or more, got ", max_norm);
+    TORCH_CHECK_VALUE(!out || !dtype, "clip_grad_norm: dtype is for new tensors, without out");
     check_grads(grads);
-    check_grads(outs);
-    TORCH_CHECK(outs[0].device() == grads[0].device(), "outputs must be on the gradients' device");
+    at::NoGradGuard no_grad;
     c10::DeviceGuard guard(grads[0].device());
+    std::vector<torch::Tensor> outs;
+    if (out) {
+        outs = *out;
+    } else {
+        for (auto& t : grads)
+            outs.push_back(torch::empty_like(t, t.options().dtype(dtype.value_or(t.scalar_type()))));
+    }
+    const std::vector<torch::Tensor> results = outs;
+    TORCH_CHECK_VALUE(outs.size() == grads.size(), "clip_grad_norm: needs one output a gradient");
+    check_grads(outs);
+    TORCH_CHECK_VALUE(outs[0].device() == grads[0].device(),
+                      "clip_grad_norm: outputs must be on the gradients' device");
 
     // Blocks read and write without an order between them: what is written
     // may be read only as the same values' own input.
@@ -379,13 +392,14 @@ torch::Tensor clip_grad_norm(std::vector<torch::Tensor> grads, std::vector<torch
         return a.is_non_overlapping_and_dense() && same_strides(a, b);
     };
     for (size_t i = 0; i < outs.size(); ++i) {
-        TORCH_CHECK(outs[i].sizes() == grads[i].sizes(), "output ", i, " has another shape");
+        TORCH_CHECK_VALUE(outs[i].sizes() == grads[i].sizes(), "clip_grad_norm: output ", i,
+                          " has another shape");
         if (outs[i].numel()) ranges.push_back(range(outs[i], i));
     }
     std::sort(ranges.begin(), ranges.end(),
               [](const Range& a, const Range& b) { return a.at < b.at; });
     for (size_t i = 1; i < ranges.size(); ++i)
-        TORCH_CHECK(ranges[i].at >= ranges[i - 1].end, "outputs ", ranges[i - 1].i, " and ",
+        TORCH_CHECK_VALUE(ranges[i].at >= ranges[i - 1].end, "clip_grad_norm: outputs ", ranges[i - 1].i, " and ",
                     ranges[i].i, " share memory");
     for (size_t i = 0; i < grads.size(); ++i) {
         if (!grads[i].numel()) continue;
@@ -393,10 +407,10 @@ torch::Tensor clip_grad_norm(std::vector<torch::Tensor> grads, std::vector<torch
         auto it = std::upper_bound(ranges.begin(), ranges.end(), r.at,
                                    [](const char* a, const Range& b) { return a < b.end; });
         if (it == ranges.end() || it->at >= r.end) continue;
-        TORCH_CHECK(it->i == i && it->at == r.at && it->end == r.end &&
+        TORCH_CHECK_VALUE(it->i == i && it->at == r.at && it->end == r.end &&
                         outs[i].scalar_type() == grads[i].scalar_type() &&
                         same_strides(outs[i], grads[i]),
-                    "gradient ", i, " shares memory with output ", it->i);
+                    "clip_grad_norm: gradient ", i, " shares memory with output ", it->i);
     }
 
     // other orders than dense ones go through copies
@@ -423,5 +437,7 @@ torch::Tensor clip_grad_norm(std::vector<torch::Tensor> grads, std::vector<torch
                            p.chunk, partial.data_ptr<double>(), p.partials, max_norm,
                            norm.data_ptr<float>());
     for (auto& c : copies) c.second.copy_(outs[c.first]);
-    return norm;
+    if (out)
+        for (auto& t : results) t.unsafeGetTensorImpl()->bump_version();
+    return {results, norm};
 }

@@ -3246,11 +3246,16 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("pack_ints_cpu", &pack_ints_cpu, "n-bit pack (C++ CPU)");
     m.def("unpack_ints_cpu", &unpack_ints_cpu, "n-bit unpack (C++ CPU)");
     m.def("huffman_decode_cpu", &huffman_decode_cpu, "canonical Huffman decode (C++ CPU)");
+    namespace py = pybind11;
     m.def("grad_norm", &grad_norm, "global 2-norm of many tensors (HIP)");
     m.def("clip_grad_norm", &clip_grad_norm,
-          "global 2-norm of many tensors, and the tensors scaled to at most max_norm (HIP)");
-    m.def("rotary", &rotary, "rotary positions of one or two tensors (HIP)");
-    m.def("attention_forward", &attention_forward,
-          "attention with documents, distance bias and causality -> (out, lse, document ranges if it made any) (HIP)");
-    m.def("attention_backward", &attention_backward, "its gradient -> (dq, dk, dv) (HIP)");
+          "(tensors scaled to a global 2-norm of at most max_norm, that norm) (HIP)",
+          py::arg("grads"), py::arg("max_norm"), py::arg("out") = py::none(),
+          py::arg("dtype") = py::none());
+    m.def("rotary", &rotary, "rotary positions of queries and keys (HIP)");
+    m.def("attention", &attention,
+          "attention with documents, distance bias and causality (HIP)", py::arg("q"),
+          py::arg("k"), py::arg("v"), py::arg("documents") = py::none(),
+          py::arg("slopes") = py::none(), py::arg("causal") = false,
+          py::arg("scale") = py::none());
 }

@@ -147,33 +147,21 @@ void launch_vec(const Args& a, int v, bool interleaved, int blocks, hipStream_t 
     }
 }
 
-}  // namespace
-
-std::vector<torch::Tensor> rotary(std::vector<torch::Tensor> xs, torch::Tensor positions,
-                                  torch::Tensor frequencies, bool interleaved, bool inverse) {
-    TORCH_CHECK(xs.size() >= 1 && xs.size() <= 2, "rotary takes one or two tensors");
-    const auto& x0 = xs[0];
+// xs [batch, length, heads, d], turned
+torch::autograd::variable_list rotate(torch::autograd::variable_list xs,
+                                      const torch::Tensor& positions,
+                                      const torch::Tensor& frequencies, bool interleaved,
+                                      bool inverse) {
+    const torch::Tensor x0 = xs[0];
     c10::DeviceGuard guard(x0.device());
     Args a{};
-    a.d = (int)x0.size(-1);
+    a.d = (int)x0.size(3);
     a.half = (int)frequencies.numel();
     a.length = (int)x0.size(1);
     a.tokens = x0.size(0) * x0.size(1);
-    TORCH_CHECK(frequencies.is_cuda() && frequencies.scalar_type() == torch::kFloat64 &&
-                    frequencies.dim() == 1 && frequencies.is_contiguous() &&
-                    frequencies.device() == x0.device(),
-                "frequencies must be a contiguous float64 vector on the tensors' device");
-    TORCH_CHECK(a.half >= 1 && 2 * a.half <= a.d && a.half <= MOST_PAIRS,
-                "frequencies turn more values than a head has");
-    TORCH_CHECK(positions.is_cuda() && positions.device() == x0.device() &&
-                    (positions.scalar_type() == torch::kInt64 ||
-                     positions.scalar_type() == torch::kInt32) &&
-                    positions.dim() == 2 && positions.size(0) == x0.size(0) &&
-                    positions.size(1) == x0.size(1),
-                "positions must be int32 or int64 [batch, length] on the tensors' device");
     a.positions = positions.data_ptr();
-    a.pb = positions.stride(0);
-    a.ps = positions.stride(1);
+    a.pb = positions.dim() == 2 ? positions.stride(0) : 0;
+    a.ps = positions.stride(-1);
     a.wide = positions.scalar_type() == torch::kInt64;
     a.frequencies = frequencies.data_ptr<double>();
     a.sign = inverse ? -1.f : 1.f;
@@ -182,15 +170,11 @@ std::vector<torch::Tensor> rotary(std::vector<torch::Tensor> xs, torch::Tensor p
     // the widest vector that every address and extent is a multiple of
     int size = (int)x0.element_size();
     int v = 16 / size;
-    std::vector<torch::Tensor> outs;
+    torch::autograd::variable_list outs;
     int heads = 0;
     for (size_t t = 0; t < xs.size(); ++t) {
         auto& x = xs[t];
-        TORCH_CHECK(x.is_cuda() && x.dim() == 4 && x.device() == x0.device() &&
-                        x.scalar_type() == x0.scalar_type() && x.size(0) == x0.size(0) &&
-                        x.size(1) == x0.size(1) && x.size(3) == a.d,
-                    "rotary takes [batch, length, heads, d] tensors of one type");
-        if (x.stride(3) != 1 && a.d > 1) x = x.contiguous();
+        if (x.stride(3) != 1) x = x.contiguous();
         outs.push_back(torch::empty(x.sizes(), x.options()));
         a.x[t] = {x.data_ptr(), outs[t].data_ptr(), x.stride(0), x.stride(1), x.stride(2),
                   (int)x.size(2)};
@@ -201,16 +185,14 @@ std::vector<torch::Tensor> rotary(std::vector<torch::Tensor> xs, torch::Tensor p
     }
     while (v > 1 && (a.d % v || (interleaved ? 2 * a.half : a.half) % v)) v /= 2;
     if (interleaved && v == 1) {
-        // pairs at odd addresses: a copy is aligned, and 2 divides its extents
-        // but for an odd head size
+        // pairs at odd addresses: a copy's are even
         for (size_t t = 0; t < xs.size(); ++t) {
-            xs[t] = xs[t].contiguous();
+            xs[t] = xs[t].clone(at::MemoryFormat::Contiguous);
             a.x[t].in = xs[t].data_ptr();
             a.x[t].sb = xs[t].stride(0);
             a.x[t].ss = xs[t].stride(1);
             a.x[t].sh = xs[t].stride(2);
         }
-        TORCH_CHECK(a.d % 2 == 0, "interleaved pairs need an even head size");
         v = 2;
     }
     if (a.tokens == 0 || heads == 0) return outs;
@@ -220,15 +202,79 @@ std::vector<torch::Tensor> rotary(std::vector<torch::Tensor> xs, torch::Tensor p
     int64_t per = std::max<int64_t>(1, a.tokens / 2048);
     a.per_block = (int)std::min<int64_t>({per, (int64_t)8, (int64_t)(MOST_PAIRS / a.half)});
     int64_t blocks = (a.tokens + a.per_block - 1) / a.per_block;
-    TORCH_CHECK(blocks <= INT_MAX, "too many tokens for one launch");
+    TORCH_CHECK_VALUE(blocks <= INT_MAX, "rotary: too many tokens for one launch");
     hipStream_t stream = at::hip::getCurrentHIPStream();
     switch (x0.scalar_type()) {
         case torch::kFloat32: launch_vec<float>(a, v, interleaved, (int)blocks, stream); break;
         case torch::kBFloat16: launch_vec<__bf16>(a, v, interleaved, (int)blocks, stream); break;
-        case torch::kFloat16:
-            launch_vec<_Float16>(a, v, interleaved, (int)blocks, stream);
-            break;
-        default: TORCH_CHECK(false, "rotary takes float32, bfloat16 or float16");
+        default: launch_vec<_Float16>(a, v, interleaved, (int)blocks, stream); break;
     }
     return outs;
+}
+
+struct RotaryFunction : torch::autograd::Function<RotaryFunction> {
+    static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx,
+                                                  const torch::Tensor& q, const torch::Tensor& k,
+                                                  const torch::Tensor& positions,
+                                                  const torch::Tensor& frequencies,
+                                                  bool interleaved) {
+        ctx->save_for_backward({positions, frequencies});
+        ctx->saved_data["interleaved"] = interleaved;
+        return rotate({q, k}, positions, frequencies, interleaved, false);
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                   torch::autograd::variable_list grads) {
+        const auto x = ctx->get_saved_variables();
+        torch::autograd::variable_list need, d(5);
+        for (int n = 0; n < 2; ++n)
+            if (ctx->needs_input_grad(n)) need.push_back(grads[n]);
+        {
+            at::AutoGradMode no(false);
+            need = rotate(std::move(need), x[0], x[1], ctx->saved_data["interleaved"].toBool(),
+                          true);
+        }
+        need = once_differentiable(std::move(need), "rotary");
+        for (int n = 0, at = 0; n < 2; ++n)
+            if (ctx->needs_input_grad(n)) d[n] = need[at++];
+        return d;
+    }
+};
+
+}  // namespace
+
+std::vector<torch::Tensor> rotary(torch::Tensor q, torch::Tensor k, torch::Tensor positions,
+                                  torch::Tensor frequencies, bool interleaved) {
+    for (auto* x : {&q, &k})
+        TORCH_CHECK_VALUE(x->is_cuda() && x->dim() == 4 && x->device() == q.device() &&
+                              x->scalar_type() == q.scalar_type() && x->size(0) == q.size(0) &&
+                              x->size(1) == q.size(1) && x->size(3) == q.size(3),
+                          "rotary: q ", q.sizes(), " and k ", k.sizes(),
+                          " must be [batch, length, heads, head size] with one batch, length and "
+                          "head size, of one type on one device");
+    const auto type = q.scalar_type();
+    TORCH_CHECK_VALUE(type == torch::kFloat32 || type == torch::kBFloat16 ||
+                          type == torch::kFloat16,
+                      "rotary: takes float32, bfloat16 or float16, got ", type);
+    const int64_t b = q.size(0), s = q.size(1), d = q.size(3);
+    TORCH_CHECK_VALUE(d % 2 == 0 && d <= 1024,
+                      "rotary: the head size must be even and at most 1024, got ", d);
+    TORCH_CHECK_VALUE(positions.device() == q.device() &&
+                          (positions.scalar_type() == torch::kInt64 ||
+                           positions.scalar_type() == torch::kInt32) &&
+                          (positions.sizes() == at::IntArrayRef({s}) ||
+                           positions.sizes() == at::IntArrayRef({b, s})),
+                      "rotary: positions must be int32 or int64, [", s, "] or [", b, ", ", s,
+                      "], on q's device");
+    TORCH_CHECK_VALUE(frequencies.device() == q.device() &&
+                          frequencies.scalar_type() == torch::kFloat64 &&
+                          frequencies.dim() == 1 && frequencies.numel() >= 1 &&
+                          frequencies.numel() <= d / 2,
+                      "rotary: frequencies must be float64 with 1 to ", d / 2,
+                      " values on q's device");
+    TORCH_CHECK_VALUE(!frequencies.requires_grad(),
+                      "rotary: frequencies are constants and get no gradient");
+    frequencies = frequencies.contiguous();
+    if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad()))
+        return RotaryFunction::apply(q, k, positions, frequencies, interleaved);
+    return rotate({q, k}, positions, frequencies, interleaved, false);
 }

@@ -357,6 +357,22 @@ def test_attention_refuses(device):
             ops.attention(**{**dict(q=q, k=k, v=v), **change})
 
 
+@pytest.mark.parametrize("device", BOTH)
+def test_differentiable_once(device):
+    q, k, v, dout = attention_inputs(1, 9, 9, 2, 1, 16, torch.float32, device)
+    positions = torch.arange(9, device=device)
+    frequencies = ops.rotary_frequencies(16, device=device)
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    x, y = ops.rotary(q, k, positions, frequencies)
+    out = ops.attention(x, y, v, causal=True)
+    plain = torch.autograd.grad(out, leaves, dout, retain_graph=True)
+    again = torch.autograd.grad(out, leaves, dout, create_graph=True)
+    for a, c in zip(plain, again):
+        assert torch.equal(a, c)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(again[0].sum(), q)
+
+
 @pytest.mark.gpu
 def test_attention_repeats_and_replays():
     """Two eager calls, calls on another stream and every replay of a captured
