@@ -25,26 +25,35 @@
 
 namespace {
 
-constexpr int TABLE = 128;    // 29 bytes each: the arguments stay under 4 KB
+constexpr int TABLE = 165;    // 24 bytes each, and the arguments stay under 4 KB
 constexpr int THREADS = 256;
 constexpr int WAVES = THREADS / 64;
 constexpr int UNROLL = 4;     // 16-byte loads in flight for each thread
+constexpr int BLOCKS = 4096;
 
 enum Kind : uint8_t { F32 = 0, BF16 = 1, F16 = 2 };
 
 struct Table {
-    const void* in[TABLE];
-    void* out[TABLE];
-    int64_t n[TABLE];
+    uint64_t in[TABLE];       // address | type << 56
+    uint64_t out[TABLE];
     int first[TABLE];         // first chunk of each tensor, INT_MAX behind the last
-    uint8_t kind[TABLE];      // input type | output type << 4
+    int tail[TABLE];          // values of its last chunk
+    int blocks;               // chunks of all
     int chunks_before;        // partial sums of earlier launches
+    int chunk;                // values of a chunk
 };
-static_assert(sizeof(Table) + 64 <= 4096, "kernel arguments are limited to 4 KB");
+static_assert(sizeof(Table) + 48 <= 4096, "kernel arguments are limited to 4 KB");
 
 // 16 bytes at any element's address: buckets put tensors at odd offsets
 typedef uint32_t raw4 __attribute__((ext_vector_type(4)));
 struct __attribute__((packed, aligned(2))) Raw { raw4 v; };
+
+// results are not read again soon: they pass the caches that still hold the
+// gradients
+__device__ __forceinline__ void store(Raw* at, raw4 v) {
+    typedef raw4 loose __attribute__((aligned(2)));
+    __builtin_nontemporal_store(v, (loose*)at);
+}
 
 template <int KIND> struct Type;
 template <> struct Type<F32> {
@@ -83,12 +92,32 @@ __device__ __forceinline__ uint16_t to_bf16(float x) {
     return r;
 }
 
-// The block's tensor: each lane compares two starts, one memory latency for
-// all of them where a binary search would take seven.
-__device__ __forceinline__ int tensor_of(const Table& t, int block) {
-    int lane = threadIdx.x & 63;
-    uint64_t a = __ballot(t.first[lane] <= block), b = __ballot(t.first[lane + 64] <= block);
-    return __popcll(a) + __popcll(b) - 1;
+__device__ __forceinline__ int kind_size(int kind) { return kind == F32 ? 4 : 2; }
+
+// What a block works on.  Each lane compares three starts: one memory latency
+// for all where a binary search would take eight.
+struct Chunk {
+    const char* in;
+    char* out;
+    int n, from, to;
+};
+__device__ __forceinline__ Chunk chunk_of(const Table& t, int block) {
+    const int lane = threadIdx.x & 63;
+    int i = -1;
+#pragma unroll
+    for (int n = 0; n < TABLE; n += 64)
+        i += __popcll(__ballot(n + lane < TABLE && t.first[min(n + lane, TABLE - 1)] <= block));
+    i = __builtin_amdgcn_readfirstlane(i);
+    const int end = i + 1 < TABLE ? min(t.first[i + 1], t.blocks) : t.blocks;
+    const uint64_t mask = (1ull << 56) - 1;
+    Chunk c;
+    c.from = (int)(t.in[i] >> 56);
+    c.to = (int)(t.out[i] >> 56);
+    const int64_t start = (int64_t)(block - t.first[i]) * t.chunk;
+    c.in = (const char*)(t.in[i] & mask) + start * kind_size(c.from);
+    c.out = (char*)(t.out[i] & mask) + start * kind_size(c.to);
+    c.n = block + 1 == end ? t.tail[i] : t.chunk;
+    return c;
 }
 
 __device__ __forceinline__ double block_sum(double x, double* shared) {
@@ -101,17 +130,30 @@ __device__ __forceinline__ double block_sum(double x, double* shared) {
     return x;
 }
 
+// values before the first 16-byte address
+__device__ __forceinline__ int head_of(const void* at, int size, int n) {
+    return min(n, (int)((16 - ((uintptr_t)at & 15)) & 15) / size);
+}
+
 template <int KIND>
-__device__ double chunk_sum(const void* in, int64_t n) {
+__device__ double chunk_sum(const void* in, int n) {
     using T = Type<KIND>;
-    const Raw* raw = (const Raw*)in;
-    int64_t vecs = n / T::PER;
+    constexpr int SIZE = KIND == F32 ? 4 : 2;
     double s = 0;
-    int64_t i = threadIdx.x;
+    const int head = head_of(in, SIZE, n);
+    if ((int)threadIdx.x < head) {
+        double x = T::load(in, threadIdx.x);
+        s = x * x;
+    }
+    in = (const char*)in + head * SIZE;
+    n -= head;
+    const raw4* raw = (const raw4*)in;
+    const int vecs = n / T::PER;
+    int i = threadIdx.x;
     for (; i + (UNROLL - 1) * THREADS < vecs; i += UNROLL * THREADS) {
         raw4 r[UNROLL];
 #pragma unroll
-        for (int u = 0; u < UNROLL; ++u) r[u] = raw[i + u * THREADS].v;
+        for (int u = 0; u < UNROLL; ++u) r[u] = raw[i + u * THREADS];
 #pragma unroll
         for (int u = 0; u < UNROLL; ++u)
 #pragma unroll
@@ -121,7 +163,7 @@ __device__ double chunk_sum(const void* in, int64_t n) {
             }
     }
     for (; i < vecs; i += THREADS) {
-        raw4 r = raw[i].v;
+        raw4 r = raw[i];
 #pragma unroll
         for (int e = 0; e < T::PER; ++e) {
             double x = T::get((const uint32_t*)&r, e);
@@ -135,21 +177,14 @@ __device__ double chunk_sum(const void* in, int64_t n) {
     return s;
 }
 
-__device__ __forceinline__ int kind_size(int kind) { return kind == F32 ? 4 : 2; }
-
-__global__ __launch_bounds__(THREADS) void norm_partial_kernel(const Table t, int64_t chunk,
+__global__ __launch_bounds__(THREADS) void norm_partial_kernel(const Table t,
                                                                double* __restrict__ partial) {
     __shared__ double shared[WAVES];
-    int block = blockIdx.x;
-    int i = __builtin_amdgcn_readfirstlane(tensor_of(t, block));
-    int64_t start = (int64_t)(block - t.first[i]) * chunk;
-    int64_t n = min(chunk, t.n[i] - start);
-    int kind = t.kind[i] & 15;
-    const char* in = (const char*)t.in[i] + start * kind_size(kind);
-    double s = kind == F32 ? chunk_sum<F32>(in, n)
-             : kind == BF16 ? chunk_sum<BF16>(in, n) : chunk_sum<F16>(in, n);
+    const Chunk c = chunk_of(t, blockIdx.x);
+    double s = c.from == F32 ? chunk_sum<F32>(c.in, c.n)
+             : c.from == BF16 ? chunk_sum<BF16>(c.in, c.n) : chunk_sum<F16>(c.in, c.n);
     s = block_sum(s, shared);
-    if (threadIdx.x == 0) partial[t.chunks_before + block] = s;
+    if (threadIdx.x == 0) partial[t.chunks_before + blockIdx.x] = s;
 }
 
 __global__ __launch_bounds__(1024) void norm_join_kernel(const double* __restrict__ partial,
@@ -187,7 +222,7 @@ __device__ __forceinline__ void put_vec(Raw* out, int64_t i, double factor, raw4
             for (int e = 0; e < 4; ++e)
                 o[e] = __float_as_uint(
                     (float)((double)Type<IN>::get((const uint32_t*)&r, h * 4 + e) * factor));
-            out[i * (PER / 4) + h].v = o;
+            store(out + i * (PER / 4) + h, o);
         }
     } else {
         uint32_t w[PER / 2];
@@ -208,7 +243,7 @@ __device__ __forceinline__ void put_vec(Raw* out, int64_t i, double factor, raw4
         }
         if constexpr (PER == 8) {
             raw4 o = {w[0], w[1], w[2], w[3]};
-            out[i].v = o;
+            store(out + i, o);
         } else {
             struct __attribute__((packed, aligned(2))) Two { uint32_t a, b; };
             ((Two*)out)[i] = Two{w[0], w[1]};
@@ -217,11 +252,17 @@ __device__ __forceinline__ void put_vec(Raw* out, int64_t i, double factor, raw4
 }
 
 template <int IN, int OUT>
-__device__ void chunk_scale(const void* in, void* out, int64_t n, double factor) {
-    constexpr int PER = Type<IN>::PER;
+__device__ void chunk_scale(const void* in, void* out, int n, double factor) {
+    constexpr int PER = Type<IN>::PER, SIZE = IN == F32 ? 4 : 2, TO = OUT == F32 ? 4 : 2;
+    const int head = head_of(out, TO, n);  // stores at 16-byte addresses, loads at any
+    if ((int)threadIdx.x < head)
+        put<OUT>(out, threadIdx.x, factor, Type<IN>::load(in, threadIdx.x));
+    in = (const char*)in + head * SIZE;
+    out = (char*)out + head * TO;
+    n -= head;
     const Raw* raw = (const Raw*)in;
-    int64_t vecs = n / PER;
-    int64_t i = threadIdx.x;
+    const int vecs = n / PER;
+    int i = threadIdx.x;
     for (; i + (UNROLL - 1) * THREADS < vecs; i += UNROLL * THREADS) {
         raw4 r[UNROLL];
 #pragma unroll
@@ -234,36 +275,29 @@ __device__ void chunk_scale(const void* in, void* out, int64_t n, double factor)
         put<OUT>(out, i, factor, Type<IN>::load(in, i));
 }
 
-__global__ __launch_bounds__(THREADS) void clip_kernel(const Table t, int64_t chunk,
+__global__ __launch_bounds__(THREADS) void clip_kernel(const Table t,
                                                        const double* __restrict__ partial, int n,
                                                        double max_norm,
                                                        float* __restrict__ norm) {
     __shared__ double shared[WAVES];
+    const Chunk c = chunk_of(t, t.blocks - 1 - blockIdx.x);
     double s = 0;
     for (int i = threadIdx.x; i < n; i += THREADS) s += partial[i];
     double total = sqrt(block_sum(s, shared));
     if (blockIdx.x == 0 && t.chunks_before == 0 && threadIdx.x == 0) *norm = (float)total;
     // a NaN norm is no norm below the bound: it reaches every value
     double factor = total <= max_norm ? 1.0 : max_norm / total;
-
-    int block = gridDim.x - 1 - blockIdx.x;
-    int i = __builtin_amdgcn_readfirstlane(tensor_of(t, block));
-    int64_t start = (int64_t)(block - t.first[i]) * chunk;
-    int64_t len = min(chunk, t.n[i] - start);
-    int from = t.kind[i] & 15, to = t.kind[i] >> 4;
-    const char* in = (const char*)t.in[i] + start * kind_size(from);
-    char* out = (char*)t.out[i] + start * kind_size(to);
-    if (in == out && factor == 1.0) return;  // in place and under the bound
-    switch (from * 3 + to) {
-        case 0: chunk_scale<F32, F32>(in, out, len, factor); break;
-        case 1: chunk_scale<F32, BF16>(in, out, len, factor); break;
-        case 2: chunk_scale<F32, F16>(in, out, len, factor); break;
-        case 3: chunk_scale<BF16, F32>(in, out, len, factor); break;
-        case 4: chunk_scale<BF16, BF16>(in, out, len, factor); break;
-        case 5: chunk_scale<BF16, F16>(in, out, len, factor); break;
-        case 6: chunk_scale<F16, F32>(in, out, len, factor); break;
-        case 7: chunk_scale<F16, BF16>(in, out, len, factor); break;
-        default: chunk_scale<F16, F16>(in, out, len, factor); break;
+    if (c.in == c.out && factor == 1.0) return;  // in place and under the bound
+    switch (c.from * 3 + c.to) {
+        case 0: chunk_scale<F32, F32>(c.in, c.out, c.n, factor); break;
+        case 1: chunk_scale<F32, BF16>(c.in, c.out, c.n, factor); break;
+        case 2: chunk_scale<F32, F16>(c.in, c.out, c.n, factor); break;
+        case 3: chunk_scale<BF16, F32>(c.in, c.out, c.n, factor); break;
+        case 4: chunk_scale<BF16, BF16>(c.in, c.out, c.n, factor); break;
+        case 5: chunk_scale<BF16, F16>(c.in, c.out, c.n, factor); break;
+        case 6: chunk_scale<F16, F32>(c.in, c.out, c.n, factor); break;
+        case 7: chunk_scale<F16, BF16>(c.in, c.out, c.n, factor); break;
+        default: chunk_scale<F16, F16>(c.in, c.out, c.n, factor); break;
     }
 }
 
@@ -280,39 +314,40 @@ Kind kind_of(const torch::Tensor& t) {
 
 struct Plan {
     std::vector<Table> tables;
-    std::vector<int> blocks;
-    int64_t chunk = 0;
     int partials = 0;
 };
 
 // Chunks of a power of two, from 4096 values (a block's four loads of 16
-// bytes a thread) up so that 2048 blocks, 8 on each of the 256 CUs, hold all.
+// bytes a thread) up so that 4096 blocks, two rounds of the 8 that each of the
+// 256 CUs holds, take all.
 Plan plan_for(const std::vector<torch::Tensor>& ins, const std::vector<torch::Tensor>* outs) {
     Plan p;
-    int64_t total = 0;
+    int64_t total = 0, chunk = 4096;
     for (auto& t : ins) total += t.numel();
-    p.chunk = 4096;
-    while (p.chunk * 2048 < total) p.chunk *= 2;
+    while (chunk * BLOCKS < total) chunk *= 2;
+    TORCH_CHECK_VALUE(chunk < INT_MAX, "too many values");
     int used = TABLE;
     for (size_t i = 0; i < ins.size(); ++i) {
         int64_t n = ins[i].numel();
         if (n == 0) continue;
         if (used == TABLE) {
             p.tables.emplace_back();
-            p.blocks.push_back(0);
-            std::fill_n(p.tables.back().first, TABLE, INT_MAX);
-            p.tables.back().chunks_before = p.partials;
+            Table& t = p.tables.back();
+            std::fill_n(t.first, TABLE, INT_MAX);
+            t.blocks = 0;
+            t.chunks_before = p.partials;
+            t.chunk = (int)chunk;
             used = 0;
         }
         Table& t = p.tables.back();
-        t.in[used] = ins[i].data_ptr();
-        t.out[used] = outs ? (*outs)[i].data_ptr() : nullptr;
-        t.n[used] = n;
-        t.kind[used] = kind_of(ins[i]) | (outs ? kind_of((*outs)[i]) << 4 : 0);
-        t.first[used++] = p.blocks.back();
-        int64_t chunks = (n + p.chunk - 1) / p.chunk;
-        p.blocks.back() += (int)chunks;
-        p.partials += (int)chunks;
+        t.in[used] = (uint64_t)ins[i].data_ptr() | (uint64_t)kind_of(ins[i]) << 56;
+        t.out[used] = outs ? (uint64_t)(*outs)[i].data_ptr() | (uint64_t)kind_of((*outs)[i]) << 56
+                           : 0;
+        t.first[used] = t.blocks;
+        const int chunks = (int)((n + chunk - 1) / chunk);
+        t.tail[used++] = (int)(n - (chunks - 1) * chunk);
+        t.blocks += chunks;
+        p.partials += chunks;
     }
     return p;
 }
@@ -327,9 +362,9 @@ void check_grads(const std::vector<torch::Tensor>& grads) {
 
 torch::Tensor partial_sums(const Plan& p, const torch::Tensor& like, hipStream_t stream) {
     auto partial = torch::empty({std::max(1, p.partials)}, like.options().dtype(torch::kFloat64));
-    for (size_t i = 0; i < p.tables.size(); ++i)
-        hipLaunchKernelGGL(norm_partial_kernel, dim3(p.blocks[i]), dim3(THREADS), 0, stream,
-                           p.tables[i], p.chunk, partial.data_ptr<double>());
+    for (auto& t : p.tables)
+        hipLaunchKernelGGL(norm_partial_kernel, dim3(t.blocks), dim3(THREADS), 0, stream, t,
+                           partial.data_ptr<double>());
     return partial;
 }
 
@@ -433,8 +468,8 @@ std::pair<std::vector<torch::Tensor>, torch::Tensor> clip_grad_norm(
     // last launch and last block first: what the sums read last is still in
     // the last-level cache
     for (size_t i = p.tables.size(); i-- > 0;)
-        hipLaunchKernelGGL(clip_kernel, dim3(p.blocks[i]), dim3(THREADS), 0, stream, p.tables[i],
-                           p.chunk, partial.data_ptr<double>(), p.partials, max_norm,
+        hipLaunchKernelGGL(clip_kernel, dim3(p.tables[i].blocks), dim3(THREADS), 0, stream,
+                           p.tables[i], partial.data_ptr<double>(), p.partials, max_norm,
                            norm.data_ptr<float>());
     for (auto& c : copies) c.second.copy_(outs[c.first]);
     if (out)

@@ -23,6 +23,8 @@ namespace {
 
 constexpr int THREADS = 256;
 constexpr int MOST_PAIRS = 2048;  // (cos, sin) of a block: 16 KB
+constexpr int MOST_TOKENS = 8;
+constexpr int AHEAD = 4;          // work items that a thread has under way
 
 struct Heads {
     const void* in;
@@ -49,23 +51,77 @@ struct Args {
     float sign;             // -1: the turn back
 };
 
+// One work item: V pairs (two vectors, or one with V / 2 pairs), or one vector
+// behind them.
+template <typename T, int V, bool INTERLEAVED> struct Item {
+    Aligned<T, V> v, u;
+    const T* in;
+    T* out;
+    const float2* w;
+    bool turns;
+
+    __device__ __forceinline__ void load(const T* from, T* to, const float2* turn, int half,
+                                         int slot, int turned) {
+        turns = slot < turned;
+        const int at = turns ? slot * V : 2 * half + (slot - turned) * V;
+        in = from + at;
+        out = to + at;
+        w = turn + (INTERLEAVED ? slot * (V / 2) : slot * V);
+        v = *(const Aligned<T, V>*)in;
+        if (!INTERLEAVED && turns) u = *(const Aligned<T, V>*)(in + half);
+    }
+    __device__ __forceinline__ void store(int half) {
+        if (turns) {
+            Aligned<T, V> o, r;
+            if constexpr (INTERLEAVED) {
+#pragma unroll
+                for (int e = 0; e < V / 2; ++e) {
+                    const float2 c = w[e];
+                    const float p = (float)v.v[2 * e], q = (float)v.v[2 * e + 1];
+                    o.v[2 * e] = (T)(p * c.x - q * c.y);
+                    o.v[2 * e + 1] = (T)(p * c.y + q * c.x);
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                    const float2 c = w[e];
+                    const float p = (float)v.v[e], q = (float)u.v[e];
+                    o.v[e] = (T)(p * c.x - q * c.y);
+                    r.v[e] = (T)(p * c.y + q * c.x);
+                }
+                *(Aligned<T, V>*)(out + half) = r;
+            }
+            *(Aligned<T, V>*)out = o;
+        } else {
+            *(Aligned<T, V>*)out = v;
+        }
+    }
+};
+
 template <typename T, int V, bool INTERLEAVED>
 __global__ __launch_bounds__(THREADS) void rotary_kernel(const Args a) {
     __shared__ float2 turn[MOST_PAIRS];
-    int64_t first = (int64_t)blockIdx.x * a.per_block;
-    int tokens = (int)min((int64_t)a.per_block, a.tokens - first);
+    __shared__ double position[MOST_TOKENS];
+    __shared__ int64_t from[2][MOST_TOKENS];  // the tokens' rows in the inputs
+    const int64_t first = (int64_t)blockIdx.x * a.per_block;
+    const int tokens = (int)min((int64_t)a.per_block, a.tokens - first);
+    if ((int)threadIdx.x < tokens) {
+        const int64_t token = first + threadIdx.x, b = token / a.length, s = token - b * a.length;
+        const int64_t at = b * a.pb + s * a.ps;
+        position[threadIdx.x] = a.wide ? (double)((const int64_t*)a.positions)[at]
+                                       : (double)((const int*)a.positions)[at];
+        for (int t = 0; t < a.tensors; ++t) from[t][threadIdx.x] = b * a.x[t].sb + s * a.x[t].ss;
+    }
+    __syncthreads();
     for (int i = threadIdx.x; i < tokens * a.half; i += THREADS) {
-        int64_t token = first + i / a.half;
-        int64_t b = token / a.length, s = token % a.length;
-        int64_t at = b * a.pb + s * a.ps;
-        double position = a.wide ? (double)((const int64_t*)a.positions)[at]
-                                 : (double)((const int*)a.positions)[at];
         // quarters of a turn: what is left lies within an eighth of one
-        double quarters = position * a.frequencies[i % a.half] * 0.63661977236758134308;
-        double n = rint(quarters);
+        const int tok = i / a.half;
+        const double quarters = position[tok] * a.frequencies[i - tok * a.half] *
+                                0.63661977236758134308;
+        const double n = rint(quarters);
         float sn, cs;
         sincospif((float)(quarters - n) * 0.5f, &sn, &cs);
-        int q = (int)(n - 4.0 * floor(n * 0.25));
+        const int q = (int)(n - 4.0 * floor(n * 0.25));
         if (q & 1) {
             float t = cs;
             cs = -sn;
@@ -76,48 +132,27 @@ __global__ __launch_bounds__(THREADS) void rotary_kernel(const Args a) {
     }
     __syncthreads();
 
-    using A = Aligned<T, V>;
-    // a work item turns V pairs (two vectors, or one with V / 2 pairs) or
-    // copies one vector behind them
     const int turned = INTERLEAVED ? 2 * a.half / V : a.half / V;
     const int per_head = turned + (a.d - 2 * a.half) / V;
     for (int t = 0; t < a.tensors; ++t) {
         const Heads& x = a.x[t];
-        const unsigned per_token = (unsigned)x.heads * per_head;
-        for (unsigned i = threadIdx.x; i < tokens * per_token; i += THREADS) {
-            unsigned tok = i / per_token, rest = i % per_token;
-            unsigned head = rest / per_head, slot = rest % per_head;
-            int64_t token = first + tok;
-            int64_t b = token / a.length, s = token % a.length;
-            const T* in = (const T*)x.in + b * x.sb + s * x.ss + head * x.sh;
-            T* out = (T*)x.out + (token * x.heads + head) * a.d;
-            if (slot >= (unsigned)turned) {
-                int at = 2 * a.half + (slot - turned) * V;
-                *(A*)(out + at) = *(const A*)(in + at);
-                continue;
+        const unsigned per_token = (unsigned)x.heads * per_head, all = tokens * per_token;
+        T* to = (T*)x.out + first * x.heads * a.d;
+        for (unsigned i0 = threadIdx.x; i0 < all; i0 += AHEAD * THREADS) {
+            Item<T, V, INTERLEAVED> items[AHEAD];  // their loads travel together
+#pragma unroll
+            for (int n = 0; n < AHEAD; ++n) {
+                const unsigned i = i0 + n * THREADS;
+                if (i >= all) break;
+                const unsigned row = i / per_head, tok = row / x.heads;
+                items[n].load((const T*)x.in + from[t][tok] + (row - tok * x.heads) * x.sh,
+                              to + (int64_t)row * a.d, turn + tok * a.half, a.half,
+                              i - row * per_head, turned);
             }
-            const float2* w = turn + tok * a.half;
-            if constexpr (INTERLEAVED) {
-                A v = *(const A*)(in + slot * V), o;
 #pragma unroll
-                for (int e = 0; e < V / 2; ++e) {
-                    float2 c = w[slot * (V / 2) + e];
-                    float p = (float)v.v[2 * e], q = (float)v.v[2 * e + 1];
-                    o.v[2 * e] = (T)(p * c.x - q * c.y);
-                    o.v[2 * e + 1] = (T)(p * c.y + q * c.x);
-                }
-                *(A*)(out + slot * V) = o;
-            } else {
-                A v = *(const A*)(in + slot * V), u = *(const A*)(in + a.half + slot * V), o, r;
-#pragma unroll
-                for (int e = 0; e < V; ++e) {
-                    float2 c = w[slot * V + e];
-                    float p = (float)v.v[e], q = (float)u.v[e];
-                    o.v[e] = (T)(p * c.x - q * c.y);
-                    r.v[e] = (T)(p * c.y + q * c.x);
-                }
-                *(A*)(out + slot * V) = o;
-                *(A*)(out + a.half + slot * V) = r;
+            for (int n = 0; n < AHEAD; ++n) {
+                if (i0 + n * THREADS >= all) break;
+                items[n].store(a.half);
             }
         }
     }
@@ -200,7 +235,7 @@ torch::autograd::variable_list rotate(torch::autograd::variable_list xs,
     // A block's sines serve all its tokens' heads; tokens are shared out so
     // that 8 blocks a CU have work first, and the sines fit.
     int64_t per = std::max<int64_t>(1, a.tokens / 2048);
-    a.per_block = (int)std::min<int64_t>({per, (int64_t)8, (int64_t)(MOST_PAIRS / a.half)});
+    a.per_block = (int)std::min<int64_t>({per, (int64_t)MOST_TOKENS, (int64_t)(MOST_PAIRS / a.half)});
     int64_t blocks = (a.tokens + a.per_block - 1) / a.per_block;
     TORCH_CHECK_VALUE(blocks <= INT_MAX, "rotary: too many tokens for one launch");
     hipStream_t stream = at::hip::getCurrentHIPStream();
