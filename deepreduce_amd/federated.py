@@ -20,6 +20,7 @@ import torch
 
 from .helper import tensor_bits
 from .memory import ResidualMemory
+from .ops import clip_grad_norm_
 
 
 class FederatedServer:
@@ -60,10 +61,14 @@ class FederatedServer:
 
 
 class FederatedClient:
-    def __init__(self, server_model: torch.nn.Module, compressor, local_lr: float = 0.05):
+    """`clip_norm` bounds the global gradient norm of every local step."""
+
+    def __init__(self, server_model: torch.nn.Module, compressor, local_lr: float = 0.05,
+                 clip_norm: float | None = None):
         self.template = server_model
         self.compressor = compressor
         self.local_lr = local_lr
+        self.clip_norm = clip_norm
         self.c2s_memory = ResidualMemory()
         self.x0 = {n: p.detach().clone() for n, p in server_model.named_parameters()}
 
@@ -84,6 +89,9 @@ class FederatedClient:
             for x, y in data_iter():
                 opt.zero_grad()
                 loss_fn(model(x), y).backward()
+                if self.clip_norm is not None:
+                    clip_grad_norm_([p.grad for p in model.parameters() if p.grad is not None],
+                                    self.clip_norm)
                 opt.step()
 
         out = {}

@@ -25,6 +25,7 @@ import torch.distributed as dist
 
 from .communicator import _flatten_payload, _unflatten_payload
 from .memory import ResidualMemory
+from .ops import clip_grad_norm_
 
 __all__ = ["FederatedDistRunner", "serialize_payloads", "deserialize_payloads"]
 
@@ -87,7 +88,7 @@ class FederatedDistRunner:
     """Server (rank 0) + clients (ranks 1..W-1) federated rounds."""
 
     def __init__(self, model: torch.nn.Module, compressor, server_lr=1.0,
-                 local_lr=0.05):
+                 local_lr=0.05, clip_norm: float | None = None):
         self.rank = dist.get_rank()
         self.world = dist.get_world_size()
         assert self.world >= 2, "need >= 2 ranks (1 server + >=1 client)"
@@ -95,6 +96,7 @@ class FederatedDistRunner:
         self.compressor = compressor
         self.server_lr = server_lr
         self.local_lr = local_lr
+        self.clip_norm = clip_norm  # bounds the gradient of every local step
         self.names = [n for n, _ in model.named_parameters()]
         self.x0 = {n: p.detach().clone() for n, p in model.named_parameters()}
         self.memory = ResidualMemory()  # S2C on server / C2S on client
@@ -166,6 +168,9 @@ class FederatedDistRunner:
                 for x, y in data_iter():
                     opt.zero_grad()
                     loss_fn(local(x), y).backward()
+                    if self.clip_norm is not None:
+                        clip_grad_norm_([p.grad for p in local.parameters()
+                                         if p.grad is not None], self.clip_norm)
                     opt.step()
             out = {}
             for n, p in local.named_parameters():

@@ -18,12 +18,21 @@ Modes:
 
 Gradients are compressed in float32 regardless of compute dtype (the wire
 volume accounting and all codecs are float32, matching the reference).
+
+params['clip_norm'] bounds the global gradient norm, by ops.clip_grad_norm_
+(sync-free, so part of the captured graph).  params['clip_stage'] says where:
+  * 'local' (default): each rank's own gradients, before they enter the
+    residual memory, where an outlier would otherwise stay;
+  * 'reduced': the exchanged gradients, which are the same on every rank.
+The norm before clipping is left in `grc.last_grad_norm`, on the device.
 """
 from __future__ import annotations
 
 import os
 
 import torch
+
+from .ops import clip_grad_norm_
 
 __all__ = ["reduce_gradients", "DistributedOptimizer"]
 
@@ -37,20 +46,37 @@ def reduce_gradients(model: torch.nn.Module, grc, names=None, fused: bool = True
     """
     params = [(n, p) for n, p in reversed(list(model.named_parameters()))
               if p.grad is not None]
+    clip, stage = clip_options(grc)
+    if clip is not None and stage == "local" and params:
+        # what reaches the exchange below: the gradient itself, or its copy in 32 bits
+        grads = [p.grad.data.float() for _, p in params]
+        grc.last_grad_norm = clip_grad_norm_(grads, clip)
+    else:
+        grads = None
     if fused and hasattr(grc, "step_many") and os.environ.get("DEEPREDUCE_FUSED", "1") == "1":
-        named = [(n, p.grad.data.float()) for n, p in params]
+        named = [(n, g) for (n, _), g in zip(params, grads or
+                                             [p.grad.data.float() for _, p in params])]
         reduced = grc.step_many(named)
         for (name, p), r in zip(params, reduced):
             p.grad.data.copy_(r.view_as(p.grad.data))
-        return getattr(grc, "last_wire_bytes", 0)
-    total_bytes = 0
-    # reverse order: last layers' grads are ready first after backward
-    for name, p in params:
-        g32 = p.grad.data.float()
-        reduced = grc.step(g32, name)
-        p.grad.data.copy_(reduced.view_as(p.grad.data))
-        total_bytes += getattr(grc, "last_wire_bytes", 0)
+        total_bytes = getattr(grc, "last_wire_bytes", 0)
+    else:
+        total_bytes = 0
+        # reverse order: last layers' grads are ready first after backward
+        for i, (name, p) in enumerate(params):
+            g32 = grads[i] if grads else p.grad.data.float()
+            reduced = grc.step(g32, name)
+            p.grad.data.copy_(reduced.view_as(p.grad.data))
+            total_bytes += getattr(grc, "last_wire_bytes", 0)
+    if clip is not None and stage == "reduced" and params:
+        grc.last_grad_norm = clip_grad_norm_([p.grad.data for _, p in params], clip)
     return total_bytes
+
+
+def clip_options(grc):
+    """(clip_norm or None, clip_stage) of a communicator's params."""
+    params = getattr(grc, "params", None) or {}
+    return params.get("clip_norm"), params.get("clip_stage", "local")
 
 
 def _graph_safe(grc) -> bool:
@@ -222,6 +248,12 @@ class DistributedOptimizer:
     def step(self, closure=None):
         self._exchange()
         return self.optimizer.step(closure)
+
+    @property
+    def last_grad_norm(self):
+        """The last step's gradient norm before clipping, a scalar on the
+        device; None without params['clip_norm']."""
+        return getattr(self.grc, "last_grad_norm", None)
 
     @property
     def param_groups(self):

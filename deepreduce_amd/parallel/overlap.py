@@ -17,6 +17,9 @@ residual pool; on CPU (or for non-qualifying codecs) the bucket falls back
 to the communicator's generic step_many semantics — bit-identical to the
 synchronous DistributedOptimizer path (tested on gloo world=2).
 
+params['clip_norm'] with clip_stage='reduced' bounds the exchanged gradients'
+global norm in finalize().
+
 The residual-update ordering invariant (compensate → compress → update,
 SURVEY.md §7) is preserved per bucket inside the hook.
 """
@@ -24,6 +27,9 @@ from __future__ import annotations
 
 import torch
 import torch.distributed as dist
+
+from ..ops import clip_grad_norm_
+from ..optimizer import clip_options
 
 __all__ = ["OverlappedReducer"]
 
@@ -44,6 +50,12 @@ class OverlappedReducer:
         self.grc = grc
         self.small_threshold = small_threshold
         self.last_wire_bytes = 0
+        self._clip_norm, stage = clip_options(grc)
+        if self._clip_norm is not None and stage == "local":
+            raise ValueError(
+                "clip_stage='local' needs every gradient before the first one is "
+                "compressed, which hook-driven compression does not wait for; use "
+                "clip_stage='reduced' or DistributedOptimizer")
 
         params = [(n, p) for n, p in model.named_parameters() if p.requires_grad]
         self._small = [(n, p) for n, p in params if p.numel() <= small_threshold]
@@ -205,6 +217,10 @@ class OverlappedReducer:
             self._exchange_small(world)
         if self._comm_stream is not None:
             torch.cuda.current_stream().wait_stream(self._comm_stream)
+        if self._clip_norm is not None:
+            grads = [p.grad.data for p in self.model.parameters() if p.grad is not None]
+            if grads:
+                grc.last_grad_norm = clip_grad_norm_(grads, self._clip_norm)
 
     def _exchange_small(self, world):
         if not self._small:

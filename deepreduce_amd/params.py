@@ -36,6 +36,8 @@ _SCHEMA = {
     "fp_aware": (bool, None),
     "wire_dtype": (str, ["fp32", "fp16"]),
     "small_dense": (bool, None),
+    "clip_norm": ((int, float), None),
+    "clip_stage": (str, ["local", "reduced"]),
     "micro-benchmark": (bool, None),
     "log_stats": (str, None),
     # accepted for reference compatibility, unused here:
@@ -64,6 +66,11 @@ def validate(params: dict) -> dict:
     ratio = params.get("compress_ratio")
     if ratio is not None and not (0 < ratio <= 1):
         raise ValueError(f"compress_ratio must be in (0, 1], got {ratio}")
+    clip_norm = params.get("clip_norm")
+    if clip_norm is not None and not clip_norm > 0:
+        raise ValueError(f"clip_norm must be positive, got {clip_norm}")
+    if "clip_stage" in params and clip_norm is None:
+        raise ValueError("clip_stage needs clip_norm")
     fpr = params.get("fpr")
     if isinstance(fpr, str) and fpr != "auto":
         raise ValueError(f"fpr must be a number in (0, 1) or 'auto', got {fpr!r}")
