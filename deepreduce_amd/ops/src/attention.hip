@@ -254,10 +254,25 @@ __device__ __forceinline__ acc16 mma(f32x8 a, f32x8 b, acc16 c) {
 constexpr int RANGE = 32;            // positions whose documents share a range
 constexpr int NONE = 0x7fffffff;
 
+// Rows of a tile in shared memory: chunks of 16 bytes, a power of two a row,
+// at their number XOR a mirrored row number.  16 lanes that read one chunk of
+// 16 rows, and 16 that read four chunks of 4 rows, then meet all banks.
 template <typename T, int DP> struct Tile {
     static constexpr int PER = 16 / sizeof(T);
-    static constexpr int LD = DP + PER;  // rows 16 bytes apart of a multiple of the banks
     static constexpr int VECS = DP / PER;
+    static constexpr int CHUNKS = VECS <= 4 ? 4 : VECS <= 8 ? 8 : VECS <= 16 ? 16 : 32;
+    // 32-bit columns are read one value a lane: a padded row serves them
+    static constexpr int LD = sizeof(T) == 2 ? CHUNKS * PER : DP + PER;
+
+    static __device__ __forceinline__ int mirrored(int row) {
+        if constexpr (CHUNKS == 4) return (row >> 3 & 1) | (row >> 1 & 2);
+        if constexpr (CHUNKS == 8) return (row >> 3 & 1) | (row >> 1 & 2) | (row << 1 & 4);
+        return (row >> 3 & 1) | (row >> 1 & 2) | (row << 1 & 4) | (row << 3 & 8);
+    }
+    static __device__ __forceinline__ int at(int row, int x) {
+        if constexpr (sizeof(T) == 4) return row * LD + x;
+        return row * LD + ((x / PER) ^ mirrored(row)) * PER + x % PER;
+    }
 };
 
 // Rows of one tile on their way from memory to shared memory, through
@@ -292,36 +307,48 @@ template <typename T, int DP, int ROWS, int THREADS> struct Stage {
 #pragma unroll
         for (int n = 0; n < N; ++n) {
             int v = tid + n * THREADS, y = v / G::VECS, x = (v % G::VECS) * G::PER;
-            *(raw4*)(tile + y * G::LD + x) = r[n];
+            *(raw4*)(tile + G::at(y, x)) = r[n];
         }
     }
 };
 
 // rows y0 + l % 32 of a tile, values x0 + (l / 32) * 8 + 0..7
-template <typename T, int LD>
+template <typename T, int DP>
 __device__ __forceinline__ Frag<T> rows_of(const T* tile, int y0, int x0) {
-    const int lane = threadIdx.x & 63;
-    return *(const Frag<T>*)(tile + (y0 + (lane & 31)) * LD + x0 + (lane >> 5) * 8);
+    using G = Tile<T, DP>;
+    const int lane = threadIdx.x & 63, y = lane & 31, x = x0 + (lane >> 5) * 8;
+    Frag<T> f;
+    tile += y0 * G::LD;
+    if constexpr (sizeof(T) == 2) {
+        f = *(const Frag<T>*)(tile + G::at(y, x));
+    } else {
+        const f32x4 lo = *(const f32x4*)(tile + G::at(y, x));
+        const f32x4 hi = *(const f32x4*)(tile + G::at(y, x + 4));
+        f = Frag<T>{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+    }
+    return f;
 }
 
 // columns x0 + l % 32, rows y0 + 8 (j / 4) + 4 (l / 32) + j % 4
-template <typename T, int LD>
+template <typename T, int DP>
 __device__ __forceinline__ Frag<T> columns_of(const T* tile, int y0, int x0) {
+    using G = Tile<T, DP>;
     const int lane = threadIdx.x & 63;
     Frag<T> f;
+    tile += y0 * G::LD;
     if constexpr (sizeof(T) == 2) {
         // 16 lanes read 4 rows of 16 values and get a column of 4 each
-        const T* at = tile + (y0 + (lane >> 5) * 4 + ((lane & 15) >> 2)) * LD + x0 +
-                      ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
+        const int y = (lane >> 5) * 4 + ((lane & 15) >> 2);
+        const int x = x0 + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
         typedef __attribute__((address_space(3))) short4v* Shared;
-        short4v lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Shared)at);
-        short4v hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Shared)(at + 8 * LD));
+        short4v lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Shared)(tile + G::at(y, x)));
+        short4v hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Shared)(tile + G::at(y + 8, x)));
         __builtin_memcpy(&f, &lo, 8);
         __builtin_memcpy((char*)&f + 8, &hi, 8);
     } else {
-        const T* at = tile + (y0 + (lane >> 5) * 4) * LD + x0 + (lane & 31);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) f[j] = at[(8 * (j >> 2) + (j & 3)) * LD];
+        for (int j = 0; j < 8; ++j)
+            f[j] = tile[G::at((lane >> 5) * 4 + 8 * (j >> 2) + (j & 3), x0 + (lane & 31))];
     }
     return f;
 }
@@ -357,14 +384,13 @@ __device__ __forceinline__ float add_halves(float x) {
 // lose more bits than a product of matrices does.
 template <typename T, int DP>
 __device__ __forceinline__ void add_product(const T* tile, int y0, const acc16& c, acc16* sums) {
-    constexpr int LD = Tile<T, DP>::LD;
     const Frag<T> lo = to_frag<T>(c, 0), hi = to_frag<T>(c, 8);
 #pragma unroll
     for (int n = 0; n < DP / 32; ++n) {
         acc16 x = {};
         if constexpr (sizeof(T) == 2) x = sums[n];
-        x = mma(columns_of<T, LD>(tile, y0, n * 32), lo, x);
-        x = mma(columns_of<T, LD>(tile, y0 + 16, n * 32), hi, x);
+        x = mma(columns_of<T, DP>(tile, y0, n * 32), lo, x);
+        x = mma(columns_of<T, DP>(tile, y0 + 16, n * 32), hi, x);
         if constexpr (sizeof(T) == 4) x += sums[n];
         sums[n] = x;
     }
@@ -451,7 +477,7 @@ constexpr int tile_rows = SHARES == 4 || sizeof(T) == 4 ? 32 : 64;
 
 // the shares' tiles and, at the end, the sums they leave for the first
 template <typename T, int DP, int N, int SHARES, int FLOATS> union Shared {
-    alignas(16) T tiles[SHARES][2][N * Tile<T, DP>::LD];
+    alignas(256) T tiles[SHARES][2][N * Tile<T, DP>::LD];
     alignas(16) float boxes[FLOATS ? FLOATS : 4];
 };
 
@@ -704,7 +730,7 @@ void forward_kernel(const Args a, const Ranges keys, const Ranges queries, int t
             if (visits.block) fetch();
             if (!(visits.wave & bit) || (a.causal && at > wave_last)) continue;
             f.template step<N / 32>(
-                [&](int t, int n) { return rows_of<T, G::LD>(tile_k, t * 32, n * 16); }, tile_v,
+                [&](int t, int n) { return rows_of<T, DP>(tile_k, t * 32, n * 16); }, tile_v,
                 docs, at, !(visits.whole & bit) || at + N > a.sk,
                 a.causal && at + N - 1 > wave_first);
         }
@@ -768,7 +794,7 @@ __global__ __launch_bounds__(64, DP >= 96 ? 1 : 2) void split_kernel(const Args 
                                                    float2* part_state) {
     using G = Tile<T, DP>;
     constexpr int N = 32;
-    __shared__ alignas(16) T tile_v[N * G::LD];
+    __shared__ alignas(256) T tile_v[N * G::LD];
     __shared__ alignas(16) int docs[N];
 
     unsigned id = xcd_order(blockIdx.x, gridDim.x);
@@ -1095,10 +1121,10 @@ void dq_kernel(const Args a, const Ranges keys, const Ranges queries, int tiles_
                 acc16 s = {}, dp = {};
 #pragma unroll
                 for (int n = 0; n < DP / 16; ++n)
-                    s = mma(rows_of<T, G::LD>(tile_k, t * 32, n * 16), q[n], s);
+                    s = mma(rows_of<T, DP>(tile_k, t * 32, n * 16), q[n], s);
 #pragma unroll
                 for (int n = 0; n < DP / 16; ++n)
-                    dp = mma(rows_of<T, G::LD>(tile_v, t * 32, n * 16), dout[n], dp);
+                    dp = mma(rows_of<T, DP>(tile_v, t * 32, n * 16), dout[n], dp);
                 exponents<1>(&s, c, off, slope, (float)(pos - at - t * 32 - 4 * hf));
                 if (by_document) hide_documents(s, docs, t, doc);
                 if (by_position) hide_past(s, t, pos - at);
@@ -1296,10 +1322,10 @@ void dkv_kernel(const Args a, const Ranges keys, const Ranges queries, int tiles
                 acc16 s = {}, dp = {};
 #pragma unroll
                 for (int n = 0; n < DP / 16; ++n)
-                    s = mma(rows_of<T, G::LD>(tile_q, t * 32, n * 16), k[n], s);
+                    s = mma(rows_of<T, DP>(tile_q, t * 32, n * 16), k[n], s);
 #pragma unroll
                 for (int n = 0; n < DP / 16; ++n)
-                    dp = mma(rows_of<T, G::LD>(tile_o, t * 32, n * 16), v[n], dp);
+                    dp = mma(rows_of<T, DP>(tile_o, t * 32, n * 16), v[n], dp);
                 if (slope != 0.f)
 #pragma unroll
                     for (int e = 0; e < 16; ++e)
