@@ -358,6 +358,54 @@ def test_attention_refuses(device):
 
 
 @pytest.mark.parametrize("device", BOTH)
+def test_attention_document_numbers(device):
+    """Any number names a document: the largest, zero, far apart; every
+    negative one is padding."""
+    q, k, v, dout = attention_inputs(1, 100, 100, 2, 2, 32, torch.float32, device)
+    top, least = 2 ** 31 - 1, -2 ** 31
+    row = [top] * 20 + [least] * 10 + [0] * 30 + [-1] * 5 + [top] * 10 + [-7] * 5 + [least + 1] * 20
+    documents = torch.tensor([row], dtype=torch.int32, device=device)
+    check_attention(q, k, v, dout, documents)
+    check_attention(q[:, 75:76], k, v, dout[:, 75:76], documents, causal=True)
+    out = ops.attention(q, k, v, documents)
+    assert not out[0, 20:30].any() and not out[0, 60:65].any() and not out[0, 75:].any()
+
+
+@pytest.mark.gpu
+def test_attention_far_offsets():
+    """A cache of over 2^31 values, of which the queries see the last rows, and
+    rows that lie over 16 MB apart."""
+    d, h, sq, near = 128, 32, 256, 300
+    sk = 2 ** 19 + near
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    k, v = (torch.zeros(1, sk, h, d, dtype=torch.float16, device="cuda") for _ in range(2))
+    for t in (k, v):
+        t[:, -near:] = torch.randn(1, near, h, d, generator=gen, device="cuda").half()
+    documents = torch.zeros(1, sk, dtype=torch.int32, device="cuda")
+    documents[:, -near:] = 3
+    for rows in (sq, 1):
+        q, dout = (torch.randn(1, rows, h, d, generator=gen, device="cuda").half()
+                   for _ in range(2))
+        leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+        out = ops.attention(*leaves, documents=documents, causal=True)
+        dq, dk, dv = torch.autograd.grad(out, leaves, dout)
+        few = [t.detach().clone().requires_grad_(True) for t in (q, k[:, -near:], v[:, -near:])]
+        want = ops.attention(*few, causal=True)
+        grads = torch.autograd.grad(want, few, dout)
+        # the same sums in tiles that begin elsewhere
+        for a, c in zip((out, dq, dk[:, -near:], dv[:, -near:]), (want, *grads)):
+            assert (a.float() - c.float()).abs().max() <= 4 * 2.0 ** -11 * c.float().abs().max()
+        assert not dk[:, :-near].any() and not dv[:, :-near].any()
+        del out, dq, dk, dv, leaves
+    del k, v
+    wide = torch.randn(5, 9_000_000, generator=gen, device="cuda").half()
+    k = wide[:, :64].view(1, 5, 1, 64)
+    assert k.stride(1) * 2 > 1 << 24
+    q, dout = (torch.randn(1, 5, 1, 64, generator=gen, device="cuda").half() for _ in range(2))
+    check_attention(q, k, k, dout)
+
+
+@pytest.mark.parametrize("device", BOTH)
 def test_differentiable_once(device):
     q, k, v, dout = attention_inputs(1, 9, 9, 2, 1, 16, torch.float32, device)
     positions = torch.arange(9, device=device)
