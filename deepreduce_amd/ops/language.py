@@ -4,7 +4,8 @@ positions, the global gradient norm and clipping.
 Like the rest of `ops`: HIP kernels (ops/src/attention.hip, rotary.hip,
 grad_norm.hip) on a GPU, the torch reference on the CPU.  Everything runs on
 the current stream without a host synchronisation and can be captured into a
-hipGraph; wrong arguments raise ValueError.
+hipGraph (a backward pass, as ever, while no eager graph of the same leaves is
+alive); wrong arguments raise ValueError.
 """
 from __future__ import annotations
 
@@ -220,8 +221,8 @@ def clip_grad_norm(tensors, max_norm: float, out=None, dtype: torch.dtype | None
     """(clipped, norm): the tensors times min(1, max_norm / norm), and their `grad_norm`.
 
     Writes to `out` (one tensor for each, of its shape and any of the three
-    types; it may be the tensor itself but may not share memory otherwise) or
-    to new tensors of `dtype` (each one's own by default).  A norm that is
+    types; it may be the tensor itself, but the stretches of memory that
+    outputs lie in, gaps included, may not overlap otherwise) or to new tensors of `dtype` (each one's own by default).  A norm that is
     infinite or NaN enters the product as it is: NaN reaches every value.  No
     gradient flows back.
     """

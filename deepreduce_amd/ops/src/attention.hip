@@ -19,6 +19,7 @@
 
 #include <ATen/hip/HIPContext.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPException.h>
 #include <hip/hip_runtime.h>
 #include <algorithm>
 #include <cmath>

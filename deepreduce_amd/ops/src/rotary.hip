@@ -10,12 +10,14 @@
 // sines of its tokens once, into shared memory, and uses them for all heads
 // of all tensors.  Angles are formed and reduced in 64 bits: position 1e6 has
 // an angle that 32 bits hold to 0.06.  The kernel is bound by the one read and
-// write of the heads.
+// write of the heads: 2 x 8191 tokens, 20 heads of 128 in 32 bits, 69 us
+// (4.9 TB/s; a large copy reaches 4.8 to 5.4), where one item at a time took 84.
 
 #include "lm_ops.h"
 
 #include <ATen/hip/HIPContext.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPException.h>
 #include <hip/hip_runtime.h>
 #include <algorithm>
 
@@ -244,6 +246,7 @@ torch::autograd::variable_list rotate(torch::autograd::variable_list xs,
         case torch::kBFloat16: launch_vec<__bf16>(a, v, interleaved, (int)blocks, stream); break;
         default: launch_vec<_Float16>(a, v, interleaved, (int)blocks, stream); break;
     }
+    C10_HIP_KERNEL_LAUNCH_CHECK();
     return outs;
 }
 
