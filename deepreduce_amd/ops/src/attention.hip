@@ -503,6 +503,15 @@ __device__ __forceinline__ unsigned xcd_order(unsigned block, unsigned blocks) {
     return x * each + min(x, more) + block / 8;
 }
 
+// The tile of queries (the last sees most keys) that the n-th block of a head
+// takes where rows are causal.  Blocks go round the CUs: where all fit at once, every other head runs
+// the other way and each CU gets long and short ones (24 heads of 64, 4096
+// rows, 768 blocks, three a CU: forward 99 us for 118); where some wait for
+// others, the longest go first (dq of the same, two a CU: 147 us for 170).
+__device__ __forceinline__ int causal_order(int n, int tiles, int head, bool alternate) {
+    return alternate && (head & 1) ? n : tiles - 1 - n;
+}
+
 constexpr float HEADROOM = 3.f;  // how far (log2) a score may pass the reference maximum
 constexpr float SHIFT = 12.f;    // probabilities carry a factor 2^12, at most 2^15 in all:
                                  // in fp16 the small ones keep their bits
@@ -668,7 +677,8 @@ __device__ __forceinline__ void put4(T* at, float a, float b, float c, float d) 
 // cost more registers than they save (650 -> 580).
 template <typename T, int DP, int ROWS, int SHARES>
 __global__ __launch_bounds__(ROWS * SHARES * 64, (DP >= 96 && SHARES > 1) || (DP == 128 && sizeof(T) == 4) || SHARES == 4 ? 1 : 2)
-void forward_kernel(const Args a, const Ranges keys, const Ranges queries, int tiles_q) {
+void forward_kernel(const Args a, const Ranges keys, const Ranges queries, int tiles_q,
+                    bool alternate) {
     using G = Tile<T, DP>;
     constexpr int BOX = (DP / 2 + 2) * 64;  // o, off and total
     constexpr int THREADS = ROWS * 64, N = tile_rows<T, SHARES>;
@@ -677,7 +687,7 @@ void forward_kernel(const Args a, const Ranges keys, const Ranges queries, int t
 
     unsigned id = xcd_order(blockIdx.x, gridDim.x);
     int qt = id % tiles_q, h = id / tiles_q % a.hq, b = id / tiles_q / a.hq;
-    if (a.causal) qt = tiles_q - 1 - qt;  // the longest first
+    if (a.causal) qt = causal_order(qt, tiles_q, h, alternate);
     const int g = h / (a.hq / a.hkv), lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % ROWS;
     const int share = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) / ROWS;
@@ -902,6 +912,19 @@ __global__ __launch_bounds__(256) void join_kernel(const Args a, int parts, cons
     const int column = blockIdx.x % columns, g = blockIdx.x / columns % a.hkv;
     const int b = blockIdx.x / columns / a.hkv, h = g * group + column / a.sq, i = column % a.sq;
     const int tid = threadIdx.x, wave = tid >> 6;
+    // the first parts' values travel while their weights are found
+    constexpr int SHARES = 256 / DP, AHEAD = 16;
+    const int d = tid % DP, share = tid / DP < SHARES ? tid / DP : parts;
+    const float* from = part_o + (int64_t)blockIdx.x * parts * DP + d;
+    float x[AHEAD];
+    auto fetch = [&](int p0) {
+#pragma unroll
+        for (int n = 0; n < AHEAD; ++n) {
+            const int p = p0 + n * SHARES;
+            x[n] = p < parts ? from[(int64_t)p * DP] : 0.f;
+        }
+    };
+    fetch(share);
     const float2 state = tid < parts ? part_state[(int64_t)blockIdx.x * parts + tid]
                                      : make_float2(0.f, 0.f);
     const float exponent = state.y == 0.f ? -INFINITY : state.x;
@@ -918,15 +941,14 @@ __global__ __launch_bounds__(256) void join_kernel(const Args a, int parts, cons
     total = shared[4] + shared[5] + shared[6] + shared[7];
     const float inv = total == 0.f ? 0.f : 1.f / total;
 
-    constexpr int SHARES = 256 / DP;
-    const int d = tid % DP, share = tid / DP;
     float o = 0;
-    if (share < SHARES) {
-        const float* from = part_o + (int64_t)blockIdx.x * parts * DP + d;
-#pragma unroll 4
-        for (int p = share; p < parts; p += SHARES) {
-            const float w = weight[p], x = from[(int64_t)p * DP];
-            o = w == 0.f ? o : fmaf(w, x, o);
+    for (int p0 = share; p0 < parts; p0 += AHEAD * SHARES) {
+        if (p0 != share) fetch(p0);
+#pragma unroll
+        for (int n = 0; n < AHEAD; ++n) {
+            const int p = p0 + n * SHARES;
+            const float w = p < parts ? weight[p] : 0.f;
+            o = w == 0.f ? o : fmaf(w, x[n], o);
         }
     }
     values[tid] = o;
@@ -994,7 +1016,8 @@ void launch_forward(const Args& a, const Ranges& keys, const Ranges& queries,
     for_shape((int64_t)a.b * a.hq, a.sq, [&](auto rows, auto shares, int tiles, unsigned blocks) {
         constexpr int ROWS = decltype(rows)::value, SHARES = decltype(shares)::value;
         hipLaunchKernelGGL((forward_kernel<T, DP, ROWS, SHARES>), dim3(blocks),
-                           dim3(ROWS * SHARES * 64), 0, stream, a, keys, queries, tiles);
+                           dim3(ROWS * SHARES * 64), 0, stream, a, keys, queries, tiles,
+                           blocks <= (DP <= 64 && sizeof(T) == 2 ? 768 : 512));
     });
 }
 
@@ -1031,7 +1054,7 @@ __device__ __forceinline__ float usable(float lse) { return lse == -INFINITY ? I
 template <typename T, int DP, int ROWS, int SHARES>
 __global__ __launch_bounds__(ROWS * SHARES * 64, DP >= 96 || SHARES > 1 ? 1 : 2)
 void dq_kernel(const Args a, const Ranges keys, const Ranges queries, int tiles_q,
-               float* factors, int factors_n) {
+               bool alternate, float* factors, int factors_n) {
     using G = Tile<T, DP>;
     constexpr int BOX = (CORRECTED<T> ? DP + 1 : DP / 2) * 64;  // acc, mean and rest
     constexpr int THREADS = ROWS * 64, N = tile_rows<T, SHARES>;
@@ -1040,7 +1063,7 @@ void dq_kernel(const Args a, const Ranges keys, const Ranges queries, int tiles_
 
     unsigned id = xcd_order(blockIdx.x, gridDim.x);
     int qt = id % tiles_q, h = id / tiles_q % a.hq, b = id / tiles_q / a.hq;
-    if (a.causal) qt = tiles_q - 1 - qt;
+    if (a.causal) qt = causal_order(qt, tiles_q, h, alternate);
     const int g = h / (a.hq / a.hkv), lane = threadIdx.x & 63, hf = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % ROWS;
     const int share = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) / ROWS;
@@ -1214,7 +1237,7 @@ void dq_kernel(const Args a, const Ranges keys, const Ranges queries, int tiles_
 template <typename T, int DP, int ROWS, int SHARES>
 __global__ __launch_bounds__(ROWS * SHARES * 64, DP >= 96 || (DP == 64 && sizeof(T) == 4) || SHARES == 4 ? 1 : 2)
 void dkv_kernel(const Args a, const Ranges keys, const Ranges queries, int tiles_k,
-                const float* factors, int factors_n) {
+                bool alternate, const float* factors, int factors_n) {
     using G = Tile<T, DP>;
     constexpr int THREADS = ROWS * 64, N = tile_rows<T, SHARES>;  // queries a tile
     constexpr int BOX = DP * 64;  // dk and dv
@@ -1223,7 +1246,9 @@ void dkv_kernel(const Args a, const Ranges keys, const Ranges queries, int tiles
     __shared__ alignas(16) float tile_lses[SHARES][N], tile_deltas[SHARES][N];
 
     unsigned id = xcd_order(blockIdx.x, gridDim.x);
-    const int kt = id % tiles_k, g = id / tiles_k % a.hkv, b = id / tiles_k / a.hkv;
+    const int g = id / tiles_k % a.hkv, b = id / tiles_k / a.hkv;
+    int kt = id % tiles_k;
+    if (a.causal) kt = tiles_k - 1 - causal_order(kt, tiles_k, g, alternate);
     const int group = a.hq / a.hkv, lane = threadIdx.x & 63, hf = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % ROWS;
     const int share = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) / ROWS;
@@ -1413,14 +1438,14 @@ void launch_backward(const Args& a, const Ranges& keys, const Ranges& queries, f
     for_shape((int64_t)a.b * a.hq, a.sq, [&](auto rows, auto shares, int tiles, unsigned blocks) {
         constexpr int ROWS = decltype(rows)::value, SHARES = decltype(shares)::value;
         hipLaunchKernelGGL((dq_kernel<T, DP, ROWS, SHARES>), dim3(blocks),
-                           dim3(ROWS * SHARES * 64), 0, stream, a, keys, queries, tiles, factors,
-                           factors_n);
+                           dim3(ROWS * SHARES * 64), 0, stream, a, keys, queries, tiles,
+                           DP <= 64 && blocks <= 512, factors, factors_n);
     });
     for_shape((int64_t)a.b * a.hkv, a.sk, [&](auto rows, auto shares, int tiles, unsigned blocks) {
         constexpr int ROWS = decltype(rows)::value, SHARES = decltype(shares)::value;
         hipLaunchKernelGGL((dkv_kernel<T, DP, ROWS, SHARES>), dim3(blocks),
-                           dim3(ROWS * SHARES * 64), 0, stream, a, keys, queries, tiles, factors,
-                           factors_n);
+                           dim3(ROWS * SHARES * 64), 0, stream, a, keys, queries, tiles,
+                           DP <= 64 && blocks <= 512, factors, factors_n);
     });
 }
 
