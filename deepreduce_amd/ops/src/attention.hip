@@ -969,8 +969,11 @@ __global__ __launch_bounds__(256) void join_kernel(const Args a, int parts, cons
 int padded(int d) { return (d + 31) / 32 * 32; }
 
 // The shape of the blocks for `length` rows of each of `heads`: 4 waves of 32
-// rows that share their tiles where that gives two blocks a CU; else 2 of them
-// and 2 shares, or 1 and 4.
+// rows that share their tiles where that gives two blocks a CU; 1 wave of rows
+// and 4 shares where that gives no more than one; else 2 and 2.  What counts
+// for few rows is the number of blocks that a CU takes one after the other:
+// 3 x 333 positions, 12 heads of 64 in 32 bits have 396 blocks of 1 x 4, two
+// rounds, and 216 of 2 x 2, one (forward and back 101 and 85 us).
 template <typename F>
 void for_shape(int64_t heads, int length, F f) {
     auto blocks = [&](int rows) { return heads * ((length + rows - 1) / rows); };
@@ -981,15 +984,20 @@ void for_shape(int64_t heads, int length, F f) {
     };
     if (blocks(128) >= 512)
         go(std::integral_constant<int, 4>{}, std::integral_constant<int, 1>{});
-    else if (blocks(64) >= 256)
+    else if (blocks(32) > 256)
         go(std::integral_constant<int, 2>{}, std::integral_constant<int, 2>{});
     else
         go(std::integral_constant<int, 1>{}, std::integral_constant<int, 4>{});
 }
 
 // Whether the forward pass is split over the keys: where 32 queries a block
-// give fewer blocks than there are CUs.
-bool split_keys(const Args& a) { return (int64_t)a.b * a.hq * ((a.sq + 31) / 32) < 256; }
+// give fewer blocks than there are CUs, and the rows to join are fewer than the
+// keys.  12 heads of 64, bf16, split and not: 1 query of 2048 keys 9 and 22 us,
+// 128 of 2048 19 and 22, 512 of 8192 55 and 73, but 512 of 2048 36 and 23.
+bool split_keys(const Args& a) {
+    const int64_t heads = (int64_t)a.b * a.hq;
+    return heads * ((a.sq + 31) / 32) < 256 && heads * a.sq <= a.sk;
+}
 
 template <typename T, int DP>
 void launch_split(const Args& a, const torch::Tensor& like, hipStream_t stream) {
