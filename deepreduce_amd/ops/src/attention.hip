@@ -672,9 +672,9 @@ __device__ __forceinline__ void put4(T* at, float a, float b, float c, float d) 
 // Heads of 64 are bound by the vector unit (a multiply-add, an exponential, a
 // maximum, a sum and half a conversion for each pair, 53 % of its cycles beside
 // 29 % of the matrix unit's), heads of 128 by the two in turn.  2 x 16 heads,
-// 4096 x 4096, bf16: 650 TFLOP/s at 64, 900 at 128; a large matrix product
-// reaches 1244.  Tiles of 64 keys: halves of a tile passed over by documents
-// cost more registers than they save (650 -> 580).
+// 4096 x 4096, bf16: 640 TFLOP/s at 64, 850 to 900 at 128; a large matrix product
+// reaches 1244.  Tiles of 64 keys: passing over half a tile by its documents
+// costs more than it saves (582 TFLOP/s).
 template <typename T, int DP, int ROWS, int SHARES>
 __global__ __launch_bounds__(ROWS * SHARES * 64, (DP >= 96 && SHARES > 1) || (DP == 128 && sizeof(T) == 4) || SHARES == 4 ? 1 : 2)
 void forward_kernel(const Args a, const Ranges keys, const Ranges queries, int tiles_q,
@@ -795,8 +795,8 @@ void forward_kernel(const Args a, const Ranges keys, const Ranges queries, int t
         forward_row<T>(a, b, h, row0 + __builtin_ctzll(rows));
 }
 
-// Few queries over many keys: bound by one read of K and V, 6.2 TB/s for 8
-// requests with 4 heads of 64 over 32768 keys (43 us, and 7 us the join).  A wave takes up
+// Few queries over many keys: bound by one read of K and V, 6.1 TB/s for 8
+// requests with 4 heads of 64 over 32768 keys (44 us, and 5 us the join).  A wave takes up
 // to 32 columns, which are the queries of all heads of one key-value head, and
 // one part of the keys; nothing is shared between waves.  K's fragments are
 // rows as they lie in memory and go straight to registers, V passes through
@@ -1039,7 +1039,8 @@ void launch_forward(const Args& a, const Ranges& keys, const Ranges& queries,
 // 2 x 16 heads, 4096 x 4096, bf16: dq 820 TFLOP/s and dkv 700 with heads of 64,
 // 810 and 630 with heads of 128, whose sums leave one wave a SIMD: K and V in
 // shared memory make room for two, but then its reads bound the kernel (604).
-// Rows of few documents (32 x 512) are bound by the waits of short blocks.
+// Packed rows of 512 (32 of them, 12 heads of 64: dq 77 us, dkv 82) are bound by
+// their blocks' reads, in step with each other, and the masks of mixed tiles.
 //
 // dS is rounded to the inputs' type for its products.  In fp16 it first gets
 // a factor, a power of two that puts the largest dout of 32 queries near 2^-4
