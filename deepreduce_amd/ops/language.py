@@ -232,7 +232,8 @@ def clip_grad_norm(tensors, max_norm: float, out=None, dtype: torch.dtype | None
            f"clip_grad_norm: dtype must be float32, bfloat16 or float16, got {dtype}")
     hip = _hip(grads[0])
     if hip:
-        return hip.clip_grad_norm(grads, max_norm, outs, dtype)
+        new, norm = hip.clip_grad_norm(grads, max_norm, outs, dtype)
+        return new if outs is None else outs, norm
     _check_gradients(grads, "clip_grad_norm")
     _check(max_norm >= 0, f"clip_grad_norm: max_norm must be 0 or more, got {max_norm}")
     _check(dtype is None or out is None, "clip_grad_norm: dtype is for new tensors, without out")

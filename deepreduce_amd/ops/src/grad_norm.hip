@@ -385,6 +385,7 @@ torch::Tensor grad_norm(std::vector<torch::Tensor> grads) {
     return norm;
 }
 
+// the new tensors, none where `out` takes the results, and the norm
 std::pair<std::vector<torch::Tensor>, torch::Tensor> clip_grad_norm(
     std::vector<torch::Tensor> grads, double max_norm,
     std::optional<std::vector<torch::Tensor>> out, std::optional<torch::ScalarType> dtype) {
@@ -401,7 +402,7 @@ std::pair<std::vector<torch::Tensor>, torch::Tensor> clip_grad_norm(
         for (auto& t : grads)
             outs.push_back(torch::empty_like(t, t.options().dtype(dtype.value_or(t.scalar_type()))));
     }
-    const std::vector<torch::Tensor> results = outs;
+    const std::vector<torch::Tensor> results = out ? std::vector<torch::Tensor>() : outs;
     TORCH_CHECK_VALUE(outs.size() == grads.size(), "clip_grad_norm: needs one output a gradient");
     check_grads(outs);
     TORCH_CHECK_VALUE(outs[0].device() == grads[0].device(),
@@ -473,6 +474,6 @@ std::pair<std::vector<torch::Tensor>, torch::Tensor> clip_grad_norm(
     C10_HIP_KERNEL_LAUNCH_CHECK();
     for (auto& c : copies) c.second.copy_(outs[c.first]);
     if (out)
-        for (auto& t : results) t.unsafeGetTensorImpl()->bump_version();
+        for (auto& t : *out) t.unsafeGetTensorImpl()->bump_version();
     return {results, norm};
 }

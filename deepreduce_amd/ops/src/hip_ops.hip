@@ -3249,7 +3249,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     namespace py = pybind11;
     m.def("grad_norm", &grad_norm, "global 2-norm of many tensors (HIP)");
     m.def("clip_grad_norm", &clip_grad_norm,
-          "(tensors scaled to a global 2-norm of at most max_norm, that norm) (HIP)",
+          "(new tensors scaled to a global 2-norm of at most max_norm, the norm) (HIP)",
           py::arg("grads"), py::arg("max_norm"), py::arg("out") = py::none(),
           py::arg("dtype") = py::none());
     m.def("rotary", &rotary, "rotary positions of queries and keys (HIP)");
