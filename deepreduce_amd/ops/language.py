@@ -182,7 +182,8 @@ def rotary(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor,
            and 1 <= frequencies.numel() <= d // 2,
            f"rotary: frequencies must be float64 with 1 to {d // 2} values")
     _check(not frequencies.requires_grad, "rotary: frequencies are constants and get no gradient")
-    _check(d % 2 == 0 and d <= 1024, f"rotary: the head size must be even and at most 1024, got {d}")
+    _check(d % 2 == 0 and d <= 1024,
+           f"rotary: the head size must be even and at most 1024, got {d}")
     return _Rotary.apply(q, k, positions.expand(b, s), frequencies, bool(interleaved))
 
 
@@ -222,9 +223,10 @@ def clip_grad_norm(tensors, max_norm: float, out=None, dtype: torch.dtype | None
 
     Writes to `out` (one tensor for each, of its shape and any of the three
     types; it may be the tensor itself, but the stretches of memory that
-    outputs lie in, gaps included, may not overlap otherwise) or to new tensors of `dtype` (each one's own by default).  A norm that is
-    infinite or NaN enters the product as it is: NaN reaches every value.  No
-    gradient flows back.
+    outputs lie in, gaps included, may not overlap otherwise) or to new tensors
+    of `dtype` (each one's own by default).  A norm that is infinite or NaN
+    enters the product as it is: NaN reaches every value.  No gradient flows
+    back.
     """
     grads, outs = _list(tensors), None if out is None else _list(out)
     max_norm = float(max_norm)
@@ -262,6 +264,9 @@ def _check_apart(grads, outs):
         last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
         return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
 
+    for i, o in enumerate(outs):
+        _check(all(n < 2 or s for n, s in zip(o.shape, o.stride())),
+               f"clip_grad_norm: output {i} is expanded")
     written = sorted((*span(o), i) for i, o in enumerate(outs) if o.numel())
     for (_, end, i), (at, _, j) in zip(written, written[1:]):
         _check(at >= end, f"clip_grad_norm: outputs {i} and {j} share memory")

@@ -261,7 +261,7 @@ constexpr int NONE = 0x7fffffff;
 template <typename T, int DP> struct Tile {
     static constexpr int PER = 16 / sizeof(T);
     static constexpr int VECS = DP / PER;
-    static constexpr int CHUNKS = VECS <= 4 ? 4 : VECS <= 8 ? 8 : VECS <= 16 ? 16 : 32;
+    static constexpr int CHUNKS = VECS <= 4 ? 4 : VECS <= 8 ? 8 : 16;
     // 32-bit columns are read one value a lane: a padded row serves them
     static constexpr int LD = sizeof(T) == 2 ? CHUNKS * PER : DP + PER;
 
@@ -504,13 +504,24 @@ __device__ __forceinline__ unsigned xcd_order(unsigned block, unsigned blocks) {
 }
 
 // The tile of queries (the last sees most keys) that the n-th block of a head
-// takes where rows are causal.  Blocks go round the CUs: where all fit at once, every other head runs
-// the other way and each CU gets long and short ones (24 heads of 64, 4096
-// rows, 768 blocks, three a CU: forward 99 us for 118); where some wait for
-// others, the longest go first (dq of the same, two a CU: 147 us for 170).
+// takes where rows are causal.  Blocks go round the CUs: where all fit at once,
+// every other head runs the other way and each CU gets long and short ones (24
+// heads of 64, 4096 rows, 768 blocks, three a CU: forward 99 us for 118); where
+// some wait for others, the longest go first (dq of the same, two a CU: 147 us
+// for 170).
 __device__ __forceinline__ int causal_order(int n, int tiles, int head, bool alternate) {
     return alternate && (head & 1) ? n : tiles - 1 - n;
 }
+
+// Waves a SIMD that the registers are shared out for: 2, or 1 where two would
+// spill (to 256 registers; 3 spill in the backward of heads of 64: dq 133 us for
+// 72 on packed rows of 512).
+template <typename T, int DP, int SHARES>
+constexpr int forward_waves =
+    (DP >= 96 && SHARES > 1) || (DP == 128 && sizeof(T) == 4) || SHARES == 4 ? 1 : 2;
+template <int DP, int SHARES> constexpr int dq_waves = DP >= 96 || SHARES > 1 ? 1 : 2;
+template <typename T, int DP, int SHARES>
+constexpr int dkv_waves = DP >= 96 || (DP == 64 && sizeof(T) == 4) || SHARES == 4 ? 1 : 2;
 
 constexpr float HEADROOM = 3.f;  // how far (log2) a score may pass the reference maximum
 constexpr float SHIFT = 12.f;    // probabilities carry a factor 2^12, at most 2^15 in all:
@@ -676,7 +687,7 @@ __device__ __forceinline__ void put4(T* at, float a, float b, float c, float d) 
 // reaches 1244.  Tiles of 64 keys: passing over half a tile by its documents
 // costs more than it saves (582 TFLOP/s).
 template <typename T, int DP, int ROWS, int SHARES>
-__global__ __launch_bounds__(ROWS * SHARES * 64, (DP >= 96 && SHARES > 1) || (DP == 128 && sizeof(T) == 4) || SHARES == 4 ? 1 : 2)
+__global__ __launch_bounds__(ROWS * SHARES * 64, (forward_waves<T, DP, SHARES>))
 void forward_kernel(const Args a, const Ranges keys, const Ranges queries, int tiles_q,
                     bool alternate) {
     using G = Tile<T, DP>;
@@ -803,9 +814,9 @@ void forward_kernel(const Args a, const Ranges keys, const Ranges queries, int t
 // shared memory for its columns; both travel a tile ahead.  join_kernel adds
 // the parts up, each with its own exponent.
 template <typename T, int DP>
-__global__ __launch_bounds__(64, DP >= 96 ? 1 : 2) void split_kernel(const Args a, int parts, int keys_each,
-                                                   int column_tiles, float* part_o,
-                                                   float2* part_state) {
+__global__ __launch_bounds__(64, DP >= 96 ? 1 : 2)
+void split_kernel(const Args a, int parts, int keys_each, int column_tiles, float* part_o,
+                  float2* part_state) {
     using G = Tile<T, DP>;
     constexpr int N = 32;
     __shared__ alignas(256) T tile_v[N * G::LD];
@@ -1032,9 +1043,9 @@ void launch_forward(const Args& a, const Ranges& keys, const Ranges& queries,
 // ---------------------------------------------------------------------------
 // Backward.  First the queries' gradient, whose waves hold 32 queries as the
 // forward's do, and their delta; then the keys' and values', whose waves hold
-// 32 keys and go over the queries of all heads that share them.  Scores are formed again
-// in both (7 products where 5 would do), so that nothing is added across
-// blocks: results repeat bit by bit and no buffer of gradients is needed.
+// 32 keys and go over the queries of all heads that share them.  Scores are
+// formed again in both (7 products where 5 would do), so that nothing is added
+// across blocks: results repeat bit by bit and no buffer of gradients is needed.
 //
 // 2 x 16 heads, 4096 x 4096, bf16: dq 820 TFLOP/s and dkv 700 with heads of 64,
 // 810 and 630 with heads of 128, whose sums leave one wave a SIMD: K and V in
@@ -1061,7 +1072,7 @@ template <typename T> constexpr bool CORRECTED = sizeof(T) == 2;
 __device__ __forceinline__ float usable(float lse) { return lse == -INFINITY ? INFINITY : lse; }
 
 template <typename T, int DP, int ROWS, int SHARES>
-__global__ __launch_bounds__(ROWS * SHARES * 64, DP >= 96 || SHARES > 1 ? 1 : 2)
+__global__ __launch_bounds__(ROWS * SHARES * 64, (dq_waves<DP, SHARES>))
 void dq_kernel(const Args a, const Ranges keys, const Ranges queries, int tiles_q,
                bool alternate, float* factors, int factors_n) {
     using G = Tile<T, DP>;
@@ -1244,7 +1255,7 @@ void dq_kernel(const Args a, const Ranges keys, const Ranges queries, int tiles_
 }
 
 template <typename T, int DP, int ROWS, int SHARES>
-__global__ __launch_bounds__(ROWS * SHARES * 64, DP >= 96 || (DP == 64 && sizeof(T) == 4) || SHARES == 4 ? 1 : 2)
+__global__ __launch_bounds__(ROWS * SHARES * 64, (dkv_waves<T, DP, SHARES>))
 void dkv_kernel(const Args a, const Ranges keys, const Ranges queries, int tiles_k,
                 bool alternate, const float* factors, int factors_n) {
     using G = Tile<T, DP>;

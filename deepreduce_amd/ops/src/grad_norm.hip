@@ -400,7 +400,8 @@ std::pair<std::vector<torch::Tensor>, torch::Tensor> clip_grad_norm(
         outs = *out;
     } else {
         for (auto& t : grads)
-            outs.push_back(torch::empty_like(t, t.options().dtype(dtype.value_or(t.scalar_type()))));
+            outs.push_back(
+                torch::empty_like(t, t.options().dtype(dtype.value_or(t.scalar_type()))));
     }
     const std::vector<torch::Tensor> results = out ? std::vector<torch::Tensor>() : outs;
     TORCH_CHECK_VALUE(outs.size() == grads.size(), "clip_grad_norm: needs one output a gradient");
@@ -429,13 +430,16 @@ std::pair<std::vector<torch::Tensor>, torch::Tensor> clip_grad_norm(
     for (size_t i = 0; i < outs.size(); ++i) {
         TORCH_CHECK_VALUE(outs[i].sizes() == grads[i].sizes(), "clip_grad_norm: output ", i,
                           " has another shape");
+        for (int64_t d = 0; d < outs[i].dim(); ++d)
+            TORCH_CHECK_VALUE(outs[i].size(d) < 2 || outs[i].stride(d), "clip_grad_norm: output ",
+                              i, " is expanded");
         if (outs[i].numel()) ranges.push_back(range(outs[i], i));
     }
     std::sort(ranges.begin(), ranges.end(),
               [](const Range& a, const Range& b) { return a.at < b.at; });
     for (size_t i = 1; i < ranges.size(); ++i)
-        TORCH_CHECK_VALUE(ranges[i].at >= ranges[i - 1].end, "clip_grad_norm: outputs ", ranges[i - 1].i, " and ",
-                    ranges[i].i, " share memory");
+        TORCH_CHECK_VALUE(ranges[i].at >= ranges[i - 1].end, "clip_grad_norm: outputs ",
+                          ranges[i - 1].i, " and ", ranges[i].i, " share memory");
     for (size_t i = 0; i < grads.size(); ++i) {
         if (!grads[i].numel()) continue;
         Range r = range(grads[i], i);
@@ -443,9 +447,9 @@ std::pair<std::vector<torch::Tensor>, torch::Tensor> clip_grad_norm(
                                    [](const char* a, const Range& b) { return a < b.end; });
         if (it == ranges.end() || it->at >= r.end) continue;
         TORCH_CHECK_VALUE(it->i == i && it->at == r.at && it->end == r.end &&
-                        outs[i].scalar_type() == grads[i].scalar_type() &&
-                        same_strides(outs[i], grads[i]),
-                    "clip_grad_norm: gradient ", i, " shares memory with output ", it->i);
+                              outs[i].scalar_type() == grads[i].scalar_type() &&
+                              same_strides(outs[i], grads[i]),
+                          "clip_grad_norm: gradient ", i, " shares memory with output ", it->i);
     }
 
     // other orders than dense ones go through copies

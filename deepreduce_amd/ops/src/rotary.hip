@@ -237,7 +237,8 @@ torch::autograd::variable_list rotate(torch::autograd::variable_list xs,
     // A block's sines serve all its tokens' heads; tokens are shared out so
     // that 8 blocks a CU have work first, and the sines fit.
     int64_t per = std::max<int64_t>(1, a.tokens / 2048);
-    a.per_block = (int)std::min<int64_t>({per, (int64_t)MOST_TOKENS, (int64_t)(MOST_PAIRS / a.half)});
+    a.per_block =
+        (int)std::min<int64_t>({per, (int64_t)MOST_TOKENS, (int64_t)(MOST_PAIRS / a.half)});
     int64_t blocks = (a.tokens + a.per_block - 1) / a.per_block;
     TORCH_CHECK_VALUE(blocks <= INT_MAX, "rotary: too many tokens for one launch");
     hipStream_t stream = at::hip::getCurrentHIPStream();

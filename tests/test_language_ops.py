@@ -685,6 +685,8 @@ def test_clip_refuses(device):
                  lambda: ops.clip_grad_norm([x], 1.0, out=[y.double()]),
                  lambda: ops.clip_grad_norm([x], 1.0, out=[y], dtype=torch.float16),
                  lambda: ops.clip_grad_norm([x], 1.0, dtype=torch.int32),
+                 lambda: ops.clip_grad_norm([x.new_ones(4, 8)], 1.0, out=[y.expand(4, 8)]),
+                 lambda: ops.clip_grad_norm_([x.expand(4, 8)], 1.0),
                  lambda: ops.clip_grad_norm_([x, x], 1.0),
                  lambda: ops.clip_grad_norm_([x[:5], x[4:]], 1.0),
                  lambda: ops.clip_grad_norm([x[:4], y[:4]], 1.0, out=[y[4:], y[2:6]]),
