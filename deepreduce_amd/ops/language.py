@@ -4,8 +4,9 @@ positions, the global gradient norm and clipping.
 Like the rest of `ops`: HIP kernels (ops/src/attention.hip, rotary.hip,
 grad_norm.hip) on a GPU, the torch reference on the CPU.  Everything runs on
 the current stream without a host synchronisation and can be captured into a
-hipGraph (a backward pass, as ever, while no eager graph of the same leaves is
-alive); wrong arguments raise ValueError.
+hipGraph; wrong arguments raise ValueError.  A backward pass is captured while
+no eager graph of the same leaves is alive: with one, torch ends the process,
+which attention and rotary refuse where the leaves are their own inputs.
 """
 from __future__ import annotations
 

@@ -1689,11 +1689,13 @@ struct AttentionFunction : torch::autograd::Function<AttentionFunction> {
         ctx->save_for_backward(saved);
         ctx->saved_data["causal"] = causal;
         ctx->saved_data["scale"] = scale;
+        ctx->saved_data["elsewhere"] = held_elsewhere({q, k, v});
         return r[0];
     }
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
                                                    torch::autograd::variable_list grads) {
         const auto x = ctx->get_saved_variables();
+        check_capture(ctx->saved_data["elsewhere"].toBool(), "attention");
         torch::autograd::variable_list d;
         {
             at::AutoGradMode no(false);

@@ -3,6 +3,8 @@
 #pragma once
 #include <torch/extension.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <ATen/hip/HIPContext.h>
+#include <c10/core/impl/VirtualGuardImpl.h>
 #include <optional>
 #include <string>
 #include <vector>
@@ -19,6 +21,30 @@ torch::Tensor attention(torch::Tensor q, torch::Tensor k, torch::Tensor v,
                         std::optional<torch::Tensor> documents,
                         std::optional<torch::Tensor> slopes, bool causal,
                         std::optional<double> scale);
+
+// A leaf keeps the node that takes its gradient, and that node's stream, as
+// long as any graph holds it.  A backward pass that is captured on another
+// stream would leave the capture through it, which ends the process: the
+// functions note such leaves and refuse that backward.
+inline bool held_elsewhere(std::initializer_list<torch::Tensor> leaves) {
+    for (auto& t : leaves) {
+        if (!t.requires_grad() || !t.is_leaf()) continue;
+        auto node = torch::autograd::impl::try_get_grad_accumulator(t);
+        if (!node) continue;
+        const c10::impl::VirtualGuardImpl device(t.device().type());
+        const auto stream = node->stream();
+        if (stream && *stream != device.getStream(t.device())) return true;
+    }
+    return false;
+}
+inline void check_capture(bool elsewhere, const char* name) {
+    if (!elsewhere) return;
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    C10_HIP_CHECK(hipStreamIsCapturing(at::hip::getCurrentHIPStream(), &status));
+    TORCH_CHECK(status == hipStreamCaptureStatusNone, name,
+                ": an eager graph of the same leaves is alive on another stream; let it go before "
+                "a backward pass is captured");
+}
 
 // gradients that may be used in a graph of their own but not through it
 inline torch::autograd::variable_list once_differentiable(torch::autograd::variable_list grads,

@@ -259,11 +259,13 @@ struct RotaryFunction : torch::autograd::Function<RotaryFunction> {
                                                   bool interleaved) {
         ctx->save_for_backward({positions, frequencies});
         ctx->saved_data["interleaved"] = interleaved;
+        ctx->saved_data["elsewhere"] = held_elsewhere({q, k});
         return rotate({q, k}, positions, frequencies, interleaved, false);
     }
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
                                                    torch::autograd::variable_list grads) {
         const auto x = ctx->get_saved_variables();
+        check_capture(ctx->saved_data["elsewhere"].toBool(), "rotary");
         torch::autograd::variable_list need, d(5);
         for (int n = 0; n < 2; ++n)
             if (ctx->needs_input_grad(n)) need.push_back(grads[n]);

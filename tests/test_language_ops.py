@@ -723,3 +723,67 @@ def test_clip_repeats_and_replays():
         assert torch.equal(n, norm) and torch.equal(n, alone)
         for a, c in zip(first, eager):
             assert torch.equal(a, c)
+
+
+@pytest.mark.gpu
+def test_two_streams_and_a_graph():
+    """Calls on two streams at once, and two captured graphs replayed in turn,
+    each with its own workspaces, against the same calls one by one."""
+    def make(seed):
+        q, k, v, dout = attention_inputs(2, 150, 150, 4, 2, 64, torch.float16, "cuda", seed)
+        grads = [torch.randn(n, device="cuda") for n in (70_001, 33)]
+        return [q.requires_grad_(True), k.requires_grad_(True), v.requires_grad_(True)], dout, grads
+
+    documents = DOCS["packed"](2, 150).cuda()
+    positions, frequencies = torch.arange(150, device="cuda"), ops.rotary_frequencies(
+        64, device="cuda")
+
+    def work(x):
+        leaves, dout, grads = x
+        q, k = ops.rotary(*leaves[:2], positions, frequencies, interleaved=True)
+        out = ops.attention(q, k, leaves[2], documents)
+        clipped, norm = ops.clip_grad_norm(grads, 0.5)
+        few = ops.attention(q[:, -1:].detach(), k.detach(), leaves[2].detach(), documents)
+        # no graph of the leaves outlives the call: see the test below
+        return [out.detach(), few, *torch.autograd.grad(out, leaves, dout), *clipped, norm]
+
+    inputs = [make(1), make(2)]
+    want = [work(x) for x in inputs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [None, None]
+    for _ in range(5):
+        for n, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[n] = work(inputs[n])
+    torch.cuda.synchronize()
+    for a, c in zip(got[0] + got[1], want[0] + want[1]):
+        assert torch.equal(a, c)
+    graphs, held = [], []
+    for x in inputs:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            held.append(work(x))
+    for turn in (0, 1, 0, 0, 1):
+        graphs[turn].replay()
+        torch.cuda.synchronize()
+        for a, c in zip(held[turn], want[turn]):
+            assert torch.equal(a, c)
+
+
+@pytest.mark.gpu
+def test_captured_backward_beside_an_eager_graph_is_refused():
+    """The leaves' gradients would go to another stream than the captured one."""
+    q, k, v, dout = attention_inputs(1, 40, 40, 2, 2, 32, torch.float32, "cuda")
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    positions, frequencies = torch.arange(40, device="cuda"), ops.rotary_frequencies(
+        32, device="cuda")
+    calls = (lambda: ops.attention(*leaves),
+             lambda: ops.rotary(q, k, positions, frequencies)[0])
+    for call in calls:
+        alive = call()
+        with pytest.raises(RuntimeError, match="eager graph"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                torch.autograd.grad(call(), leaves[:1], dout)
+        torch.cuda.synchronize()
+        torch.autograd.grad(alive, leaves[:1], dout)
