@@ -7,6 +7,9 @@ the current stream without a host synchronisation and can be captured into a
 hipGraph; wrong arguments raise ValueError.  A backward pass is captured while
 no eager graph of the same leaves is alive: with one, torch ends the process,
 which attention and rotary refuse where the leaves are their own inputs.
+Attention and rotary have no forward-mode derivatives and refuse dual tensors;
+on a GPU none of the operators can be traced (torch.jit.trace, make_fx), since
+a trace holds torch operations only.
 """
 from __future__ import annotations
 
@@ -209,7 +212,8 @@ def grad_norm(tensors) -> torch.Tensor:
     """The 2-norm of all values of all tensors: a float32 scalar on their device.
 
     Tensors of any shape, order and mixture of float32, bfloat16 and float16.
-    Squares are added in 64 bits, in a fixed order.  No gradient flows back.
+    Squares are added in 64 bits, in a fixed order.  A constant for both
+    modes of differentiation.
     """
     grads = _list(tensors)
     hip = _hip(grads[0])
@@ -226,8 +230,8 @@ def clip_grad_norm(tensors, max_norm: float, out=None, dtype: torch.dtype | None
     types; it may be the tensor itself, but the stretches of memory that
     outputs lie in, gaps included, may not overlap otherwise) or to new tensors
     of `dtype` (each one's own by default).  A norm that is infinite or NaN
-    enters the product as it is: NaN reaches every value.  No gradient flows
-    back.
+    enters the product as it is: NaN reaches every value.  Constants for both
+    modes of differentiation.
     """
     grads, outs = _list(tensors), None if out is None else _list(out)
     max_norm = float(max_norm)

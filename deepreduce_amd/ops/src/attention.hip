@@ -1720,11 +1720,12 @@ torch::Tensor attention(torch::Tensor q, torch::Tensor k, torch::Tensor v,
     if (documents && documents->dim() == 2 && documents->size(1) > 1 && documents->stride(1) != 1)
         documents = documents->contiguous();
     if (slopes) slopes = slopes->contiguous();
+    const torch::Tensor none;
+    check_seen({q, k, v, slopes.value_or(none)}, "attention");
     const double by = scale.value_or(1.0 / std::sqrt((double)q.size(3)));
     if (at::GradMode::is_enabled() &&
         (q.requires_grad() || k.requires_grad() || v.requires_grad()))
         return AttentionFunction::apply(q, k, v, documents, slopes, causal, by);
-    const torch::Tensor none;
     return attention_forward(q, k, v, documents.value_or(none), slopes.value_or(none), causal, by,
                              false)[0];
 }

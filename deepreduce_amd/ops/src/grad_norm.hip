@@ -371,6 +371,7 @@ torch::Tensor partial_sums(const Plan& p, const torch::Tensor& like, hipStream_t
 torch::Tensor grad_norm(std::vector<torch::Tensor> grads) {
     TORCH_CHECK_VALUE(!grads.empty() && grads[0].is_cuda(), "grad_norm: needs GPU tensors");
     check_grads(grads);
+    check_seen({}, "grad_norm");
     at::NoGradGuard no_grad;
     c10::DeviceGuard guard(grads[0].device());
     for (auto& t : grads)
@@ -393,6 +394,7 @@ std::pair<std::vector<torch::Tensor>, torch::Tensor> clip_grad_norm(
     TORCH_CHECK_VALUE(max_norm >= 0, "clip_grad_norm: max_norm must be 0 or more, got ", max_norm);
     TORCH_CHECK_VALUE(!out || !dtype, "clip_grad_norm: dtype is for new tensors, without out");
     check_grads(grads);
+    check_seen({}, "clip_grad_norm");
     at::NoGradGuard no_grad;
     c10::DeviceGuard guard(grads[0].device());
     std::vector<torch::Tensor> outs;

@@ -3,7 +3,9 @@
 #pragma once
 #include <torch/extension.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <ATen/hip/HIPContext.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/core/impl/VirtualGuardImpl.h>
 #include <optional>
 #include <string>
@@ -44,6 +46,19 @@ inline void check_capture(bool elsewhere, const char* name) {
     TORCH_CHECK(status == hipStreamCaptureStatusNone, name,
                 ": an eager graph of the same leaves is alive on another stream; let it go before "
                 "a backward pass is captured");
+}
+
+// A kernel's launch is no operation that torch sees: forward-mode derivatives
+// would end at it, and a tracer would record its empty results.
+inline void check_seen(std::initializer_list<torch::Tensor> inputs, const char* name) {
+    using c10::impl::TorchDispatchModeTLS;
+    TORCH_CHECK(!torch::jit::tracer::isTracing() &&
+                    !TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY),
+                name, ": cannot be traced on a GPU");
+    if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+    for (auto& t : inputs)
+        TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(0).defined(), name,
+                                    ": has no forward-mode derivative");
 }
 
 // gradients that may be used in a graph of their own but not through it

@@ -314,6 +314,7 @@ std::vector<torch::Tensor> rotary(torch::Tensor q, torch::Tensor k, torch::Tenso
                       " values on q's device");
     TORCH_CHECK_VALUE(!frequencies.requires_grad(),
                       "rotary: frequencies are constants and get no gradient");
+    check_seen({q, k, frequencies}, "rotary");
     frequencies = frequencies.contiguous();
     if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad()))
         return RotaryFunction::apply(q, k, positions, frequencies, interleaved);
