@@ -1054,11 +1054,18 @@ void launch_forward(const Args& a, const Ranges& keys, const Ranges& queries,
 // their blocks' reads, in step with each other, and the masks of mixed tiles.
 //
 // dS is rounded to the inputs' type for its products.  In fp16 it first gets
-// a factor, a power of two that puts the largest dout of 32 queries near 2^-4
-// and P's 2^12 with it, so that gradients of any size keep their bits.
+// a factor, a power of two that puts the largest dout of its query near 2^-4
+// and P's 2^12 with it, so that dq keeps its bits at any size of gradient.  For
+// dk the queries of a tile share the least of their factors, and the sums go
+// along with it from tile to tile (by no more than they have to: the scale may
+// lie FACTOR_ROOM below the tile's), so that queries with large gradients cost
+// others no bits unless they share a tile.  A query without a gradient has the
+// largest factor, that of the least dout, and so takes nothing from its tile.
 // ---------------------------------------------------------------------------
 
 constexpr int FACTOR_ROWS = 32;
+constexpr float MOST_FACTOR = 0x1p20f;  // 2^-4 over the least fp16
+constexpr float FACTOR_ROOM = 16.f;
 
 template <typename T> constexpr bool FACTORED = std::is_same<T, _Float16>::value;
 
@@ -1119,11 +1126,15 @@ void dq_kernel(const Args a, const Ranges keys, const Ranges queries, int tiles_
     for (int n = 0; n < DP / 32; ++n) acc[n] = acc16{}, mean[n] = acc16{};
     float off = there ? usable(a.lse[at_row]) : INFINITY, rest = 0, factor = 1.f;
     if constexpr (FACTORED<T>) {
-        most = wave_max(most);
-        factor = most == 0.f ? 1.f : exp2f(-4.f - ceilf(log2f(most)));
+        const float largest = wave_max(most);
+        auto factor_of = [](float x) {
+            return x == 0.f ? MOST_FACTOR : exp2f(-4.f - ceilf(log2f(x)));
+        };
+        factor = factor_of(max_halves(most));
         off -= SHIFT;
         if (lane == 0 && row0 < a.sq)
-            factors[((int64_t)b * a.hq + h) * factors_n + row0 / FACTOR_ROWS] = factor;
+            factors[((int64_t)b * a.hq + h) * factors_n + row0 / FACTOR_ROWS] =
+                factor_of(largest);
     }
 
     const int seen = there ? doc_row ? doc_row[pos] : 0 : -1;
@@ -1358,8 +1369,8 @@ void dkv_kernel(const Args a, const Ranges keys, const Ranges queries, int tiles
             const bool by_document = !(visits.whole & bit);
             const bool by_position = a.causal && at + first < wave_last;
             if constexpr (FACTORED<T>) {
-                // larger gradients than before: dk's sums go to their factor
-                if (!begun || tile_factor < factor) {
+                // dk's sums go to the factor of gradients of another size
+                if (!begun || tile_factor < factor || tile_factor > factor * FACTOR_ROOM) {
                     float by = begun ? tile_factor / factor : 1.f;
 #pragma unroll
                     for (int n = 0; n < DP / 32; ++n)

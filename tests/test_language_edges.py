@@ -76,3 +76,63 @@ def test_tracing_on_the_cpu():
         traced = torch.jit.trace(call, inputs)
         other = tuple(x * 0.5 for x in inputs)
         assert torch.equal(traced(*other), call(*other))
+
+
+# --------------------------------------------------------------------------
+# gradients of all sizes in 16 bits
+# --------------------------------------------------------------------------
+
+def relative_error(got, want):
+    return ((got.detach().double().cpu() - want).norm() / want.norm()).item()
+
+
+# P, dS and the result are rounded to half a step each; the errors of thousands
+# of pairs are independent, so that they add up as the sums themselves do
+THREE_ROUNDINGS = 3 * half_step(torch.float16)
+
+
+def small_gradient(name, sizes, documents=None):
+    """The gradient of leaf `name`, fp16, and its value in 64 bits: one head
+    with dout of `sizes`, one for each query, and the leaf itself so small that
+    its gradient, with a scale that makes up for it, is not."""
+    n = len(sizes)
+    x = dict(zip(("q", "k", "v", "dout"),
+                 attention_inputs(1, n, n, 1, 1, 64, torch.float32, "cuda")))
+    x["dout"] = x["dout"] * sizes.cuda().view(1, n, 1, 1)
+    x[name] = x[name] * 2.0 ** -16
+    q, k, v, dout = (t.half() for t in x.values())
+    leaves = {"q": q.requires_grad_(True), "k": k.requires_grad_(True)}
+    out = ops.attention(q, k, v, documents=documents, scale=2.0 ** 13)
+    (got,) = torch.autograd.grad(out, leaves[name], dout)
+    return got, attention_oracle(q, k, v, documents, None, False, 2.0 ** 13, dout)["d" + name][0]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["q", "k"])
+@pytest.mark.parametrize("zeros", ["front", "between", "none"])
+def test_queries_without_a_gradient_cost_no_bits(name, zeros):
+    """Small gradients beside queries that have none, such as unscored tokens."""
+    sizes = torch.full((4096,), 3e-7)
+    if zeros == "front":
+        sizes[:64] = 0
+    if zeros == "between":
+        sizes.view(-1, 256)[:, 100:200] = 0
+    assert relative_error(*small_gradient(name, sizes)) <= THREE_ROUNDINGS
+
+
+@pytest.mark.gpu
+def test_gradients_of_other_sizes():
+    """A document whose gradients are 300000 times those of the next, which begins
+    inside a tile; and queries of both sizes in turn."""
+    n, edge, tile = 2400, 200, 256
+    sizes = torch.full((n,), 3e-7)
+    sizes[:edge], sizes[edge:tile] = 0.1, 0
+    documents = torch.tensor([pack([edge, n - edge], n)], dtype=torch.int32, device="cuda")
+    got, want = small_gradient("k", sizes, documents)
+    assert relative_error(got[:, :edge], want[:, :edge]) <= THREE_ROUNDINGS
+    assert relative_error(got[:, edge:], want[:, edge:]) <= THREE_ROUNDINGS
+    sizes = torch.full((n,), 3e-7)
+    sizes[::2] = 0.1
+    got, want = small_gradient("q", sizes)
+    assert relative_error(got[:, ::2], want[:, ::2]) <= THREE_ROUNDINGS
+    assert relative_error(got[:, 1::2], want[:, 1::2]) <= THREE_ROUNDINGS
