@@ -62,7 +62,6 @@ class BertBase(nn.Module):
             raise ValueError(f"positions must be 'learned', 'rotary' or 'distance', "
                              f"got {positions!r}")
         self.positions, self.heads, self.max_len = positions, heads, max_len
-        self._constants = {}  # rotary frequencies and slopes by device, not part of the state
         self.tok = nn.Embedding(vocab, hidden)
         if positions == "learned":
             self.pos = nn.Embedding(max_len, hidden)
@@ -70,6 +69,16 @@ class BertBase(nn.Module):
         self.layers = nn.ModuleList(EncoderLayer(hidden, heads, ffn) for _ in range(layers))
         self.head = nn.Linear(hidden, vocab, bias=False)
         self.head.weight = self.tok.weight  # tied
+        # rotary frequencies or slopes by device, not part of the state: they
+        # keep their type whatever the parameters are cast to
+        self._constants = {}
+        self._constant(self.tok.weight.device)
+
+    def _apply(self, fn, recurse=True):
+        super()._apply(fn, recurse)
+        # made where the model moves to, so that no captured call has to
+        self._constant(self.tok.weight.device)
+        return self
 
     def forward(self, ids: torch.Tensor, documents: torch.Tensor | None = None) -> torch.Tensor:
         """documents: int32 [B, S] for packed rows, the document of each token
@@ -92,12 +101,15 @@ class BertBase(nn.Module):
             x = layer(x, documents, rotary, slopes)
         return self.head(x)
 
+    @torch.inference_mode(False)  # constants made in an evaluation serve training too
     def _constant(self, device):
+        if self.positions == "learned" or device.type == "meta":
+            return None
         if device not in self._constants:
             if self.positions == "rotary":
                 value = ops.rotary_frequencies(self.tok.embedding_dim // self.heads)
             else:  # slopes from 1/2 to 2^-8 or so, each head's a fixed part of the last
                 value = torch.tensor([2.0 ** (-8.0 * (h + 1) / self.heads)
-                                      for h in range(self.heads)])
+                                      for h in range(self.heads)], dtype=torch.float32)
             self._constants[device] = value.to(device)
         return self._constants[device]
