@@ -1303,8 +1303,7 @@ void dkv_kernel(const Args a, const Ranges keys, const Ranges queries, int tiles
     acc16 dk[DP / 32], dv[DP / 32];
 #pragma unroll
     for (int n = 0; n < DP / 32; ++n) dk[n] = acc16{}, dv[n] = acc16{};
-    float factor = 1.f;  // what dk's sums have
-    bool begun = false;
+    float factor = 0.f;  // what dk's sums have, 0 before the first tile
 
     const int seen = there ? doc_row ? doc_row[j] : 0 : -1;
     const int doc = seen < 0 ? INT_MIN : seen;
@@ -1370,14 +1369,13 @@ void dkv_kernel(const Args a, const Ranges keys, const Ranges queries, int tiles
             const bool by_position = a.causal && at + first < wave_last;
             if constexpr (FACTORED<T>) {
                 // dk's sums go to the factor of gradients of another size
-                if (!begun || tile_factor < factor || tile_factor > factor * FACTOR_ROOM) {
-                    float by = begun ? tile_factor / factor : 1.f;
+                if (fminf(fmaxf(tile_factor, factor), factor * FACTOR_ROOM) != tile_factor) {
+                    float by = factor == 0.f ? 1.f : tile_factor / factor;
 #pragma unroll
                     for (int n = 0; n < DP / 32; ++n)
 #pragma unroll
                         for (int e = 0; e < 16; ++e) dk[n][e] *= by;
                     factor = tile_factor;
-                    begun = true;
                 }
             }
             const float slope = slope_of(a, h), far = (float)(at + first + 4 * hf - j);
@@ -1421,7 +1419,7 @@ void dkv_kernel(const Args a, const Ranges keys, const Ranges queries, int tiles
     float back_k = a.scale, back_v = 1.f;
     if constexpr (FACTORED<T>) {
         back_v = exp2f(-SHIFT);
-        back_k *= back_v / factor;
+        back_k *= factor == 0.f ? 0.f : back_v / factor;
     }
 #pragma unroll
     for (int n = 0; n < DP / 32; ++n)
