@@ -194,17 +194,24 @@ __global__ __launch_bounds__(1024) void norm_join_kernel(const double* __restric
     if (threadIdx.x == 0) *norm = (float)sqrt(s);
 }
 
-// x * factor, rounded once: a 32-bit product of 64-bit factors is exact before
-// its rounding; for the 16-bit types the factor's 32-bit rounding adds 2^-24
-// to a step of 2^-8 or 2^-11.
-template <int OUT>
+// x * factor as OUT holds it: a 64-bit product (off by 2^-53), rounded.  For the
+// 16-bit types a factor and a product of 32 bits serve, which add 2^-23 to half
+// a step of 2^-8 or 2^-11, where the factor is a normal number (151 M values of
+// fp16 take 173 us so, 254 with 64 bits).  Gradients near the largest value put
+// it below 2^-126, 100 values of 3e38 cut to a norm of 1e-6 at 3e-46: then their
+// products have 64 bits as well.
+template <bool WIDE> __device__ __forceinline__ float scaled(float x, double factor) {
+    return WIDE ? (float)((double)x * factor) : x * (float)factor;
+}
+
+template <int OUT, bool WIDE>
 __device__ __forceinline__ void put(void* out, int64_t i, double factor, float x) {
     if (OUT == F32) {
-        ((float*)out)[i] = (float)((double)x * factor);
+        ((float*)out)[i] = scaled<true>(x, factor);
     } else if (OUT == BF16) {
-        ((uint16_t*)out)[i] = to_bf16(x * (float)factor);
+        ((uint16_t*)out)[i] = to_bf16(scaled<WIDE>(x, factor));
     } else {
-        ((_Float16*)out)[i] = (_Float16)(x * (float)factor);
+        ((_Float16*)out)[i] = (_Float16)scaled<WIDE>(x, factor);
     }
 }
 
@@ -219,16 +226,15 @@ __device__ __forceinline__ void put_vec(Raw* out, int64_t i, double factor, raw4
 #pragma unroll
             for (int e = 0; e < 4; ++e)
                 o[e] = __float_as_uint(
-                    (float)((double)Type<IN>::get((const uint32_t*)&r, h * 4 + e) * factor));
+                    scaled<true>(Type<IN>::get((const uint32_t*)&r, h * 4 + e), factor));
             out[i * (PER / 4) + h].v = o;
         }
     } else {
         uint32_t w[PER / 2];
-        float f = (float)factor;
 #pragma unroll
         for (int e = 0; e < PER / 2; ++e) {
-            float a = Type<IN>::get((const uint32_t*)&r, 2 * e) * f;
-            float b = Type<IN>::get((const uint32_t*)&r, 2 * e + 1) * f;
+            const float a = scaled<false>(Type<IN>::get((const uint32_t*)&r, 2 * e), factor);
+            const float b = scaled<false>(Type<IN>::get((const uint32_t*)&r, 2 * e + 1), factor);
             uint16_t u, v;
             if constexpr (OUT == BF16) {
                 u = to_bf16(a), v = to_bf16(b);
@@ -254,7 +260,7 @@ __device__ void chunk_scale(const void* in, void* out, int n, double factor) {
     constexpr int PER = Type<IN>::PER, SIZE = IN == F32 ? 4 : 2, TO = OUT == F32 ? 4 : 2;
     const int head = head_of(out, TO, n);  // stores at 16-byte addresses, loads at any
     if ((int)threadIdx.x < head)
-        put<OUT>(out, threadIdx.x, factor, Type<IN>::load(in, threadIdx.x));
+        put<OUT, OUT == F32>(out, threadIdx.x, factor, Type<IN>::load(in, threadIdx.x));
     in = (const char*)in + head * SIZE;
     out = (char*)out + head * TO;
     n -= head;
@@ -270,7 +276,15 @@ __device__ void chunk_scale(const void* in, void* out, int n, double factor) {
     }
     for (; i < vecs; i += THREADS) put_vec<IN, OUT>((Raw*)out, i, factor, raw[i].v);
     for (i = vecs * PER + threadIdx.x; i < n; i += THREADS)
-        put<OUT>(out, i, factor, Type<IN>::load(in, i));
+        put<OUT, OUT == F32>(out, i, factor, Type<IN>::load(in, i));
+}
+
+// value by value, in 64 bits
+template <int IN, int OUT>
+__device__ void chunk_scale_wide(const void* in, void* out, int n, double factor) {
+#pragma unroll 1
+    for (int i = threadIdx.x; i < n; i += THREADS)
+        put<OUT, true>(out, i, factor, Type<IN>::load(in, i));
 }
 
 __global__ __launch_bounds__(THREADS) void clip_kernel(const Table t,
@@ -286,17 +300,20 @@ __global__ __launch_bounds__(THREADS) void clip_kernel(const Table t,
     // a NaN norm is no norm below the bound: it reaches every value
     double factor = total <= max_norm ? 1.0 : max_norm / total;
     if (c.in == c.out && factor == 1.0) return;  // in place and under the bound
-    switch (c.from * 3 + c.to) {
-        case 0: chunk_scale<F32, F32>(c.in, c.out, c.n, factor); break;
-        case 1: chunk_scale<F32, BF16>(c.in, c.out, c.n, factor); break;
-        case 2: chunk_scale<F32, F16>(c.in, c.out, c.n, factor); break;
-        case 3: chunk_scale<BF16, F32>(c.in, c.out, c.n, factor); break;
-        case 4: chunk_scale<BF16, BF16>(c.in, c.out, c.n, factor); break;
-        case 5: chunk_scale<BF16, F16>(c.in, c.out, c.n, factor); break;
-        case 6: chunk_scale<F16, F32>(c.in, c.out, c.n, factor); break;
-        case 7: chunk_scale<F16, BF16>(c.in, c.out, c.n, factor); break;
-        default: chunk_scale<F16, F16>(c.in, c.out, c.n, factor); break;
-    }
+    const bool wide = factor < 0x1p-126;
+    auto scale = [&](auto in, auto out) {
+        constexpr int IN = decltype(in)::value, OUT = decltype(out)::value;
+        if (OUT != F32 && wide)
+            chunk_scale_wide<IN, OUT>(c.in, c.out, c.n, factor);
+        else
+            chunk_scale<IN, OUT>(c.in, c.out, c.n, factor);
+    };
+    auto for_kind = [](int kind, auto f) {
+        if (kind == F32) f(std::integral_constant<int, F32>{});
+        else if (kind == BF16) f(std::integral_constant<int, BF16>{});
+        else f(std::integral_constant<int, F16>{});
+    };
+    for_kind(c.from, [&](auto in) { for_kind(c.to, [&](auto out) { scale(in, out); }); });
 }
 
 Kind kind_of(const torch::Tensor& t) {

@@ -136,3 +136,28 @@ def test_gradients_of_other_sizes():
     got, want = small_gradient("q", sizes)
     assert relative_error(got[:, ::2], want[:, ::2]) <= THREE_ROUNDINGS
     assert relative_error(got[:, 1::2], want[:, 1::2]) <= THREE_ROUNDINGS
+
+
+# --------------------------------------------------------------------------
+# clipping
+# --------------------------------------------------------------------------
+
+@pytest.mark.parametrize("device", BOTH)
+@pytest.mark.parametrize("to", TYPES, ids=str)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("count,bound", [(100, 1e-3), (100, 1e-6), (40_001, 1e-5), (3, 1e30)])
+def test_clip_of_exploding_gradients(device, dtype, to, count, bound):
+    """Factors that 32 bits hold as subnormal numbers or not at all."""
+    gen = torch.Generator().manual_seed(count)
+    x = (3e38 * (0.5 + 0.5 * torch.rand(count, generator=gen))).to(dtype)
+    norm = math.sqrt(math.fsum((x.double() ** 2).tolist()))
+    (y,), n = ops.clip_grad_norm([x.to(device)], bound, dtype=to)
+    assert n.isinf() == (norm > torch.finfo(torch.float32).max)
+    want = x.double() * (bound / norm)
+    if bound > torch.finfo(to).max:
+        assert y.isinf().all()
+        return
+    # rounded to 32 bits and to the type; below its normal numbers a fixed half step
+    info = torch.finfo(to)
+    least = info.tiny * info.eps / 2
+    assert_within(y, want, want.abs() * (half_step(to) + 2 * E) + least * 1.001, "clipped")
