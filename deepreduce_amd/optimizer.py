@@ -24,7 +24,8 @@ params['clip_norm'] bounds the global gradient norm, by ops.clip_grad_norm_
   * 'local' (default): each rank's own gradients, before they enter the
     residual memory, where an outlier would otherwise stay;
   * 'reduced': the exchanged gradients, which are the same on every rank.
-The norm before clipping is left in `grc.last_grad_norm`, on the device.
+The norm before clipping is left in `grc.last_grad_norm`, on the device, a
+tensor of its own for each step.
 """
 from __future__ import annotations
 
@@ -144,6 +145,7 @@ class DistributedOptimizer:
         self._graph_warmup = max(2, graph_warmup)  # residuals must exist
         self._use_graph = use_graph if use_graph is not None else _graph_safe(grc)
         self._graph_wire_bytes = 0
+        self._graph_norm = None  # what the captured exchange writes its gradient norm to
 
     def zero_grad(self, set_to_none: bool = True):
         if not set_to_none:
@@ -172,8 +174,7 @@ class DistributedOptimizer:
                     self.last_wire_bytes = reduce_gradients(self.model, self.grc)
                     return
             else:
-                self._graph.replay()
-                self.last_wire_bytes = self._graph_wire_bytes
+                self._replay(self._graph)
                 return
         self._graph_calls += 1
         if self._graph_calls <= self._graph_warmup:
@@ -201,18 +202,25 @@ class DistributedOptimizer:
             g = torch.cuda.CUDAGraph()
             with torch.cuda.graph(g):
                 self._graph_wire_bytes = reduce_gradients(self.model, self.grc)
+            self._graph_norm = self.last_grad_norm
             # capture RECORDS without executing: replay once so this step's
             # exchange actually happens (on the restored, pristine grads —
             # exactly one compress + one residual update this step)
-            g.replay()
+            self._replay(g)
             self._graph = g
             self._graph_grad_ptrs = self._grad_ptrs()
-            self.last_wire_bytes = self._graph_wire_bytes
         except Exception:
             self._use_graph = False
             self._graph = None
             torch.cuda.synchronize()
             self.last_wire_bytes = reduce_gradients(self.model, self.grc)
+
+    def _replay(self, graph):
+        graph.replay()
+        self.last_wire_bytes = self._graph_wire_bytes
+        if self._graph_norm is not None:
+            # a tensor of this step's own: the next replay overwrites the graph's
+            self.grc.last_grad_norm = self._graph_norm.clone()
 
     def _snapshot_state(self):
         """Clone p.grad buffers and residual-memory tensors (pre-warmup)."""

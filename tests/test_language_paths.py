@@ -59,3 +59,36 @@ def test_bert_constants(device, positions):
     with torch.device("meta"):
         empty = tiny_bert(positions, "meta")
     assert at in empty.to_empty(device=device)._constants
+
+
+# --------------------------------------------------------------------------
+# clipping around the exchange
+# --------------------------------------------------------------------------
+
+@pytest.mark.parametrize("device", BOTH)
+@pytest.mark.parametrize("stage", ["local", "reduced"])
+def test_norms_of_steps_stay(device, stage):
+    """Norms that are collected without a synchronisation and read at the end,
+    before and after the exchange is captured."""
+    gen = torch.Generator().manual_seed(6)
+    torch.manual_seed(6)
+    model = torch.nn.Linear(60, 40).to(device)
+    opt = dr.DistributedOptimizer(torch.optim.SGD(model.parameters(), lr=0.0),
+                                  make_grc(clip_norm=1e-3, clip_stage=stage,
+                                           memory="none"), model)
+    norms, want = [], []
+    for step in range(9):
+        x = torch.randn(5, 60, generator=gen).to(device)
+        opt.zero_grad(set_to_none=False)
+        (model(x).sum() * 2 ** step).backward()
+        if stage == "local":
+            want.append(global_norm(p.grad for p in model.parameters()))
+        opt.step()
+        norms.append(opt.last_grad_norm)
+        if stage == "reduced":
+            want.append(norms[-1].item())
+    assert (opt._graph is not None) == (device == "cuda")
+    assert len({n.data_ptr() for n in norms}) == len(norms)
+    for a, c in zip(norms, want):
+        assert abs(a.item() - c) <= 1e-6 * c
+    assert norms[-1].item() > 50 * norms[0].item()
