@@ -34,6 +34,7 @@ import os
 import torch
 
 from .ops import clip_grad_norm_
+from .ops.language import TYPES
 
 __all__ = ["reduce_gradients", "DistributedOptimizer"]
 
@@ -70,7 +71,7 @@ def reduce_gradients(model: torch.nn.Module, grc, names=None, fused: bool = True
             p.grad.data.copy_(reduced.view_as(p.grad.data))
             total_bytes += getattr(grc, "last_wire_bytes", 0)
     if clip is not None and stage == "reduced" and params:
-        grc.last_grad_norm = clip_grad_norm_([p.grad.data for _, p in params], clip)
+        grc.last_grad_norm = clip_reduced([p.grad.data for _, p in params], clip)
     return total_bytes
 
 
@@ -78,6 +79,17 @@ def clip_options(grc):
     """(clip_norm or None, clip_stage) of a communicator's params."""
     params = getattr(grc, "params", None) or {}
     return params.get("clip_norm"), params.get("clip_stage", "local")
+
+
+def clip_reduced(grads, bound: float):
+    """clip_grad_norm_ of exchanged gradients of any type: the exchange is in 32
+    bits, so those that hold more lose nothing on the way."""
+    parts = [g if g.dtype in TYPES else g.float() for g in grads]
+    norm = clip_grad_norm_(parts, bound)
+    for g, part in zip(grads, parts):
+        if part is not g:
+            g.copy_(part)
+    return norm
 
 
 def _graph_safe(grc) -> bool:

@@ -28,8 +28,7 @@ from __future__ import annotations
 import torch
 import torch.distributed as dist
 
-from ..ops import clip_grad_norm_
-from ..optimizer import clip_options
+from ..optimizer import clip_options, clip_reduced
 
 __all__ = ["OverlappedReducer"]
 
@@ -220,7 +219,7 @@ class OverlappedReducer:
         if self._clip_norm is not None:
             grads = [p.grad.data for p in self.model.parameters() if p.grad is not None]
             if grads:
-                grc.last_grad_norm = clip_grad_norm_(grads, self._clip_norm)
+                grc.last_grad_norm = clip_reduced(grads, self._clip_norm)
 
     def _exchange_small(self, world):
         if not self._small:

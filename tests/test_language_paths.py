@@ -9,6 +9,7 @@ import torch
 
 import deepreduce_amd as dr
 from deepreduce_amd import ops
+from deepreduce_amd.parallel import OverlappedReducer
 from test_language_training import BOTH, POSITIONS, global_norm, make_grc, tiny_bert
 
 
@@ -92,3 +93,33 @@ def test_norms_of_steps_stay(device, stage):
     for a, c in zip(norms, want):
         assert abs(a.item() - c) <= 1e-6 * c
     assert norms[-1].item() > 50 * norms[0].item()
+
+
+@pytest.mark.parametrize("device", BOTH)
+@pytest.mark.parametrize("dtype", [torch.float64, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("way", ["local", "reduced", "overlapped"])
+def test_clip_of_parameters_of_other_types(device, dtype, way):
+    """Parameters in 64 and 16 bits beside some in 32 clip at every stage."""
+    from deepreduce_amd.optimizer import reduce_gradients
+
+    torch.manual_seed(7)
+    model = torch.nn.Sequential(torch.nn.Linear(40, 60), torch.nn.Linear(60, 50)).to(device)
+    model[1].to(dtype)
+    grc = dr.deepreduce_from_params({
+        "compressor": "none", "memory": "none", "communicator": "allgather", "clip_norm": 0.25,
+        "clip_stage": "local" if way == "local" else "reduced"})
+    reducer = OverlappedReducer(model, grc) if way == "overlapped" else None
+    x = torch.randn(8, 40, device=device)
+    model[1](model[0](x).to(dtype)).float().square().sum().backward()
+    before = [p.grad.double().clone() for p in model.parameters()]
+    if reducer:
+        reducer.finalize()
+    else:
+        reduce_gradients(model, grc)
+    norm = global_norm(before)
+    # a gradient is rounded to its type once or twice
+    u = torch.finfo(dtype).eps if dtype == torch.bfloat16 else 2.0 ** -22
+    assert norm > 1 and abs(grc.last_grad_norm.item() - norm) <= u * norm
+    for p, b in zip(model.parameters(), before):
+        assert p.grad.dtype == p.dtype
+        assert (p.grad.double() - b * 0.25 / norm).abs().max() <= u * 0.25
