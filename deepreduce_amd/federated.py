@@ -23,6 +23,13 @@ from .memory import ResidualMemory
 from .ops import clip_grad_norm_
 
 
+def clip_local_step(model: torch.nn.Module, clip_norm: float | None) -> None:
+    """Bounds the global norm of the gradients that a local step left, if any."""
+    grads = [p.grad for p in model.parameters() if p.grad is not None]
+    if clip_norm is not None and grads:
+        clip_grad_norm_(grads, clip_norm)
+
+
 class FederatedServer:
     def __init__(self, model: torch.nn.Module, compressor, lr: float = 1.0):
         self.model = model
@@ -89,9 +96,7 @@ class FederatedClient:
             for x, y in data_iter():
                 opt.zero_grad()
                 loss_fn(model(x), y).backward()
-                if self.clip_norm is not None:
-                    clip_grad_norm_([p.grad for p in model.parameters() if p.grad is not None],
-                                    self.clip_norm)
+                clip_local_step(model, self.clip_norm)
                 opt.step()
 
         out = {}

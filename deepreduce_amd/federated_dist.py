@@ -24,8 +24,8 @@ import torch
 import torch.distributed as dist
 
 from .communicator import _flatten_payload, _unflatten_payload
+from .federated import clip_local_step
 from .memory import ResidualMemory
-from .ops import clip_grad_norm_
 
 __all__ = ["FederatedDistRunner", "serialize_payloads", "deserialize_payloads"]
 
@@ -168,9 +168,7 @@ class FederatedDistRunner:
                 for x, y in data_iter():
                     opt.zero_grad()
                     loss_fn(local(x), y).backward()
-                    if self.clip_norm is not None:
-                        clip_grad_norm_([p.grad for p in local.parameters()
-                                         if p.grad is not None], self.clip_norm)
+                    clip_local_step(local, self.clip_norm)
                     opt.step()
             out = {}
             for n, p in local.named_parameters():

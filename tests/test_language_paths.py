@@ -123,3 +123,28 @@ def test_clip_of_parameters_of_other_types(device, dtype, way):
     for p, b in zip(model.parameters(), before):
         assert p.grad.dtype == p.dtype
         assert (p.grad.double() - b * 0.25 / norm).abs().max() <= u * 0.25
+
+
+# --------------------------------------------------------------------------
+# federated clients and several ranks
+# --------------------------------------------------------------------------
+
+def test_federated_step_without_gradients():
+    """A step that leaves no parameter a gradient has nothing to clip."""
+    from deepreduce_amd.federated import FederatedClient, FederatedServer
+
+    torch.manual_seed(8)
+    compressor = make_grc().compressor
+    model = torch.nn.Linear(30, 20)
+    for p in model.parameters():
+        p.requires_grad_(False)
+    x = torch.randn(4, 30, requires_grad=True)
+    sent = []
+    for bound in (None, 0.1):
+        server = FederatedServer(model, compressor)
+        client = FederatedClient(model, compressor, clip_norm=bound)
+        sent.append(client.round(server.broadcast_payload(), lambda: [(x, None)],
+                                 loss_fn=lambda out, y: out.square().sum()))
+    for name, (payload, _) in sent[0].items():
+        for a, c in zip(payload, sent[1][name][0]):
+            assert torch.equal(a, c)
