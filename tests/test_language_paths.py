@@ -148,3 +148,148 @@ def test_federated_step_without_gradients():
     for name, (payload, _) in sent[0].items():
         for a, c in zip(payload, sent[1][name][0]):
             assert torch.equal(a, c)
+
+
+def rank_main(rank, world, port, work, queue):
+    """Runs work(rank) in a process group over the loopback address."""
+    import os
+    import traceback
+
+    import torch.distributed as dist
+
+    os.environ.update(MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port))
+    torch.set_num_threads(1)
+    try:
+        dist.init_process_group("gloo", rank=rank, world_size=world)
+        queue.put((rank, work(rank), None))
+        dist.barrier()
+        dist.destroy_process_group()
+    except Exception:  # noqa: BLE001
+        queue.put((rank, None, traceback.format_exc()[-1500:]))
+
+
+def run_ranks(world, work):
+    """What work(rank) returned (plain values) on each of `world` ranks."""
+    import socket
+
+    import torch.multiprocessing as mp
+
+    with socket.socket() as s:
+        s.bind(("127.0.0.1", 0))
+        port = s.getsockname()[1]
+    ctx = mp.get_context("spawn")
+    queue = ctx.Queue()
+    procs = [ctx.Process(target=rank_main, args=(r, world, port, work, queue))
+             for r in range(world)]
+    for p in procs:
+        p.start()
+    results = {}
+    for _ in procs:
+        rank, value, error = queue.get(timeout=240)
+        assert error is None, error
+        results[rank] = value
+    for p in procs:
+        p.join(timeout=60)
+    return [results[r] for r in range(world)]
+
+
+def clipped_exchange(rank, stage, way):
+    """[largest deviation from clipping by hand, this rank's norm, the norm
+    that the first step should have], after two steps on this rank's data."""
+    from deepreduce_amd.optimizer import reduce_gradients
+
+    torch.manual_seed(9)
+    bound = 0.5
+    models = [torch.nn.Sequential(torch.nn.Linear(60, 80), torch.nn.Tanh(),
+                                  torch.nn.Linear(80, 50)) for _ in range(2)]
+    models[1].load_state_dict(models[0].state_dict())
+    grcs = [make_grc(clip_norm=bound, clip_stage=stage), make_grc()]
+    reducers = [OverlappedReducer(m, g) for m, g in zip(models, grcs)] if way == "overlapped" \
+        else [None, None]
+    gen = torch.Generator().manual_seed(100 + rank)
+    worst, norms = 0.0, []
+    for step in range(2):
+        x = torch.randn(16, 60, generator=gen)
+        for model in models:
+            model.zero_grad()
+            (model(x) ** 2).sum().backward()
+        grads = [p.grad for p in models[1].parameters()]
+
+        def by_hand():
+            norm = global_norm(grads)
+            for g in grads:
+                g.mul_(min(1.0, bound / norm))
+            return norm
+
+        before = by_hand() if stage == "local" else None
+        for model, grc, reducer in zip(reversed(models), reversed(grcs), reversed(reducers)):
+            if reducer:
+                reducer.finalize()
+            else:
+                reduce_gradients(model, grc, fused=way == "fused")
+        before = by_hand() if stage == "reduced" else before
+        norms.append((grcs[0].last_grad_norm.item(), before))
+        for p, q in zip(models[0].parameters(), models[1].parameters()):
+            worst = max(worst, (p.grad - q.grad).abs().max().item())
+    return worst, norms
+
+
+def local_fused(rank):
+    return clipped_exchange(rank, "local", "fused")
+
+
+def local_by_tensor(rank):
+    return clipped_exchange(rank, "local", "by tensor")
+
+
+def reduced_fused(rank):
+    return clipped_exchange(rank, "reduced", "fused")
+
+
+def reduced_overlapped(rank):
+    return clipped_exchange(rank, "reduced", "overlapped")
+
+
+@pytest.mark.timeout(300)
+@pytest.mark.parametrize("work", [local_fused, local_by_tensor, reduced_fused,
+                                  reduced_overlapped], ids=lambda w: w.__name__)
+def test_two_ranks_clip(work):
+    """Each rank its own gradients before the exchange, all the same ones after
+    it, against the same steps clipped by hand."""
+    results = run_ranks(2, work)
+    for worst, norms in results:
+        # a product rounded to 32 bits once more, of values of at most the bound
+        assert worst <= 1e-6 * 0.5
+        for got, want in norms:
+            assert want > 0.5 and abs(got - want) <= 1e-6 * want
+    first, second = ([n for n, _ in r[1]] for r in results)
+    assert (first == second) == work.__name__.startswith("reduced")
+
+
+def federated_rank(rank):
+    """One round of one local step: the norms of what this rank compressed, and
+    of how far the server's model went."""
+    from deepreduce_amd.federated_dist import FederatedDistRunner
+
+    torch.manual_seed(10)
+    model = torch.nn.Linear(30, 10)
+    start = [p.detach().clone() for p in model.parameters()]
+    compressor, seen = make_grc(compress_ratio=1.0).compressor, []
+    compress = compressor.compress
+    compressor.compress = lambda t, n: (seen.append(t.clone()), compress(t, n))[1]
+    runner = FederatedDistRunner(model, compressor, local_lr=0.5, clip_norm=0.1)
+    runner.memory = dr.NoneMemory()
+    gen = torch.Generator().manual_seed(rank)
+    x, y = torch.randn(12, 30, generator=gen) * 50, torch.randint(0, 10, (12,), generator=gen)
+    runner.round(lambda: [(x, y)])
+    moved = [p.detach() - s for p, s in zip(model.parameters(), start)]
+    return global_norm(seen), global_norm(moved)
+
+
+@pytest.mark.timeout(300)
+def test_federated_ranks_clip():
+    (sent, moved), (client, also), (other, _) = run_ranks(3, federated_rank)
+    # what a client sends is its one step's gradient, clipped; 32-bit rounding
+    # of the parameters, of size 0.2 or less, shows in the difference of two
+    assert abs(client - 0.1) <= 1e-4 and abs(other - 0.1) <= 1e-4
+    assert sent == 0 and moved == also and 0 < moved <= 0.1 + 1e-4
