@@ -1001,13 +1001,24 @@ void for_shape(int64_t heads, int length, F f) {
         go(std::integral_constant<int, 1>{}, std::integral_constant<int, 4>{});
 }
 
-// Whether the forward pass is split over the keys: where 32 queries a block
-// give fewer blocks than there are CUs, and the rows to join are fewer than the
-// keys.  12 heads of 64, bf16, split and not: 1 query of 2048 keys 9 and 22 us,
-// 128 of 2048 19 and 22, 512 of 8192 55 and 73, but 512 of 2048 36 and 23.
+// Whether the forward pass is split over the keys, either
+// - where 32 queries a block give fewer blocks than there are CUs, and the rows
+//   to join are fewer than the keys: 12 heads of 64, bf16, split and not: 1
+//   query of 2048 keys 9 and 22 us, 128 of 2048 19 and 22, 512 of 8192 55 and 73,
+//   but 512 of 2048 36 and 23;
+// - or where few queries of many requests leave most of a wave's 32 columns
+//   empty, which the split fills with the heads that share keys.  A tile of 32
+//   x 32 pairs that this saves pays for a row to join, 4096 for the second
+//   launch.  One query, 12 heads on 4 of 64, bf16, split and not: 32 requests of
+//   8192 keys 48 and 111 us, 64 of 2048 30 and 65, but 64 of 128 10 and 9; 16 on 1,
+//   fp32, 32 of 32768 keys 116 and 4520; 16 queries, 16 on 1, bf16, 16 of 2048 29 and
+//   23.
 bool split_keys(const Args& a) {
-    const int64_t heads = (int64_t)a.b * a.hq;
-    return heads * ((a.sq + 31) / 32) < 256 && heads * a.sq <= a.sk;
+    const int64_t heads = (int64_t)a.b * a.hq, rows = heads * a.sq;
+    const int64_t blocks = heads * ((a.sq + 31) / 32);
+    const int64_t packed =
+        (int64_t)a.b * a.hkv * (((int64_t)(a.hq / a.hkv) * a.sq + 31) / 32);
+    return (blocks < 256 && rows <= a.sk) || (blocks - packed) * a.sk / 32 > rows + 4096;
 }
 
 template <typename T, int DP>
@@ -1019,6 +1030,7 @@ void launch_split(const Args& a, const torch::Tensor& like, hipStream_t stream) 
                                        std::max<int64_t>(1, a.sk / 64), MOST_PARTS});
     int64_t each = ((a.sk + parts - 1) / parts + 31) / 32 * 32;
     parts = (a.sk + each - 1) / each;
+    TORCH_CHECK(units * parts <= INT_MAX && rows <= INT_MAX, "too many rows for one launch");
     auto f32 = like.options().dtype(torch::kFloat32);
     auto part_o = torch::empty({rows, parts, DP}, f32), state = torch::empty({rows, parts, 2}, f32);
     hipLaunchKernelGGL((split_kernel<T, DP>), dim3((unsigned)(units * parts)), dim3(64), 0, stream,

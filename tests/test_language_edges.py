@@ -161,3 +161,48 @@ def test_clip_of_exploding_gradients(device, dtype, to, count, bound):
     info = torch.finfo(to)
     least = info.tiny * info.eps / 2
     assert_within(y, want, want.abs() * (half_step(to) + 2 * E) + least * 1.001, "clipped")
+
+
+# --------------------------------------------------------------------------
+# many requests
+# --------------------------------------------------------------------------
+
+def time_of(call):
+    """Seconds of a call among others, the least of three groups."""
+    for _ in range(3):
+        call()
+    least = math.inf
+    for _ in range(3):
+        begin, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        begin.record()
+        for _ in range(5):
+            call()
+        end.record()
+        torch.cuda.synchronize()
+        least = min(least, begin.elapsed_time(end) / 5e3)
+    return least
+
+
+@pytest.mark.gpu
+def test_many_requests_read_their_keys_once():
+    """Heads that share keys read them together at any number of requests: well
+    within the time of a few copies (once a query head takes 20 copies)."""
+    q = torch.randn(32, 1, 16, 64, device="cuda")
+    k, v = (torch.randn(32, 32768, 1, 64, device="cuda") for _ in range(2))
+    copies = time_of(lambda: (k.clone(), v.clone()))
+    assert time_of(lambda: ops.attention(q, k, v)) <= 4 * copies
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("shape", [(64, 1, 700, 12, 4, 64), (40, 2, 601, 16, 1, 128),
+                                   (600, 1, 300, 3, 1, 32), (33, 5, 1111, 16, 2, 40)], ids=str)
+def test_many_requests(dtype, shape):
+    b, sq, sk, hq, hkv, d = shape
+    q, k, v, dout = attention_inputs(*shape, dtype, "cuda", seed=sum(shape))
+    lengths = torch.randint(0, sk, (b,), generator=torch.Generator().manual_seed(b))
+    documents = torch.tensor([pack([n], sk) for n in lengths], dtype=torch.int32)
+    documents[::3] = 4  # whole caches, and padding behind the others
+    slopes = torch.linspace(0.05, 0.0, hq, device="cuda")
+    check_attention(q, k, v, dout, documents.cuda(), slopes, causal=True)
+    check_attention(q, k, v, dout, causal=sq > 1)
