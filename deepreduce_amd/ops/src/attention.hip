@@ -74,12 +74,53 @@ __device__ __forceinline__ bool visible(const Args& a, int b, int pos, int j) {
     return true;
 }
 
+// rows start at 16-byte addresses and d is a multiple of 8
 template <typename T>
 __device__ __forceinline__ float dot(const T* x, const T* y, int d) {
+    typedef T Vec __attribute__((ext_vector_type(16 / sizeof(T))));
     float s = 0;
-    for (int i = 0; i < d; ++i) s = fmaf((float)x[i], (float)y[i], s);
+#pragma unroll 4
+    for (int i = 0; i < d; i += 16 / sizeof(T)) {
+        const Vec u = *(const Vec*)(x + i), v = *(const Vec*)(y + i);
+#pragma unroll
+        for (int e = 0; e < (int)(16 / sizeof(T)); ++e) s = fmaf((float)u[e], (float)v[e], s);
+    }
     return s;
 }
+
+// A weighted sum of rows of up to DP values, of which a lane holds 16 bytes'
+// worth and CHUNKS lanes a row: 64 / CHUNKS rows are read at a time.
+template <typename T, int DP> struct RowSum {
+    static constexpr int PER = 16 / sizeof(T), VECS = DP / PER;
+    static constexpr int CHUNKS = VECS <= 4 ? 4 : VECS <= 8 ? 8 : VECS <= 16 ? 16 : 32;
+    typedef T Vec __attribute__((ext_vector_type(PER)));
+    float x[PER] = {};
+
+    // w of lane n times row_of(n) for the lanes n in `any`; others' rows are not read
+    template <typename R>
+    __device__ __forceinline__ void add(float w, uint64_t any, int d, R row_of) {
+        const int lane = threadIdx.x & 63, c = (lane % CHUNKS) * PER;
+#pragma unroll 4
+        for (int n = 0; n < CHUNKS; ++n) {
+            const int r = n * (64 / CHUNKS) + lane / CHUNKS;
+            const float by = __shfl(w, r);
+            if (!(any >> r & 1) || c >= d) continue;
+            const Vec v = *(const Vec*)(row_of(r) + c);
+#pragma unroll
+            for (int e = 0; e < PER; ++e) x[e] = fmaf(by, (float)v[e], x[e]);
+        }
+    }
+    __device__ __forceinline__ void store(T* to, int d, float scale) {
+        const int lane = threadIdx.x & 63, c = (lane % CHUNKS) * PER;
+        Vec v;
+#pragma unroll
+        for (int e = 0; e < PER; ++e) {
+            for (int m = CHUNKS; m < 64; m <<= 1) x[e] += __shfl_xor(x[e], m);
+            v[e] = (T)(x[e] * scale);
+        }
+        if (lane < CHUNKS && c < d) *(Vec*)(to + c) = v;
+    }
+};
 
 __device__ __forceinline__ float slope_of(const Args& a, int h) {
     return a.slopes ? a.slopes[h] * LOG2E : 0.f;
@@ -92,7 +133,7 @@ __device__ __forceinline__ float slope_of(const Args& a, int h) {
 // there.
 // ---------------------------------------------------------------------------
 
-template <typename T>
+template <typename T, int DP>
 __device__ void forward_row(const Args& a, int b, int h, int i) {
     const int lane = threadIdx.x & 63, g = h / (a.hq / a.hkv), pos = i + a.sk - a.sq;
     const float slope = slope_of(a, h);
@@ -115,35 +156,28 @@ __device__ void forward_row(const Args& a, int b, int h, int i) {
     base = base == -INFINITY ? 0.f : base;
     total = wave_sum(total * exp2_fast(top - base));
     const float inv = total == 0.f ? 0.f : 1.f / total;
-    float o[2] = {0, 0};
+    RowSum<T, DP> o;
     for (int j0 = 0; j0 < end; j0 += 64) {
         int j = j0 + lane;
         bool seen = j < end && visible(a, b, pos, j);
         float p = seen ? exp2_fast(score(j) - base) * inv : 0.f;
-        for (uint64_t any = __ballot(seen); any; any &= any - 1) {
-            int n = __builtin_ctzll(any);
-            float w = __shfl(p, n);
-            const T* v = row<T>(a.v, b, j0 + n, g);
-            if (lane < a.d) o[0] = fmaf(w, (float)v[lane], o[0]);
-            if (lane + 64 < a.d) o[1] = fmaf(w, (float)v[lane + 64], o[1]);
-        }
+        o.add(p, __ballot(seen), a.d, [&](int n) { return row<T>(a.v, b, j0 + n, g); });
     }
-    T* out = row<T>(a.out, b, i, h);
-    if (lane < a.d) out[lane] = (T)o[0];
-    if (lane + 64 < a.d) out[lane + 64] = (T)o[1];
+    o.store(row<T>(a.out, b, i, h), a.d, 1.f);
     if (lane == 0 && a.lse)
         a.lse[((int64_t)b * a.hq + h) * a.sq + i] = total == 0.f ? -INFINITY : base + log2f(total);
 }
 
 // also leaves the row's delta, from probabilities of 32 bits
-template <typename T>
+template <typename T, int DP>
 __device__ void dq_row(const Args& a, int b, int h, int i) {
     const int lane = threadIdx.x & 63, g = h / (a.hq / a.hkv), pos = i + a.sk - a.sq;
     const float slope = slope_of(a, h);
     const int64_t at = ((int64_t)b * a.hq + h) * a.sq + i;
     const float lse = a.lse[at];
     const T *q = row<T>(a.q, b, i, h), *dout = row<T>(a.dout, b, i, h);
-    float acc[2] = {0, 0}, delta = 0;
+    RowSum<T, DP> acc;
+    float delta = 0;
     const int end = lse == -INFINITY ? 0 : a.causal ? pos + 1 : a.sk;
     auto p_of = [&](int j) {
         return exp2_fast(dot(q, row<T>(a.k, b, j, g), a.d) * (a.scale * LOG2E) -
@@ -157,25 +191,17 @@ __device__ void dq_row(const Args& a, int b, int h, int i) {
         int j = j0 + lane;
         bool seen = j < end && visible(a, b, pos, j);
         float ds = seen ? p_of(j) * (dot(dout, row<T>(a.v, b, j, g), a.d) - delta) : 0.f;
-        for (uint64_t any = __ballot(seen); any; any &= any - 1) {
-            int n = __builtin_ctzll(any);
-            float w = __shfl(ds, n);
-            const T* k = row<T>(a.k, b, j0 + n, g);
-            if (lane < a.d) acc[0] = fmaf(w, (float)k[lane], acc[0]);
-            if (lane + 64 < a.d) acc[1] = fmaf(w, (float)k[lane + 64], acc[1]);
-        }
+        acc.add(ds, __ballot(seen), a.d, [&](int n) { return row<T>(a.k, b, j0 + n, g); });
     }
-    T* dq = row<T>(a.dq, b, i, h);
-    if (lane < a.d) dq[lane] = (T)(acc[0] * a.scale);
-    if (lane + 64 < a.d) dq[lane + 64] = (T)(acc[1] * a.scale);
+    acc.store(row<T>(a.dq, b, i, h), a.d, a.scale);
     if (lane == 0) a.delta[at] = delta;
 }
 
-template <typename T>
+template <typename T, int DP>
 __device__ void dkv_row(const Args& a, int b, int g, int j) {
     const int lane = threadIdx.x & 63, group = a.hq / a.hkv;
     const T *k = row<T>(a.k, b, j, g), *v = row<T>(a.v, b, j, g);
-    float dk[2] = {0, 0}, dv[2] = {0, 0};
+    RowSum<T, DP> dk, dv;
     const int begin = a.causal ? max(0, j - (a.sk - a.sq)) : 0;
     for (int h = g * group; h < (g + 1) * group; ++h) {
         const float slope = slope_of(a, h);
@@ -191,24 +217,12 @@ __device__ void dkv_row(const Args& a, int b, int g, int j) {
                 p = exp2_fast(s - a.lse[at + i]);
                 ds = p * (dot(row<T>(a.dout, b, i, h), v, a.d) - a.delta[at + i]);
             }
-            for (; any; any &= any - 1) {
-                int n = __builtin_ctzll(any);
-                float w = __shfl(p, n), u = __shfl(ds, n);
-                const T *dout = row<T>(a.dout, b, i0 + n, h), *q = row<T>(a.q, b, i0 + n, h);
-                if (lane < a.d) {
-                    dv[0] = fmaf(w, (float)dout[lane], dv[0]);
-                    dk[0] = fmaf(u, (float)q[lane], dk[0]);
-                }
-                if (lane + 64 < a.d) {
-                    dv[1] = fmaf(w, (float)dout[lane + 64], dv[1]);
-                    dk[1] = fmaf(u, (float)q[lane + 64], dk[1]);
-                }
-            }
+            dv.add(p, any, a.d, [&](int n) { return row<T>(a.dout, b, i0 + n, h); });
+            dk.add(ds, any, a.d, [&](int n) { return row<T>(a.q, b, i0 + n, h); });
         }
     }
-    T *to_k = row<T>(a.dk, b, j, g), *to_v = row<T>(a.dv, b, j, g);
-    if (lane < a.d) to_k[lane] = (T)(dk[0] * a.scale), to_v[lane] = (T)dv[0];
-    if (lane + 64 < a.d) to_k[lane + 64] = (T)(dk[1] * a.scale), to_v[lane + 64] = (T)dv[1];
+    dk.store(row<T>(a.dk, b, j, g), a.d, a.scale);
+    dv.store(row<T>(a.dv, b, j, g), a.d, 1.f);
 }
 
 // ---------------------------------------------------------------------------
@@ -303,6 +317,12 @@ template <typename T, int DP, int ROWS, int THREADS> struct Stage {
 #pragma unroll
         for (int n = 0; n < N; ++n)
             r[n] = __builtin_amdgcn_raw_buffer_load_b128(buffer, offset[n], 0, 0);
+    }
+    // rows that `there` does not say become zero
+    template <typename F> __device__ __forceinline__ void keep(F there) {
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+            if (!there((tid + n * THREADS) / G::VECS)) r[n] = raw4{};
     }
     __device__ __forceinline__ void store(T* tile) const {
 #pragma unroll
@@ -669,6 +689,164 @@ template <typename T, int DP> struct Forward {
     }
 };
 
+// ---------------------------------------------------------------------------
+// Results that are not finite.  A hidden infinity or NaN times a probability
+// of zero is NaN, and a scaled sum may pass the largest value: such rows are
+// done again pair by pair, one after the other by their wave, which takes
+// hundreds of times as long.  A row whose own inputs make it so is left as it
+// is, so that an overflowed step, an ordinary one under loss scaling, costs about
+// what others do.  Its inputs make a column NaN if a NaN in that column is
+// visible, or if a score is NaN, and infinite if an infinity is.  Forward and
+// back of 2048 causal rows, 4 heads of 64, bf16, take 90 us, 105 with NaN all
+// over, and 1.4 to 4.2 ms with one infinity, whose tiles are done again.
+// ---------------------------------------------------------------------------
+
+__device__ __forceinline__ uint32_t wave_or(uint32_t x, int from, int to) {
+    for (int m = from; m < to; m <<= 1) x |= __shfl_xor(x, m);
+    return x;
+}
+
+// columns of a head that hold NaN and infinities
+template <int DP> struct Columns {
+    static constexpr int N = DP / 32;
+    uint32_t nan[N] = {}, inf[N] = {};
+
+    static __device__ __forceinline__ uint32_t all(int n, int d) {
+        return d - n * 32 >= 32 ? ~0u : (1u << (d - n * 32)) - 1;
+    }
+    // those of each lane's row, which lies in a result's registers
+    __device__ __forceinline__ void of(const acc16* x, int d) {
+        const int hf = (threadIdx.x & 63) >> 5;
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const uint32_t bit = 1u << (8 * (i >> 2) + (i & 3));
+                if (x[n][i] != x[n][i]) nan[n] |= bit;
+                if (fabsf(x[n][i]) == INFINITY) inf[n] |= bit;
+            }
+            nan[n] = wave_or(nan[n] << (4 * hf), 32, 64) & all(n, d);
+            inf[n] = wave_or(inf[n] << (4 * hf), 32, 64) & all(n, d);
+        }
+    }
+    // those of any row among the lanes that `mine` says
+    __device__ __forceinline__ Columns joined(bool mine) const {
+        Columns c;
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            c.nan[n] = wave_or(mine ? nan[n] : 0, 1, 64);
+            c.inf[n] = wave_or(mine ? inf[n] : 0, 1, 64);
+        }
+        return c;
+    }
+    __device__ __forceinline__ bool any() const {
+        uint32_t x = 0;
+#pragma unroll
+        for (int n = 0; n < N; ++n) x |= nan[n] | inf[n];
+        return x;
+    }
+    __device__ __forceinline__ bool all_nan(int d) const {
+        bool yes = true;
+#pragma unroll
+        for (int n = 0; n < N; ++n) yes &= nan[n] == all(n, d);
+        return yes;
+    }
+    // `seen` makes them so
+    __device__ __forceinline__ bool within(const Columns& seen) const {
+        uint32_t x = 0;
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+            x |= (nan[n] & ~seen.nan[n]) | (inf[n] & ~(seen.nan[n] | seen.inf[n]));
+        return x == 0;
+    }
+};
+
+// Adds to `seen` the columns of NaN and infinities in those of the rows first
+// to end of a head of x that `sees` says, until it holds all of `need`.  The
+// wave reads 64 rows at a time; all lanes get the same.
+template <typename T, int DP, typename S>
+__device__ __forceinline__ void look_for(const Columns<DP>& need, const View& x, int b, int h,
+                                         int first, int end, int d, S sees, Columns<DP>& seen) {
+    constexpr int PER = 16 / sizeof(T), VECS = DP / PER;
+    constexpr int CHUNKS = VECS <= 4 ? 4 : VECS <= 8 ? 8 : VECS <= 16 ? 16 : 32;  // of a row
+    typedef T Vec __attribute__((ext_vector_type(PER)));
+    const int lane = threadIdx.x & 63, c = (lane % CHUNKS) * PER, y = lane / CHUNKS;
+    auto part = [&](const uint32_t* words) {  // this lane's columns
+        uint32_t w = 0;
+#pragma unroll
+        for (int n = 0; n < DP / 32; ++n) w = c / 32 == n ? words[n] : w;
+        return w >> (c % 32) & ((1u << PER) - 1);
+    };
+    const uint32_t need_nan = part(need.nan), need_inf = part(need.inf);
+    uint32_t nan = part(seen.nan), inf = part(seen.inf);
+    for (int j0 = first; j0 < end; j0 += 64) {
+        if (__all((need_nan & ~nan) == 0 && (need_inf & ~(nan | inf)) == 0)) break;
+        const uint64_t rows = __ballot(j0 + lane < end && sees(j0 + lane));
+        if (!rows) continue;
+#pragma unroll 4
+        for (int n = 0; n < CHUNKS; ++n) {
+            const int r = n * (64 / CHUNKS) + y;
+            if (!(rows >> r & 1) || c >= d) continue;
+            const Vec v = *(const Vec*)(row<T>(x, b, j0 + r, h) + c);
+#pragma unroll
+            for (int e = 0; e < PER; ++e) {
+                const float f = (float)v[e];
+                if (f != f) nan |= 1u << e;
+                if (fabsf(f) == INFINITY) inf |= 1u << e;
+            }
+        }
+        nan = wave_or(nan, CHUNKS, 64);
+        inf = wave_or(inf, CHUNKS, 64);
+    }
+#pragma unroll
+    for (int n = 0; n < DP / 32; ++n) {
+        seen.nan[n] |= wave_or(c / 32 == n ? nan << (c % 32) : 0, 1, CHUNKS);
+        seen.inf[n] |= wave_or(c / 32 == n ? inf << (c % 32) : 0, 1, CHUNKS);
+    }
+}
+
+// Calls f with the document, the first row and all rows of each group of a
+// wave's rows (a bit each) that are of one document.
+template <typename F>
+__device__ __forceinline__ void for_documents(uint32_t rows, int doc, F f) {
+    while (rows) {
+        const int lead = __builtin_ctz(rows), of = __shfl(doc, lead);
+        const bool mine = (rows >> (threadIdx.x & 31) & 1) && doc == of;
+        const uint32_t group = (uint32_t)__ballot(mine);
+        rows &= ~group;
+        f(of, mine, group);
+    }
+}
+
+// Those of the wave's queries `rows` whose columns `lost` are not explained by
+// the rows of x, V or K, that they see.  Keys of a probability of 0 times an
+// infinity make NaN of K's (`zeros`).
+template <typename T, int DP>
+__device__ __forceinline__ uint32_t unexplained(const Args& a, const View& x, int b, int g,
+                                                uint32_t rows, int doc, int pos, bool zeros,
+                                                const Columns<DP>& lost) {
+    uint32_t again = 0;
+    for_documents(rows, doc, [&](int of, bool mine, uint32_t group) {
+        bool fine = false;
+        if (of >= 0) {  // others see nothing
+            const int* doc_row = a.documents ? a.documents + b * a.documents_sb : nullptr;
+            const int end = a.causal ? __shfl(pos, __builtin_ctz(group)) + 1 : a.sk;
+            Columns<DP> need = lost.joined(mine), seen;
+            if (zeros)
+#pragma unroll
+                for (int n = 0; n < DP / 32; ++n) need.inf[n] |= need.nan[n], need.nan[n] = 0;
+            look_for<T, DP>(need, x, b, g, 0, end, a.d,
+                            [&](int j) { return !doc_row || doc_row[j] == of; }, seen);
+            if (zeros)
+#pragma unroll
+                for (int n = 0; n < DP / 32; ++n) seen.nan[n] |= seen.inf[n];
+            fine = lost.within(seen);
+        }
+        again |= group & (uint32_t)__ballot(mine && !fine);
+    });
+    return again;
+}
+
 // four values of a row, as they lie in a result's registers
 template <typename T>
 __device__ __forceinline__ void put4(T* at, float a, float b, float c, float d) {
@@ -798,12 +976,15 @@ void forward_kernel(const Args a, const Ranges keys, const Ranges queries, int t
             a.lse[((int64_t)b * a.hq + h) * a.sq + i] =
                 total == 0.f ? -INFINITY : f.off + log2f(total);
     }
-    // A hidden infinity or NaN times a probability of zero is NaN, and values
-    // near the largest pass it with the factor 2^12: such rows are done again
-    // pair by pair.
-    uint64_t bad = __ballot(there && !f.finite());
-    for (uint64_t rows = (bad | bad >> 32) & 0xffffffffull; rows; rows &= rows - 1)
-        forward_row<T>(a, b, h, row0 + __builtin_ctzll(rows));
+    if (__any(there && !f.finite())) {
+        Columns<DP> lost;
+        lost.of(f.o, a.d);
+        // a NaN sum is one of scores, which makes all of the row NaN
+        const uint32_t rows = (uint32_t)__ballot(there && total == total && lost.any());
+        for (uint32_t again = unexplained<T, DP>(a, a.v, b, g, rows, f.doc, f.pos, false, lost);
+             again; again &= again - 1)
+            forward_row<T, DP>(a, b, h, row0 + __builtin_ctz(again));
+    }
 }
 
 // Few queries over many keys: bound by one read of K and V, 6.1 TB/s for 8
@@ -856,13 +1037,16 @@ void split_kernel(const Args a, int parts, int keys_each, int column_tiles, floa
         // tiles with a key that some query may see, of 64
         const int tiles = min(64, (end - chunk + N - 1) / N);
         uint64_t visits = tiles == 64 ? ~0ull : (1ull << tiles) - 1;
+        uint64_t whole = visits;  // those that all their keys may be seen of
         if (doc_row) {
-            visits = 0;
+            visits = whole = 0;
             for (int t = 0; t < tiles; t += 2) {
                 int j = chunk + t * N + lane, d = j < end ? doc_row[j] : -1;
                 uint64_t met = __ballot(d >= least && d <= largest);
                 if (met & 0xffffffffull) visits |= 1ull << t;
                 if (met >> 32) visits |= 2ull << t;
+                if ((met & 0xffffffffull) == 0xffffffffull) whole |= 1ull << t;
+                if (met >> 32 == 0xffffffffull) whole |= 2ull << t;
             }
         }
         int key_doc = -1;
@@ -872,13 +1056,19 @@ void split_kernel(const Args a, int parts, int keys_each, int column_tiles, floa
 #pragma unroll
             for (int n = 0; n < DP / 16; ++n)
                 next_k[n] = row_frag<T>(kr, n * 16 + hf * 8, a.d, row_there);
-            sv.load(v + (int64_t)at * a.v.ss, a.sk - at);
+            sv.load(v + (int64_t)at * a.v.ss, end - at);
             int j = at + lane;
             if (lane < N) key_doc = j < a.sk ? doc_row ? max(doc_row[j], -1) : 0 : -1;
         };
         int at = visits ? chunk + __builtin_ctzll(visits) * N : 0;
         if (visits) fetch(at);
         while (visits) {
+            // what a cache holds where there is no sequence may be anything
+            if (!(whole >> __builtin_ctzll(visits) & 1))
+                sv.keep([&](int y) {
+                    const int d = __shfl(key_doc, y);
+                    return d >= least && d <= largest;
+                });
             visits &= visits - 1;
             // one wave: its own reads and writes of shared memory keep order
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -915,10 +1105,10 @@ constexpr int MOST_PARTS = 256;
 // One row a block: the parts' exponents and sums first, then their values in
 // 256 / DP shares of the parts.
 template <typename T, int DP>
-__global__ __launch_bounds__(256) void join_kernel(const Args a, int parts, const float* part_o,
+__global__ __launch_bounds__(256, 6) void join_kernel(const Args a, int parts, const float* part_o,
                                                    const float2* part_state) {
     __shared__ float weight[MOST_PARTS], shared[8], values[256];
-    __shared__ int lost;
+    __shared__ uint32_t lost[2][DP / 32], found[2][DP / 32];  // columns of NaN, of infinities
     const int group = a.hq / a.hkv, columns = group * a.sq;
     const int column = blockIdx.x % columns, g = blockIdx.x / columns % a.hkv;
     const int b = blockIdx.x / columns / a.hkv, h = g * group + column / a.sq, i = column % a.sq;
@@ -941,7 +1131,7 @@ __global__ __launch_bounds__(256) void join_kernel(const Args a, int parts, cons
     const float exponent = state.y == 0.f ? -INFINITY : state.x;
     float most = wave_max(exponent);
     if ((tid & 63) == 0) shared[wave] = most;
-    if (tid == 0) lost = 0;
+    if (tid < 2 * (DP / 32)) lost[0][tid] = 0, found[0][tid] = 0;
     __syncthreads();
     most = fmaxf(fmaxf(shared[0], shared[1]), fmaxf(shared[2], shared[3]));
     const float w = state.y == 0.f ? 0.f : exp2_fast(exponent - most);
@@ -969,12 +1159,32 @@ __global__ __launch_bounds__(256) void join_kernel(const Args a, int parts, cons
         for (int n = 0; n < SHARES; ++n) o += values[n * DP + tid];
         o *= inv;
         row<T>(a.out, b, i, h)[tid] = (T)o;
-        if (!(fabsf(o) <= 3.4028235e38f)) lost = 1;
+        if (!(fabsf(o) <= 3.4028235e38f)) atomicOr(&lost[o == o][tid / 32], 1u << (tid % 32));
     }
     if (tid == 0 && a.lse)
         a.lse[((int64_t)b * a.hq + h) * a.sq + i] = total == 0.f ? -INFINITY : most + log2f(total);
     __syncthreads();
-    if (lost && wave == 0) forward_row<T>(a, b, h, i);  // as in forward_kernel
+    // as in forward_kernel, a quarter of the keys each wave
+    Columns<DP> need;
+#pragma unroll
+    for (int n = 0; n < DP / 32; ++n) need.nan[n] = lost[0][n], need.inf[n] = lost[1][n];
+    if (!need.any() || total != total) return;
+    const int pos = i + a.sk - a.sq, end = a.causal ? pos + 1 : a.sk;
+    const int* doc_row = a.documents ? a.documents + b * a.documents_sb : nullptr;
+    const int doc = doc_row ? doc_row[pos] : 0, each = (end + 255) / 256 * 64;
+    Columns<DP> seen;
+    look_for<T, DP>(need, a.v, b, g, min(wave * each, end), min((wave + 1) * each, end), a.d,
+                    [&](int j) { return !doc_row || doc_row[j] == doc; }, seen);
+    if ((tid & 63) == 0)
+#pragma unroll
+        for (int n = 0; n < DP / 32; ++n) {
+            atomicOr(&found[0][n], seen.nan[n]);
+            atomicOr(&found[1][n], seen.inf[n]);
+        }
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < DP / 32; ++n) seen.nan[n] = found[0][n], seen.inf[n] = found[1][n];
+    if (wave == 0 && !need.within(seen)) forward_row<T, DP>(a, b, h, i);
 }
 
 int padded(int d) { return (d + 31) / 32 * 32; }
@@ -1256,6 +1466,8 @@ void dq_kernel(const Args a, const Ranges keys, const Ranges queries, int tiles_
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[n][e] = fmaf(-by, mean[n][e], acc[n][e]);
         delta += FACTORED<T> ? by / factor : rest;
+    } else {
+        delta += delta - delta;  // an infinity is NaN here too
     }
     if (there && hf == 0) a.delta[at_row] = delta;
     if (there) {
@@ -1272,9 +1484,29 @@ void dq_kernel(const Args a, const Ranges keys, const Ranges queries, int tiles_
                 for (int e = 0; e < 4; ++e) fine &= fabsf(acc[n][r * 4 + e]) <= 3.4028235e38f;
             }
     }
-    uint64_t bad = __ballot(there && !fine);
-    for (uint64_t rows = (bad | bad >> 32) & 0xffffffffull; rows; rows &= rows - 1)
-        dq_row<T>(a, b, h, row0 + __builtin_ctzll(rows));
+    if (__any(there && !fine)) {
+        Columns<DP> lost;
+        lost.of(acc, a.d);
+        // a row with a visible NaN among its scores, or one of whose output or
+        // its gradient is not finite, is NaN
+        bool given = true;
+#pragma unroll
+        for (int n = 0; n < DP / 16; ++n) {
+            const Frag<T> o =
+                row_frag<T>(row<T>(a.out, b, there ? i : 0, h), n * 16 + hf * 8, a.d, there);
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                given &= fabsf((float)o[e]) < INFINITY && fabsf((float)dout[n][e]) < INFINITY;
+        }
+        given = !wave_or(!given, 32, 64);
+        const bool stands = lost.all_nan(a.d) && (off != off || (off < INFINITY && !given));
+        const bool sum = fabsf(rest) <= 3.4028235e38f;
+        uint32_t again = (uint32_t)__ballot(there && !stands && !sum);
+        again |= unexplained<T, DP>(a, a.k, b, g,
+                                    (uint32_t)__ballot(there && !stands && sum && lost.any()),
+                                    doc, pos, true, lost);
+        for (; again; again &= again - 1) dq_row<T, DP>(a, b, h, row0 + __builtin_ctz(again));
+    }
 }
 
 template <typename T, int DP, int ROWS, int SHARES>
@@ -1468,9 +1700,50 @@ void dkv_kernel(const Args a, const Ranges keys, const Ranges queries, int tiles
                     fine &= fabsf(dk[n][x]) <= 3.4028235e38f && fabsf(dv[n][x]) <= 3.4028235e38f;
             }
     }
-    uint64_t bad = __ballot(there && !fine);
-    for (uint64_t rows = (bad | bad >> 32) & 0xffffffffull; rows; rows &= rows - 1)
-        dkv_row<T>(a, b, g, key0 + __builtin_ctzll(rows));
+    if (__any(there && !fine)) {
+        Columns<DP> lost_k, lost_v;
+        lost_k.of(dk, a.d);
+        lost_v.of(dv, a.d);
+        uint32_t again = 0;
+        for_documents((uint32_t)__ballot(there && (lost_k.any() || lost_v.any())), doc,
+                      [&](int of, bool mine, uint32_t rows) {
+            if (of < 0) {  // seen by no query
+                again |= rows;
+                return;
+            }
+            // queries that see all of these keys: a NaN among the scores of one
+            // makes dk and dv NaN, one as its delta dk
+            const int from = a.causal ? max(0, key0 + 31 - __builtin_clz(rows) - first) : 0;
+            bool nan_score = false, nan_delta = false;
+            auto sees = [&](int64_t at, int i) {
+                return (!doc_row || doc_row[i + first] == of) && a.lse[at + i] != -INFINITY;
+            };
+            for (int h = g * group; h < (g + 1) * group && !nan_score; ++h) {
+                const int64_t at = ((int64_t)b * a.hq + h) * a.sq;
+                for (int i0 = from; i0 < a.sq && !nan_score; i0 += 64) {
+                    const int i = i0 + lane;
+                    const bool seen = i < a.sq && sees(at, i);
+                    const float l = seen ? a.lse[at + i] : 0.f, x = seen ? a.delta[at + i] : 0.f;
+                    nan_score = __any(l != l);
+                    nan_delta |= __any(x != x);
+                }
+            }
+            Columns<DP> seen;
+            if (!nan_score) {
+                const Columns<DP> need = lost_v.joined(mine);
+                for (int h = g * group; h < (g + 1) * group && need.any(); ++h) {
+                    const int64_t at = ((int64_t)b * a.hq + h) * a.sq;
+                    look_for<T, DP>(need, a.dout, b, h, from, a.sq, a.d,
+                                    [&](int i) { return sees(at, i); }, seen);
+                }
+            }
+            const bool fine_k = !lost_k.any() || (lost_k.all_nan(a.d) && (nan_score || nan_delta));
+            const bool fine_v = nan_score ? !lost_v.any() || lost_v.all_nan(a.d)
+                                          : lost_v.within(seen);
+            again |= rows & (uint32_t)__ballot(mine && !(fine_k && fine_v));
+        });
+        for (; again; again &= again - 1) dkv_row<T, DP>(a, b, g, key0 + __builtin_ctz(again));
+    }
 }
 
 template <typename T, int DP>

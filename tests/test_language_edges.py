@@ -10,7 +10,7 @@ import torch.autograd.forward_ad as forward_ad
 
 from deepreduce_amd import ops
 from test_language_ops import (BOTH, E, TYPES, assert_within, attention_inputs, attention_oracle,
-                               check_attention, half_step, pack)
+                               check_attention, half_step, pack, seen_pairs)
 
 
 # --------------------------------------------------------------------------
@@ -206,3 +206,147 @@ def test_many_requests(dtype, shape):
     slopes = torch.linspace(0.05, 0.0, hq, device="cuda")
     check_attention(q, k, v, dout, documents.cuda(), slopes, causal=True)
     check_attention(q, k, v, dout, causal=sq > 1)
+
+
+# --------------------------------------------------------------------------
+# steps that are not finite
+# --------------------------------------------------------------------------
+
+def spoil(x, which, bad, where):
+    """Copies of x's tensors with `bad` in one value of `which`, or in all."""
+    y = {n: t.clone() for n, t in x.items()}
+    t = y[which]
+    if where == "all":
+        t[:] = bad
+    else:
+        t[0, t.shape[1] * 2 // 3, t.shape[2] - 1, 5] = bad
+    return y
+
+
+def attention_step(x, **options):
+    leaves = [x[n].detach().requires_grad_(True) for n in ("q", "k", "v")]
+    out = ops.attention(*leaves, **options)
+    return [out.detach(), *torch.autograd.grad(out, leaves, x["dout"])]
+
+
+def formulas(q, k, v, dout, documents, causal):
+    """Results of one entry in 64 bits; hidden pairs are in no product."""
+    sq, hq, d = q.shape
+    sk, hkv = k.shape[:2]
+    seen, _ = seen_pairs(documents.unsqueeze(0), causal, 1, sq, sk)
+    seen = seen[0]
+
+    def product(w, x, s):
+        bad = ~x.isfinite()
+        y = w @ x.masked_fill(bad, 0.0)
+        for j in bad.any(1).nonzero().flatten().tolist():
+            y = y + torch.where(s[:, j:j + 1], w[:, j:j + 1] * x[j].masked_fill(~bad[j], 0.0), 0.0)
+        return y
+
+    got = {n: torch.zeros(t.shape, dtype=torch.float64)
+           for n, t in (("out", q), ("dq", q), ("dk", k), ("dv", v))}
+    for h in range(hq):
+        g, scale = h * hkv // hq, d ** -0.5
+        Q, K, V, dO = q[:, h], k[:, g], v[:, g], dout[:, h]
+        s = (scale * (Q @ K.T)).masked_fill(~seen, -math.inf)
+        P = torch.where(seen, torch.softmax(s, 1), 0.0)
+        O = product(P, V, seen)
+        dP = torch.where(seen, dO @ V.T, 0.0)
+        delta = torch.where(seen.any(1), (dO * O).sum(1), 0.0).unsqueeze(1)
+        dS = torch.where(seen, P * (dP - delta), 0.0)
+        got["out"][:, h], got["dq"][:, h] = O, scale * product(dS, K, seen)
+        got["dk"][:, g] += scale * product(dS.T, Q, seen.T)
+        got["dv"][:, g] += product(P.T, dO, seen.T)
+    return got
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("bad", [math.inf, math.nan], ids=str)
+@pytest.mark.parametrize("which", ["q", "k", "v", "dout"])
+@pytest.mark.parametrize("where", ["one", "all"])
+@pytest.mark.parametrize("shape", [(1, 300, 300, 2, 1, 64), (1, 100, 333, 2, 2, 40),
+                                   (1, 3, 1000, 4, 2, 128), (32, 130, 130, 16, 16, 32)], ids=str)
+def test_what_is_not_finite_stays_where_it_is_seen(dtype, bad, which, where, shape):
+    """What a row sees that is not finite makes it so, as in the formulas; rows that
+    do not see it are those of a call without it, and hidden NaN change nothing."""
+    b, sq, sk, hq, hkv, d = shape
+    names = ("q", "k", "v", "dout")
+    x = dict(zip(names, attention_inputs(*shape, dtype, "cpu", seed=sk)))
+    n = sk - sk // 4
+    documents = torch.tensor([pack([n - 7, 7], n)] * b, dtype=torch.int32)
+    documents = torch.cat((documents, torch.full((b, sk - n), 2, dtype=torch.int32)), 1)
+    dirty = spoil(x, which, bad, where)
+    hidden = {n: t.clone() for n, t in dirty.items()}
+    for t in hidden.values():  # the last document, which no check below looks at
+        t[:, -(sk // 4):] = math.nan
+    for causal in (False, True):
+        on = lambda y, e=slice(None): {n: t[e].cuda() for n, t in y.items()}  # noqa: E731
+        options = dict(documents=documents.cuda(), causal=causal)
+        got = attention_step(on(dirty), **options)
+        more = attention_step(on(hidden), **options)
+        clean = attention_step(on(x), **options)
+        want = formulas(*[dirty[n][0].double() for n in names], documents[0], causal)
+        for name, g, m, c in zip(("out", "dq", "dk", "dv"), got, more, clean):
+            g, m, c, w = (t.double().cpu() for t in (g, m, c, want[name].unsqueeze(0)))
+            assert torch.equal(g[:1].isfinite(), w.isfinite()), name
+            seen = slice(0, max(0, g.shape[1] - sk // 4))
+            assert torch.equal(g[:, seen].isfinite(), m[:, seen].isfinite()), name
+            fine = g.isfinite()
+            size = c.abs().max()
+            # scores and sums as in a clean call, or added in another order
+            tol = 8 * (half_step(dtype) + 256 * E) * size
+            fine[0] &= False
+            if where == "one":
+                assert ((g - c).abs()[fine] <= tol).all() and fine[1:].all(), name
+            both = g[:1].isfinite()
+            assert ((g[:1] - w).abs()[both] <= 2 * tol).all(), name
+            both = g[:, seen].isfinite()
+            assert ((g[:, seen] - m[:, seen]).abs()[both] <= tol).all(), name
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("which,bad,where", [
+    ("v", math.nan, "all"), ("q", math.nan, "all"), ("dout", math.nan, "all"),
+    ("dout", math.inf, "all"), ("dout", math.inf, "one"), ("dout", math.nan, "one"),
+    ("v", math.inf, "one"), ("v", math.nan, "one"), ("k", math.inf, "one"),
+    ("q", math.inf, "one")])
+def test_steps_that_are_not_finite(dtype, which, bad, where):
+    """Overflow is an ordinary step under loss scaling: one that is NaN all over
+    takes no longer than others, and one value that is not finite makes no more
+    rows be done again than share a tile with it (all of them: 100 to 800 times)."""
+    x = dict(zip(("q", "k", "v", "dout"),
+                 attention_inputs(1, 2048, 2048, 4, 4, 64, dtype, "cuda")))
+    dirty = spoil(x, which, bad, where)
+    documents = torch.zeros(1, 2048, dtype=torch.int32, device="cuda")
+    documents[:, :900] = 1
+    for options in (dict(causal=True), dict(documents=documents)):
+        usual = time_of(lambda: attention_step(x, **options))
+        this = time_of(lambda: attention_step(dirty, **options))
+        print(f"\n{this * 1e6:.0f} us, usual {usual * 1e6:.0f}", end="")
+        assert this <= (2 if where == "all" and bad != math.inf else 64) * usual
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_caches_of_anything_behind_their_sequences(dtype):
+    """Tokens over caches whose padding holds NaN, in time and results those of
+    caches that hold zeros there."""
+    b, sk = 8, 8192
+    q, k, v, _ = attention_inputs(b, 1, sk, 12, 4, 64, dtype, "cuda")
+    lengths = [8191, 5000, 4097, 4095, 33, 1, 7000, 6432]
+    ahead = torch.tensor([pack([n], sk - 1) + [0] for n in lengths], dtype=torch.int32,
+                         device="cuda")
+    behind = torch.tensor([[-1] * (sk - n) + [0] * n for n in lengths], dtype=torch.int32,
+                          device="cuda")
+    for documents in (ahead, behind):
+        hidden = (documents < 0)[..., None, None]
+        zeros, anything = ([t.masked_fill(hidden, x) for t in (k, v)] for x in (0.0, math.nan))
+        want = ops.attention(q, *zeros, documents)
+        assert want.isfinite().all()
+        assert torch.equal(ops.attention(q, *anything, documents), want)
+        usual = time_of(lambda: ops.attention(q, *zeros, documents))
+        this = time_of(lambda: ops.attention(q, *anything, documents))
+        print(f"\n{this * 1e6:.0f} us, usual {usual * 1e6:.0f}", end="")
+        assert this <= 2 * usual
