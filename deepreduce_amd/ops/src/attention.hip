@@ -1993,7 +1993,7 @@ struct AttentionFunction : torch::autograd::Function<AttentionFunction> {
         torch::autograd::variable_list d;
         {
             at::AutoGradMode no(false);
-            d = attention_backward(grads[0], x[0], x[1], x[2], x[5], x[6],
+            d = attention_backward(grads[0].resolve_neg(), x[0], x[1], x[2], x[5], x[6],
                                    {x.begin() + 7, x.end()}, x[3], x[4],
                                    ctx->saved_data["causal"].toBool(),
                                    ctx->saved_data["scale"].toDouble());
@@ -2013,7 +2013,9 @@ torch::Tensor attention(torch::Tensor q, torch::Tensor k, torch::Tensor v,
     TORCH_CHECK_VALUE(q.dim() == 4, "attention: q must be [batch, length, heads, head size]");
     if (documents && documents->dim() == 2 && documents->size(1) > 1 && documents->stride(1) != 1)
         documents = documents->contiguous();
-    if (slopes) slopes = slopes->contiguous();
+    if (slopes) slopes = slopes->resolve_neg().contiguous();
+    // views that torch negates when it reads them
+    q = q.resolve_neg(), k = k.resolve_neg(), v = v.resolve_neg();
     const torch::Tensor none;
     check_seen({q, k, v, slopes.value_or(none)}, "attention");
     const double by = scale.value_or(1.0 / std::sqrt((double)q.size(3)));

@@ -471,12 +471,13 @@ std::pair<std::vector<torch::Tensor>, torch::Tensor> clip_grad_norm(
                           "clip_grad_norm: gradient ", i, " shares memory with output ", it->i);
     }
 
-    // other orders than dense ones go through copies
+    // other orders than dense ones go through copies, and so do views that torch
+    // negates when it reads or writes them
     std::vector<std::pair<size_t, torch::Tensor>> copies;
     for (size_t i = 0; i < grads.size(); ++i) {
-        if (same_order(grads[i], outs[i])) continue;
-        grads[i] = grads[i].contiguous();
-        if (!same_order(grads[i], outs[i])) {
+        if (same_order(grads[i], outs[i]) && grads[i].is_neg() == outs[i].is_neg()) continue;
+        grads[i] = grads[i].resolve_neg().contiguous();
+        if (!same_order(grads[i], outs[i]) || outs[i].is_neg()) {
             copies.emplace_back(i, outs[i]);
             outs[i] = torch::empty(grads[i].sizes(), outs[i].options());
         }

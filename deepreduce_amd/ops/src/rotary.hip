@@ -211,6 +211,7 @@ torch::autograd::variable_list rotate(torch::autograd::variable_list xs,
     int heads = 0;
     for (size_t t = 0; t < xs.size(); ++t) {
         auto& x = xs[t];
+        x = x.resolve_neg();  // a view that torch negates when it reads it
         if (x.stride(3) != 1) x = x.contiguous();
         outs.push_back(torch::empty(x.sizes(), x.options()));
         a.x[t] = {x.data_ptr(), outs[t].data_ptr(), x.stride(0), x.stride(1), x.stride(2),
@@ -315,7 +316,7 @@ std::vector<torch::Tensor> rotary(torch::Tensor q, torch::Tensor k, torch::Tenso
     TORCH_CHECK_VALUE(!frequencies.requires_grad(),
                       "rotary: frequencies are constants and get no gradient");
     check_seen({q, k, frequencies}, "rotary");
-    frequencies = frequencies.contiguous();
+    frequencies = frequencies.resolve_neg().contiguous();
     if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad()))
         return RotaryFunction::apply(q, k, positions, frequencies, interleaved);
     return rotate({q, k}, positions, frequencies, interleaved, false);

@@ -350,3 +350,46 @@ def test_caches_of_anything_behind_their_sequences(dtype):
         this = time_of(lambda: ops.attention(q, *anything, documents))
         print(f"\n{this * 1e6:.0f} us, usual {usual * 1e6:.0f}", end="")
         assert this <= 2 * usual
+
+
+# --------------------------------------------------------------------------
+# views that torch negates when it reads them
+# --------------------------------------------------------------------------
+
+def negated(x):
+    """A view with x's values over memory that holds their negatives."""
+    view = torch._neg_view(-x)
+    assert view.is_neg() and torch.equal(view, x)
+    return view
+
+
+@pytest.mark.parametrize("device", BOTH)
+@pytest.mark.parametrize("name", ["attention", "rotary", "grad_norm", "clip_grad_norm"])
+def test_negated_views(device, name):
+    call, inputs = small_calls(device)[name]
+    want = call(*inputs)
+    for n, x in enumerate(inputs):
+        others = list(inputs)
+        others[n] = negated(x)
+        assert torch.equal(call(*others), want)
+    assert torch.equal(call(*[negated(x) for x in inputs]), want)
+
+
+@pytest.mark.parametrize("device", BOTH)
+def test_negated_gradients(device):
+    q, k, v, dout = attention_inputs(1, 9, 9, 2, 1, 16, torch.float32, device)
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    positions = torch.arange(9, device=device)
+    frequencies = ops.rotary_frequencies(16, device=device)
+    for call in (lambda: ops.attention(q, k, v), lambda: ops.rotary(q, k, positions,
+                                                                     frequencies)[0]):
+        want, got = (torch.autograd.grad(call(), leaves[:1], g) for g in (dout, negated(dout)))
+        assert torch.equal(want[0], got[0])
+    x, y = (torch.randn(40, device=device) for _ in range(2))
+    (want,), _ = ops.clip_grad_norm([x], 0.5)
+    for out in (torch.empty_like(x), negated(y)):
+        ops.clip_grad_norm([x], 0.5, out=[out])
+        assert torch.equal(out, want)
+    view = negated(x)
+    ops.clip_grad_norm_([view], 0.5)
+    assert torch.equal(view, want)
