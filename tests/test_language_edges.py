@@ -9,8 +9,8 @@ import torch
 import torch.autograd.forward_ad as forward_ad
 
 from deepreduce_amd import ops
-from test_language_ops import (BOTH, E, TYPES, assert_within, attention_inputs, attention_oracle,
-                               check_attention, half_step, pack, seen_pairs)
+from test_language_ops import (BOTH, DOCS, E, TYPES, assert_within, attention_inputs,
+                               attention_oracle, check_attention, half_step, pack, seen_pairs)
 
 
 # --------------------------------------------------------------------------
@@ -393,3 +393,46 @@ def test_negated_gradients(device):
     view = negated(x)
     ops.clip_grad_norm_([view], 0.5)
     assert torch.equal(view, want)
+
+
+# --------------------------------------------------------------------------
+# the blocks of large inputs
+# --------------------------------------------------------------------------
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("shape", [
+    (32, 129, 129, 16, 16, 64),   # a last block with one row; 1024 blocks
+    (16, 200, 200, 16, 16, 32),   # 512 blocks: long and short ones alternate
+    (24, 161, 161, 12, 12, 128), (40, 140, 140, 16, 8, 96),
+    (64, 130, 197, 8, 8, 40),     # queries behind 67 keys
+    (600, 33, 33, 1, 1, 64)], ids=str)
+@pytest.mark.parametrize("docs", ["none", "packed", "mixed"])
+def test_large_batches(dtype, shape, docs):
+    """Rows enough for blocks of four waves that share their tiles, in all
+    kernels: some entries against 64 bits, the others against the same entry
+    alone, which takes other blocks."""
+    b, sq, sk, hq, hkv, d = shape
+    assert b * hkv * ((min(sq, sk) + 127) // 128) >= 512
+    x = attention_inputs(*shape, dtype, "cuda", seed=sum(shape))
+    documents = DOCS[docs](b, sk)
+    documents = None if documents is None else documents.cuda()
+    for causal in (False, True):
+        slopes = torch.linspace(0.3, 0.0, hq).cuda() if causal else None
+        run = lambda e: attention_step(  # noqa: E731
+            {n: t[e] for n, t in zip(("q", "k", "v", "dout"), x)}, slopes=slopes, causal=causal,
+            documents=None if documents is None else documents[e])
+        got = run(slice(None))
+        for e in range(b):
+            one = slice(e, e + 1)
+            if e in (0, b // 2, b - 1):
+                want = attention_oracle(*[t[one] for t in x[:3]],
+                                        None if documents is None else documents[one], slopes,
+                                        causal, d ** -0.5, x[3][one])
+                for name, g in zip(("out", "dq", "dk", "dv"), got):
+                    assert_within(g[one], *want[name], f"{name} of entry {e}")
+            elif e % max(1, b // 20) == 0:
+                for name, g, w in zip(("out", "dq", "dk", "dv"), got, run(one)):
+                    # both off by their roundings: of P or dS, and of the result
+                    tol = 4 * (half_step(dtype) + 256 * E) * w.abs().max()
+                    assert (g[one].double() - w.double()).abs().max() <= tol, f"{name} of {e}"
