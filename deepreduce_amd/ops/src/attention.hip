@@ -1499,12 +1499,13 @@ void dq_kernel(const Args a, const Ranges keys, const Ranges queries, int tiles_
                 given &= fabsf((float)o[e]) < INFINITY && fabsf((float)dout[n][e]) < INFINITY;
         }
         given = !wave_or(!given, 32, 64);
-        const bool stands = lost.all_nan(a.d) && (off != off || (off < INFINITY && !given));
+        const bool stands = lost.all_nan(a.d) && (off != off || (off != INFINITY && !given));
         const bool sum = fabsf(rest) <= 3.4028235e38f;
-        uint32_t again = (uint32_t)__ballot(there && !stands && !sum);
-        again |= unexplained<T, DP>(a, a.k, b, g,
-                                    (uint32_t)__ballot(there && !stands && sum && lost.any()),
-                                    doc, pos, true, lost);
+        const bool nothing = off == INFINITY;  // seen: its gradient is 0
+        uint32_t again = (uint32_t)__ballot(there && !stands && (!sum || nothing));
+        again |= unexplained<T, DP>(
+            a, a.k, b, g, (uint32_t)__ballot(there && !stands && sum && !nothing && lost.any()),
+            doc, pos, true, lost);
         for (; again; again &= again - 1) dq_row<T, DP>(a, b, h, row0 + __builtin_ctz(again));
     }
 }

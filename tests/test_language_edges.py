@@ -305,6 +305,21 @@ def test_what_is_not_finite_stays_where_it_is_seen(dtype, bad, which, where, sha
             assert ((g[:, seen] - m[:, seen]).abs()[both] <= tol).all(), name
 
 
+@pytest.mark.parametrize("device", BOTH)
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("sq", [1, 70])
+def test_scores_of_minus_infinity(device, dtype, sq):
+    """A query whose scores are all minus infinity sees nothing: it gives 0, with
+    zero gradients."""
+    q, k, v, dout = attention_inputs(1, sq, 70, 2, 2, 32, dtype, device)
+    q[..., 3] = q[..., 3].abs() + 1
+    k[..., 3] = -math.inf
+    x = dict(q=q, k=k, v=v, dout=dout)
+    for causal in (False, True):
+        for t in attention_step(x, causal=causal):
+            assert not t.any()
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
 @pytest.mark.parametrize("which,bad,where", [
