@@ -75,6 +75,11 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
         -slopes[h] * |query position - key position|.
     causal: a query sees no later position.
     scale: factor of the scores, D ** -0.5 by default.
+
+    On a GPU scores, sums and statistics have 32 bits.  For 16-bit inputs the
+    probabilities, and in the backward pass their gradients, are rounded to the
+    inputs' type once more before their products, as the matrix cores take
+    them: results are off by about 1.4 times their own rounding.
     """
     hip = _hip(q)
     if hip:
@@ -230,7 +235,8 @@ def clip_grad_norm(tensors, max_norm: float, out=None, dtype: torch.dtype | None
     types; it may be the tensor itself, but the stretches of memory that
     outputs lie in, gaps included, may not overlap otherwise) or to new tensors
     of `dtype` (each one's own by default).  A norm that is infinite or NaN
-    enters the product as it is: NaN reaches every value.  Constants for both
+    enters the product as it is: the one makes finite values 0 and infinities
+    NaN, the other makes every value NaN.  Constants for both
     modes of differentiation.
     """
     grads, outs = _list(tensors), None if out is None else _list(out)

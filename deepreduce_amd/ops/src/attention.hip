@@ -858,12 +858,12 @@ __device__ __forceinline__ void put4(T* at, float a, float b, float c, float d) 
 // tiles of K and V; block tiles of one head are neighbours on one XCD, whose
 // L2 then serves the head's keys once.
 //
-// Heads of 64 are bound by the vector unit (a multiply-add, an exponential, a
-// maximum, a sum and half a conversion for each pair, 53 % of its cycles beside
-// 29 % of the matrix unit's), heads of 128 by the two in turn.  2 x 16 heads,
-// 4096 x 4096, bf16: 640 TFLOP/s at 64, 850 to 900 at 128; a large matrix product
-// reaches 1244.  Tiles of 64 keys: passing over half a tile by its documents
-// costs more than it saves (582 TFLOP/s).
+// Vector and matrix unit work in turn more than side by side: for heads of 64
+// the one is busy for 53 % of the cycles (a multiply-add, an exponential, a
+// maximum, a sum and half a conversion for each pair), the other for 29 %.  2 x
+// 16 heads, 4096 x 4096, bf16: 710 TFLOP/s at 64, 890 at 128; a large matrix
+// product reaches 1373.  Tiles of 64 keys: passing over half a tile by its
+// documents costs more than it saves (582 TFLOP/s for 640).
 template <typename T, int DP, int ROWS, int SHARES>
 __global__ __launch_bounds__(ROWS * SHARES * 64, (forward_waves<T, DP, SHARES>))
 void forward_kernel(const Args a, const Ranges keys, const Ranges queries, int tiles_q,
@@ -987,10 +987,12 @@ void forward_kernel(const Args a, const Ranges keys, const Ranges queries, int t
     }
 }
 
-// Few queries over many keys: bound by one read of K and V, 6.1 TB/s for 8
-// requests with 4 heads of 64 over 32768 keys (44 us, and 5 us the join).  A wave takes up
-// to 32 columns, which are the queries of all heads of one key-value head, and
-// one part of the keys; nothing is shared between waves.  K's fragments are
+// Few queries over many keys: bound by one read of what is visible of K and V.
+// 8 requests of 32768 keys, 4 heads of 64, bf16: 268 MB in 42 us and 5 us the
+// join (5.7 TB/s in all; reads alone reach 6.1); with 30 % of the keys hidden in
+// front as long, 189 MB at 4.4 TB/s, since parts of hidden keys alone have nothing to do.
+// A wave takes up to 32 columns, which are the queries of all heads of one
+// key-value head, and one part of the keys; nothing is shared between waves.  K's fragments are
 // rows as they lie in memory and go straight to registers, V passes through
 // shared memory for its columns; both travel a tile ahead.  join_kernel adds
 // the parts up, each with its own exponent.
@@ -1266,12 +1268,14 @@ void launch_forward(const Args& a, const Ranges& keys, const Ranges& queries,
 // Backward.  First the queries' gradient, whose waves hold 32 queries as the
 // forward's do, and their delta; then the keys' and values', whose waves hold
 // 32 keys and go over the queries of all heads that share them.  Scores are
-// formed again in both (7 products where 5 would do), so that nothing is added
-// across blocks: results repeat bit by bit and no buffer of gradients is needed.
+// formed again in both (7 products where 5 would do, and in 16 bits one more in
+// dq for its correction), so that nothing is added across blocks: results repeat
+// bit by bit and no buffer of gradients is needed.
 //
-// 2 x 16 heads, 4096 x 4096, bf16: dq 820 TFLOP/s and dkv 700 with heads of 64,
-// 810 and 630 with heads of 128, whose sums leave one wave a SIMD: K and V in
-// shared memory make room for two, but then its reads bound the kernel (604).
+// 2 x 16 heads, 4096 x 4096, bf16, four products each: dq 920 TFLOP/s and dkv 830
+// with heads of 64 (298 and 331 us), 840 and 650 with heads of 128, whose sums
+// leave one wave a SIMD: K and V in shared memory make room for two, but then its
+// reads bound dkv (604 for 631).
 // Packed rows of 512 (32 of them, 12 heads of 64: dq 77 us, dkv 82) are bound by
 // their blocks' reads, in step with each other, and the masks of mixed tiles.
 //
