@@ -88,12 +88,17 @@ __device__ __forceinline__ float dot(const T* x, const T* y, int d) {
     return s;
 }
 
-// A weighted sum of rows of up to DP values, of which a lane holds 16 bytes'
-// worth and CHUNKS lanes a row: 64 / CHUNKS rows are read at a time.
-template <typename T, int DP> struct RowSum {
+// Rows of up to DP values, of which a lane reads 16 bytes and CHUNKS lanes all:
+// 64 / CHUNKS rows at a time.  RowSum is a weighted sum of them.
+template <typename T, int DP> struct Chunk {
     static constexpr int PER = 16 / sizeof(T), VECS = DP / PER;
     static constexpr int CHUNKS = VECS <= 4 ? 4 : VECS <= 8 ? 8 : VECS <= 16 ? 16 : 32;
     typedef T Vec __attribute__((ext_vector_type(PER)));
+};
+template <typename T, int DP> struct RowSum : Chunk<T, DP> {
+    using Chunk<T, DP>::PER;
+    using Chunk<T, DP>::CHUNKS;
+    using typename Chunk<T, DP>::Vec;
     float x[PER] = {};
 
     // w of lane n times row_of(n) for the lanes n in `any`; others' rows are not read
@@ -693,12 +698,13 @@ template <typename T, int DP> struct Forward {
 // Results that are not finite.  A hidden infinity or NaN times a probability
 // of zero is NaN, and a scaled sum may pass the largest value: such rows are
 // done again pair by pair, one after the other by their wave, which takes
-// hundreds of times as long.  A row whose own inputs make it so is left as it
-// is, so that an overflowed step, an ordinary one under loss scaling, costs about
-// what others do.  Its inputs make a column NaN if a NaN in that column is
-// visible, or if a score is NaN, and infinite if an infinity is.  Forward and
-// back of 2048 causal rows, 4 heads of 64, bf16, take 90 us, 105 with NaN all
-// over, and 1.4 to 4.2 ms with one infinity, whose tiles are done again.
+// hundreds of times as long.  A row that its own inputs make so is left as it
+// is, where that is certain, so that an overflowed step, an ordinary one under
+// loss scaling, costs about what others do.  They make all of it NaN if a score
+// is NaN or plus infinity, and a column not finite if a visible value is not,
+// NaN for a NaN and an infinity for an infinity.  Forward and back of 2048 causal
+// rows, 4 heads of 64, bf16, take 90 us, 105 with NaN all over, and 1.4 to 4.2 ms
+// with one infinity, whose tiles are done again.
 // ---------------------------------------------------------------------------
 
 __device__ __forceinline__ uint32_t wave_or(uint32_t x, int from, int to) {
@@ -767,9 +773,8 @@ template <int DP> struct Columns {
 template <typename T, int DP, typename S>
 __device__ __forceinline__ void look_for(const Columns<DP>& need, const View& x, int b, int h,
                                          int first, int end, int d, S sees, Columns<DP>& seen) {
-    constexpr int PER = 16 / sizeof(T), VECS = DP / PER;
-    constexpr int CHUNKS = VECS <= 4 ? 4 : VECS <= 8 ? 8 : VECS <= 16 ? 16 : 32;  // of a row
-    typedef T Vec __attribute__((ext_vector_type(PER)));
+    constexpr int PER = Chunk<T, DP>::PER, CHUNKS = Chunk<T, DP>::CHUNKS;
+    typedef typename Chunk<T, DP>::Vec Vec;
     const int lane = threadIdx.x & 63, c = (lane % CHUNKS) * PER, y = lane / CHUNKS;
     auto part = [&](const uint32_t* words) {  // this lane's columns
         uint32_t w = 0;
@@ -845,6 +850,94 @@ __device__ __forceinline__ uint32_t unexplained(const Args& a, const View& x, in
         again |= group & (uint32_t)__ballot(mine && !fine);
     });
     return again;
+}
+
+// those of the rows j0 + n, n a bit of `rows`, that hold a value that is not finite
+template <typename T, int DP>
+__device__ __forceinline__ uint64_t not_finite(const View& x, int b, int h, int j0, uint64_t rows,
+                                               int d) {
+    constexpr int PER = Chunk<T, DP>::PER, CHUNKS = Chunk<T, DP>::CHUNKS, EACH = 64 / CHUNKS;
+    typedef typename Chunk<T, DP>::Vec Vec;
+    const int lane = threadIdx.x & 63, c = (lane % CHUNKS) * PER;
+    uint64_t bad = 0;
+#pragma unroll 4
+    for (int n = 0; n < CHUNKS; ++n) {
+        const int r = n * EACH + lane / CHUNKS;
+        bool fine = true;
+        if ((rows >> r & 1) && c < d) {
+            const Vec v = *(const Vec*)(row<T>(x, b, j0 + r, h) + c);
+#pragma unroll
+            for (int e = 0; e < PER; ++e) fine &= fabsf((float)v[e]) < INFINITY;
+        }
+        const uint64_t found = __ballot(!fine);
+        for (int y = 0; y < EACH; ++y)
+            if (found >> (y * CHUNKS) & ((1ull << CHUNKS) - 1)) bad |= 1ull << (n * EACH + y);
+    }
+    return bad;
+}
+
+// Calls f for blocks of 64 keys, from j0 on and a bit each, that all of some of
+// the wave's queries see: those of document `of` (not negative) up to position
+// `last` if rows are causal; until f returns true.
+template <typename F>
+__device__ __forceinline__ void for_keys(const Args& a, int b, int of, int last, F f) {
+    const int lane = threadIdx.x & 63, end = a.causal ? last + 1 : a.sk;
+    const int* doc_row = a.documents ? a.documents + b * a.documents_sb : nullptr;
+    for (int j0 = 0; j0 < end; j0 += 64) {
+        const int j = j0 + lane;
+        const uint64_t keys = __ballot(j < end && (!doc_row || doc_row[j] == of));
+        if (keys && f(j0, keys)) return;
+    }
+}
+
+// Those of the wave's queries `rows`, i the lane's, that have a score of NaN or
+// plus infinity with a key that is not finite, or by not being finite themselves.
+template <typename T, int DP>
+__device__ __forceinline__ uint32_t nan_scores(const Args& a, int b, int h, int i, uint32_t rows,
+                                               int doc, int pos) {
+    typedef typename Chunk<T, DP>::Vec Vec;
+    const int g = h / (a.hq / a.hkv);
+    const bool there = rows >> (threadIdx.x & 31) & 1;
+    const T* q = row<T>(a.q, b, there ? i : 0, h);
+    bool fine = true;
+    for (int c = 0; c < a.d && there; c += Chunk<T, DP>::PER) {
+        const Vec v = *(const Vec*)(q + c);
+#pragma unroll
+        for (int e = 0; e < Chunk<T, DP>::PER; ++e) fine &= fabsf((float)v[e]) < INFINITY;
+    }
+    uint32_t found = 0;
+    for_documents(rows, doc, [&](int of, bool mine, uint32_t group) {
+        if (of < 0) return;
+        uint32_t left = group;
+        for_keys(a, b, of, __shfl(pos, __builtin_ctz(group)), [&](int j0, uint64_t keys) {
+            if (!(left & (uint32_t)__ballot(!fine)))
+                keys = not_finite<T, DP>(a.k, b, g, j0, keys, a.d);
+            for (; keys && left; keys &= keys - 1) {
+                const T* k = row<T>(a.k, b, j0 + __builtin_ctzll(keys), g);
+                const float x = mine ? dot(q, k, a.d) * (a.scale * LOG2E) : 0.f;
+                left &= ~(uint32_t)__ballot(!(x < INFINITY));
+            }
+            return left == 0;
+        });
+        found |= group & ~left;
+    });
+    return found;
+}
+
+// Those of the wave's queries `rows` that see a row of V that is not finite.
+template <typename T, int DP>
+__device__ __forceinline__ uint32_t see_not_finite(const Args& a, int b, int g, uint32_t rows,
+                                                   int doc, int pos) {
+    uint32_t found = 0;
+    for_documents(rows, doc, [&](int of, bool, uint32_t group) {
+        if (of < 0) return;
+        for_keys(a, b, of, __shfl(pos, __builtin_ctz(group)), [&](int j0, uint64_t keys) {
+            if (!not_finite<T, DP>(a.v, b, g, j0, keys, a.d)) return false;
+            found |= group;
+            return true;
+        });
+    });
+    return found;
 }
 
 // four values of a row, as they lie in a result's registers
@@ -979,10 +1072,11 @@ void forward_kernel(const Args a, const Ranges keys, const Ranges queries, int t
     if (__any(there && !f.finite())) {
         Columns<DP> lost;
         lost.of(f.o, a.d);
-        // a NaN sum is one of scores, which makes all of the row NaN
         const uint32_t rows = (uint32_t)__ballot(there && total == total && lost.any());
-        for (uint32_t again = unexplained<T, DP>(a, a.v, b, g, rows, f.doc, f.pos, false, lost);
-             again; again &= again - 1)
+        const uint32_t nan = (uint32_t)__ballot(there && total != total);
+        uint32_t again = unexplained<T, DP>(a, a.v, b, g, rows, f.doc, f.pos, false, lost);
+        if (nan) again |= nan & ~nan_scores<T, DP>(a, b, h, i, nan, f.doc, f.pos);
+        for (; again; again &= again - 1)
             forward_row<T, DP>(a, b, h, row0 + __builtin_ctz(again));
     }
 }
@@ -1170,10 +1264,14 @@ __global__ __launch_bounds__(256, 6) void join_kernel(const Args a, int parts, c
     Columns<DP> need;
 #pragma unroll
     for (int n = 0; n < DP / 32; ++n) need.nan[n] = lost[0][n], need.inf[n] = lost[1][n];
-    if (!need.any() || total != total) return;
+    if (!need.any()) return;
     const int pos = i + a.sk - a.sq, end = a.causal ? pos + 1 : a.sk;
     const int* doc_row = a.documents ? a.documents + b * a.documents_sb : nullptr;
     const int doc = doc_row ? doc_row[pos] : 0, each = (end + 255) / 256 * 64;
+    if (total != total) {
+        if (wave == 0 && !nan_scores<T, DP>(a, b, h, i, 1, doc, pos)) forward_row<T, DP>(a, b, h, i);
+        return;
+    }
     Columns<DP> seen;
     look_for<T, DP>(need, a.v, b, g, min(wave * each, end), min((wave + 1) * each, end), a.d,
                     [&](int j) { return !doc_row || doc_row[j] == doc; }, seen);
@@ -1491,19 +1589,25 @@ void dq_kernel(const Args a, const Ranges keys, const Ranges queries, int tiles_
     if (__any(there && !fine)) {
         Columns<DP> lost;
         lost.of(acc, a.d);
-        // a row with a visible NaN among its scores, or one of whose output or
-        // its gradient is not finite, is NaN
-        bool given = true;
+        // a row is NaN if a score is, if its output's gradient is not finite or
+        // if a visible row of V is not, as its output then shows
+        bool dout_fine = true, out_fine = true;
 #pragma unroll
         for (int n = 0; n < DP / 16; ++n) {
             const Frag<T> o =
                 row_frag<T>(row<T>(a.out, b, there ? i : 0, h), n * 16 + hf * 8, a.d, there);
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-                given &= fabsf((float)o[e]) < INFINITY && fabsf((float)dout[n][e]) < INFINITY;
+            for (int e = 0; e < 8; ++e) {
+                out_fine &= fabsf((float)o[e]) < INFINITY;
+                dout_fine &= fabsf((float)dout[n][e]) < INFINITY;
+            }
         }
-        given = !wave_or(!given, 32, 64);
-        const bool stands = lost.all_nan(a.d) && (off != off || (off != INFINITY && !given));
+        out_fine = !wave_or(!out_fine, 32, 64);
+        dout_fine = !wave_or(!dout_fine, 32, 64);
+        bool stands = there && lost.all_nan(a.d) && off != INFINITY;
+        const uint32_t by_v = (uint32_t)__ballot(stands && off == off && dout_fine && !out_fine);
+        stands = stands && (off != off || !dout_fine ||
+                            (see_not_finite<T, DP>(a, b, g, by_v, doc, pos) >> (lane & 31) & 1));
         const bool sum = fabsf(rest) <= 3.4028235e38f;
         const bool nothing = off == INFINITY;  // seen: its gradient is 0
         uint32_t again = (uint32_t)__ballot(there && !stands && (!sum || nothing));
