@@ -538,12 +538,15 @@ __device__ __forceinline__ int causal_order(int n, int tiles, int head, bool alt
     return alternate && (head & 1) ? n : tiles - 1 - n;
 }
 
-// Waves a SIMD that the registers are shared out for: 2, or 1 where two would
+// Waves a SIMD that the registers are shared out for: 2, 3 where they do for as
+// many (the forward of heads of 64 and blocks of 4 waves), or 1 where two would
 // spill (to 256 registers; 3 spill in the backward of heads of 64: dq 133 us for
 // 72 on packed rows of 512).
 template <typename T, int DP, int SHARES>
 constexpr int forward_waves =
-    (DP >= 96 && SHARES > 1) || (DP == 128 && sizeof(T) == 4) || SHARES == 4 ? 1 : 2;
+    (DP >= 96 && SHARES > 1) || (DP == 128 && sizeof(T) == 4) || SHARES == 4 ? 1
+    : sizeof(T) == 2 && DP <= 64 && SHARES == 1                              ? 3
+                                                                             : 2;
 template <int DP, int SHARES> constexpr int dq_waves = DP >= 96 || SHARES > 1 ? 1 : 2;
 template <typename T, int DP, int SHARES>
 constexpr int dkv_waves = DP >= 96 || (DP == 64 && sizeof(T) == 4) || SHARES == 4 ? 1 : 2;
@@ -551,6 +554,11 @@ constexpr int dkv_waves = DP >= 96 || (DP == 64 && sizeof(T) == 4) || SHARES == 
 constexpr float HEADROOM = 3.f;  // how far (log2) a score may pass the reference maximum
 constexpr float SHIFT = 12.f;    // probabilities carry a factor 2^12, at most 2^15 in all:
                                  // in fp16 the small ones keep their bits
+
+// Scores (log2) that 32 bits hold to less than about 1: a probability that a
+// product formed with them, and not its rounded score, could be anything.  Rows
+// with such a maximum are formed pair by pair.
+constexpr float FAR = 0x1p22f;
 
 // x = -inf for the rows of other documents, of sub-tile t of 32 rows; docs of a
 // tile's rows, with -1 behind the last
@@ -655,7 +663,10 @@ template <typename T, int DP> struct Forward {
             for (int i = 0; i < 16; i += 2) most = fmaxf(most, fmaxf(s[t][i], s[t][i + 1]));
         most = max_halves(most);
         if (__any(most > (fresh ? -INFINITY : SHIFT + HEADROOM))) {
-            float by = fresh ? most == -INFINITY ? 0.f : most - SHIFT : fmaxf(most - SHIFT, 0.f);
+            // keys far below others to come, and rows of such keys alone, whose sum
+            // will be 0, do not set the reference
+            float by = fresh ? most == -INFINITY ? 0.f : fmaxf(most - SHIFT, -FAR)
+                             : fmaxf(most - SHIFT, 0.f);
             const float next = off + by;
             by = next - off;  // as far as off really went
             const float keep = fresh ? 1.f : exp2_fast(-by);
@@ -682,6 +693,13 @@ template <typename T, int DP> struct Forward {
             add_product<T, DP>(v, t * 32, s[t], o);
         }
         total += sum;
+    }
+
+    // the sum of both halves, NaN if the row is to be formed pair by pair; the
+    // reference maximum has only grown
+    __device__ __forceinline__ float sum() const {
+        const float x = add_halves(total);
+        return off > FAR ? __builtin_nanf("") : x;
     }
 
     __device__ __forceinline__ bool finite() const {
@@ -1031,7 +1049,7 @@ void forward_kernel(const Args a, const Ranges keys, const Ranges queries, int t
         }
     }
 
-    float total = add_halves(f.total);
+    float total = f.sum();
     if constexpr (SHARES > 1) {
         float* box = shared.boxes + wave * BOX;
         __syncthreads();
@@ -1069,12 +1087,14 @@ void forward_kernel(const Args a, const Ranges keys, const Ranges queries, int t
             a.lse[((int64_t)b * a.hq + h) * a.sq + i] =
                 total == 0.f ? -INFINITY : f.off + log2f(total);
     }
-    if (__any(there && !f.finite())) {
+    const bool none = total == 0.f && f.doc >= 0;  // though a query sees itself
+    if (__any(there && (!f.finite() || total != total || none))) {
         Columns<DP> lost;
         lost.of(f.o, a.d);
-        const uint32_t rows = (uint32_t)__ballot(there && total == total && lost.any());
+        const uint32_t rows = (uint32_t)__ballot(there && total == total && !none && lost.any());
         const uint32_t nan = (uint32_t)__ballot(there && total != total);
-        uint32_t again = unexplained<T, DP>(a, a.v, b, g, rows, f.doc, f.pos, false, lost);
+        uint32_t again = (uint32_t)__ballot(there && none);
+        again |= unexplained<T, DP>(a, a.v, b, g, rows, f.doc, f.pos, false, lost);
         if (nan) again |= nan & ~nan_scores<T, DP>(a, b, h, i, nan, f.doc, f.pos);
         for (; again; again &= again - 1)
             forward_row<T, DP>(a, b, h, row0 + __builtin_ctz(again));
@@ -1184,7 +1204,7 @@ void split_kernel(const Args a, int parts, int keys_each, int column_tiles, floa
         }
     }
 
-    const float total = add_halves(f.total);
+    const float total = f.sum();
     if (!there) return;
     const int64_t at = (((int64_t)b * a.hkv + g) * columns + column) * parts + part;
 #pragma unroll
@@ -1264,10 +1284,14 @@ __global__ __launch_bounds__(256, 6) void join_kernel(const Args a, int parts, c
     Columns<DP> need;
 #pragma unroll
     for (int n = 0; n < DP / 32; ++n) need.nan[n] = lost[0][n], need.inf[n] = lost[1][n];
-    if (!need.any()) return;
+    if (!need.any() && total != 0.f) return;
     const int pos = i + a.sk - a.sq, end = a.causal ? pos + 1 : a.sk;
     const int* doc_row = a.documents ? a.documents + b * a.documents_sb : nullptr;
     const int doc = doc_row ? doc_row[pos] : 0, each = (end + 255) / 256 * 64;
+    if (total == 0.f) {
+        if (wave == 0 && doc >= 0) forward_row<T, DP>(a, b, h, i);
+        return;
+    }
     if (total != total) {
         if (wave == 0 && !nan_scores<T, DP>(a, b, h, i, 1, doc, pos)) forward_row<T, DP>(a, b, h, i);
         return;
@@ -1399,8 +1423,11 @@ template <typename T> constexpr bool FACTORED = std::is_same<T, _Float16>::value
 // how much: dq is set right with the sum of P k, and dk takes the right delta.
 template <typename T> constexpr bool CORRECTED = sizeof(T) == 2;
 
-// rows that saw nothing have probabilities of zero
-__device__ __forceinline__ float usable(float lse) { return lse == -INFINITY ? INFINITY : lse; }
+// Rows that saw nothing have probabilities of zero; those of far scores are made
+// NaN, so that what they enter is formed pair by pair.
+__device__ __forceinline__ float usable(float lse) {
+    return lse == -INFINITY ? INFINITY : fabsf(lse) > FAR ? __builtin_nanf("") : lse;
+}
 
 template <typename T, int DP, int ROWS, int SHARES>
 __global__ __launch_bounds__(ROWS * SHARES * 64, (dq_waves<DP, SHARES>))
@@ -1604,15 +1631,17 @@ void dq_kernel(const Args a, const Ranges keys, const Ranges queries, int tiles_
         }
         out_fine = !wave_or(!out_fine, 32, 64);
         dout_fine = !wave_or(!dout_fine, 32, 64);
-        bool stands = there && lost.all_nan(a.d) && off != INFINITY;
-        const uint32_t by_v = (uint32_t)__ballot(stands && off == off && dout_fine && !out_fine);
-        stands = stands && (off != off || !dout_fine ||
+        const float lse = there ? a.lse[at_row] : 0.f;
+        // no key seen, whose gradient is 0, or far scores
+        const bool apart = fabsf(lse) > FAR;
+        bool stands = there && lost.all_nan(a.d) && !apart;
+        const uint32_t by_v = (uint32_t)__ballot(stands && lse == lse && dout_fine && !out_fine);
+        stands = stands && (lse != lse || !dout_fine ||
                             (see_not_finite<T, DP>(a, b, g, by_v, doc, pos) >> (lane & 31) & 1));
         const bool sum = fabsf(rest) <= 3.4028235e38f;
-        const bool nothing = off == INFINITY;  // seen: its gradient is 0
-        uint32_t again = (uint32_t)__ballot(there && !stands && (!sum || nothing));
+        uint32_t again = (uint32_t)__ballot(there && !stands && (!sum || apart));
         again |= unexplained<T, DP>(
-            a, a.k, b, g, (uint32_t)__ballot(there && !stands && sum && !nothing && lost.any()),
+            a, a.k, b, g, (uint32_t)__ballot(there && !stands && sum && !apart && lost.any()),
             doc, pos, true, lost);
         for (; again; again &= again - 1) dq_row<T, DP>(a, b, h, row0 + __builtin_ctz(again));
     }

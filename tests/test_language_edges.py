@@ -451,3 +451,60 @@ def test_large_batches(dtype, shape, docs):
                     # both off by their roundings: of P or dS, and of the result
                     tol = 4 * (half_step(dtype) + 256 * E) * w.abs().max()
                     assert (g[one].double() - w.double()).abs().max() <= tol, f"{name} of {e}"
+
+
+# --------------------------------------------------------------------------
+# scores beyond what 32 bits hold to 1
+# --------------------------------------------------------------------------
+
+@pytest.mark.parametrize("device", BOTH)
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("size", ["large", "one", "negative"])
+@pytest.mark.parametrize("shape", [(1, 1, 1, 1, 1, 8), (2, 70, 70, 4, 2, 64),
+                                   (1, 2, 900, 4, 1, 128), (1, 300, 333, 2, 2, 40)], ids=str)
+def test_far_scores(device, dtype, size, shape):
+    """The one key of the largest score has all of the probability, in every row
+    or in those of one query and one key whose values are large."""
+    b, sq, sk, hq, hkv, d = shape
+    q, k, v, dout = attention_inputs(*shape, dtype, "cpu", seed=sum(shape))
+    if size == "one":
+        q[:, sq // 2] *= 8e3
+        k[:, sk // 3] *= 8e3
+    else:
+        q, k = q.abs() * 6000, k.abs() * 6000
+        if size == "negative":
+            k = -k
+    documents = torch.tensor([pack([sk // 2, sk - sk // 2 - 1], sk)] * b, dtype=torch.int32)
+    documents[:, -1] = 5
+    for causal in (False, True):
+        got = attention_step({n: t.to(device) for n, t in
+                              dict(q=q, k=k, v=v, dout=dout).items()},
+                             documents=documents.to(device), causal=causal)
+        for e in range(b):
+            want = formulas(*[t[e].double() for t in (q, k, v, dout)], documents[e], causal)
+            far = torch.zeros(hq, sq, dtype=torch.bool)
+            seen, _ = seen_pairs(documents[e:e + 1], causal, 1, sq, sk)
+            for h in range(hq):
+                s = d ** -0.5 * (q[e, :, h].double() @ k[e, :, h * hkv // hq].double().T)
+                top = s.masked_fill(~seen[0], -math.inf).amax(1)
+                s2 = s.masked_fill(~seen[0], -math.inf).topk(min(2, sk), 1).values
+                # rows whose two largest scores differ by more than their own
+                # roundings: d products, their sums and the scaling in 32 bits
+                size_of = d ** -0.5 * (q[e, :, h].double().abs()
+                                       @ k[e, :, h * hkv // hq].double().abs().T)
+                off = (d + 4) * E * torch.where(seen[0], size_of, 0.0).amax(1)
+                far[h] = (s2[:, 0] - s2[:, -1] > 2 * off + 200) | (seen[0].sum(1) == 1)
+                far[h] &= top.isfinite()
+            assert far.any() and (size == "one" or far.float().mean() > 0.2)
+            # those rows are one value of V, rounded nowhere
+            rows = far.T
+            tol = 1.01 * half_step(dtype) * want["out"].abs() + 1e-6
+            assert ((got[0][e].double().cpu() - want["out"]).abs() <= tol)[rows].all()
+            if size != "one" and far.all():
+                sums = (sq * hq // hkv + 4) * E
+                for n, name in ((1, "dq"), (2, "dk"), (3, "dv")):
+                    g, w = got[n][e].double().cpu(), want[name]
+                    least = 1e-6 * (1 + w.abs().max())
+                    if name != "dv":  # differences of equal products
+                        least = 1e-4 * d ** -0.5 * max(q.abs().max(), k.abs().max()).item()
+                    assert ((g - w).abs() <= (half_step(dtype) + sums) * w.abs() + least).all(), name
